@@ -42,6 +42,10 @@ extern "C" {
 #define LSPS_ACT_LRELU 1    /* nn.LeakyReLU(slope), common_net.py:252,264               */
 #define LSPS_ACT_TANH  2    /* nn.Tanh, lsps_nets.py:228-229                            */
 
+/* element types of the entry points that take more than one */
+#define LSPS_F32  0
+#define LSPS_BF16 1
+
 int         lsps_version(void);
 const char *lsps_last_error(void);
 /* number of compute units of the current device (used by callers to size split counts) */
@@ -406,6 +410,40 @@ int lsps_adam_step(float *p, const float *g, float *m, float *v,
                    const long *seg_off, const int *seg_len, const float *seg_bc1, const float *seg_bc2s,
                    int nseg, int max_seg_len, float lr, float beta1, float beta2, float eps, float weight_decay,
                    float gscale, void *stream);
+
+/* ---- Muon: orthogonalised momentum updates for weight matrices --------------------------------
+ * (no reference counterpart: the reference steps every parameter with Adam, lsps_trainer.py:26-29)
+ * lsps_newton_schulz: out = the Newton-Schulz iterate of each of `count` contiguous rows x cols matrices (dtype LSPS_F32 or
+ *   LSPS_BF16, out of the same type; may run in place):  X = G / (|G|_F + eps), then `steps` times
+ *   X <- a X + (b A + c A^2) X with A = X X^T on the short side.  Arithmetic is f32-class for either type.  (a, b, c) is
+ *   refused if it takes a value of [0, 1] out of bounds on the way (fixed-point limbs inside).
+ * lsps_muon_step: for every matrix  m <- momentum m + grad_scale g,  G = nesterov ? grad_scale g + momentum m : m,
+ *   p <- p (1 - lr weight_decay) - lr rms sqrt(max(rows, cols)) NS(G).  (A matrix with orthonormal rows or columns has entries
+ *   of root mean square 1 / sqrt(max(rows, cols)): `rms` is the size of a weight's step in units of lr; 0.2 is about Adam's.)
+ *   All matrices go through the same launches; `mats` is host memory and is not read after the call returns.
+ * Neither call allocates, synchronises or keeps anything: both can be captured. */
+typedef struct LspsMuonMatrix {
+  float *p;            /* weights   [rows][cols], updated */
+  const float *g;      /* gradients */
+  float *m;            /* momentum, updated */
+  int rows, cols;
+} LspsMuonMatrix;
+size_t lsps_newton_schulz_workspace_bytes(int count, int rows, int cols, int steps);
+int lsps_newton_schulz(const void *g, void *out, int count, int rows, int cols, int dtype, int steps, float a, float b, float c,
+                       float eps, void *ws, size_t ws_bytes, void *stream);
+size_t lsps_muon_workspace_bytes(const LspsMuonMatrix *mats, int n, int steps);
+int lsps_muon_step(const LspsMuonMatrix *mats, int n, float lr, float momentum, int nesterov, float weight_decay, float rms,
+                   float grad_scale, int steps, float a, float b, float c, float eps, void *ws, size_t ws_bytes, void *stream);
+
+/* ---- LayerNorm over the last dimension (nn.LayerNorm; no reference counterpart: its nets use Instance- and BatchNorm) ----
+ * x: `rows` rows of `cols` elements (dtype LSPS_F32 or LSPS_BF16) with a pitch of `ldx` elements between rows; y and dx have the
+ * same type, contiguous; gamma / beta (nullable), the statistics mean[rows] / rstd[rows] saved for the backward and the gradients
+ * dgamma / dbeta (nullable, overwritten) are float32.  dx nullable.  The same inputs give the same bits (no atomics). */
+size_t lsps_layernorm_workspace_bytes(long rows, long cols, int dtype);
+int lsps_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, long rows, long cols,
+                       long ldx, int dtype, float eps, void *ws, size_t ws_bytes, void *stream);
+int lsps_layernorm_bwd(const void *dy, const void *x, const float *mean, const float *rstd, const float *gamma, void *dx, float *dgamma,
+                       float *dbeta, long rows, long cols, long ldx, long lddy, int dtype, void *ws, size_t ws_bytes, void *stream);
 
 /* ---- BatchNorm (nn.BatchNorm2d / nn.BatchNorm1d of the BN block variants of common_net.py:183-322; not instantiated by
  * the shipped configs) [+ LeakyReLU].  x, y: [N][C][HW] (HW = 1 for BatchNorm1d).  training != 0: batch statistics

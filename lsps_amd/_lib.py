@@ -18,6 +18,12 @@ class LspsOptions(ctypes.Structure):
                 ('chwn_group', c_int), ('c8w_queue', c_int), ('c8_stem_bf16', c_int), ('x3_plan', c_int), ('x3_ring', c_int)]
 
 
+class LspsMuonMatrix(ctypes.Structure):
+    """include/lsps_hip.h: struct LspsMuonMatrix (one weight matrix of a Muon step; device pointers)."""
+    _fields_ = [('p', c_void_p), ('g', c_void_p), ('m', c_void_p), ('rows', c_int), ('cols', c_int)]
+
+
+F32, BF16 = 0, 1                                # element types (LSPS_F32, LSPS_BF16)
 ACT_NONE, ACT_LRELU, ACT_TANH, ACT_SOFTPLUS = 0, 1, 2, 3
 LOSS_L1, LOSS_L2, LOSS_SQ, LOSS_KLSD = 0, 1, 2, 3
 
@@ -69,6 +75,14 @@ _SIGNATURES = {
     'lsps_linear_fwd': (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, _P]),
     'lsps_linear_bwd': (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, _P, _P]),
     'lsps_adam_step': (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int] + [c_float] * 6 + [_P]),
+    'lsps_newton_schulz_workspace_bytes': (c_size_t, [c_int] * 4),
+    'lsps_newton_schulz': (c_int, [_P, _P] + [c_int] * 5 + [c_float] * 4 + [_P, c_size_t, _P]),
+    'lsps_muon_workspace_bytes': (c_size_t, [ctypes.POINTER(LspsMuonMatrix), c_int, c_int]),
+    'lsps_muon_step': (c_int, [ctypes.POINTER(LspsMuonMatrix), c_int, c_float, c_float, c_int, c_float, c_float, c_float, c_int] +
+                       [c_float] * 4 + [_P, c_size_t, _P]),
+    'lsps_layernorm_workspace_bytes': (c_size_t, [c_long, c_long, c_int]),
+    'lsps_layernorm_fwd': (c_int, [_P] * 6 + [c_long] * 3 + [c_int, c_float, _P, c_size_t, _P]),
+    'lsps_layernorm_bwd': (c_int, [_P] * 8 + [c_long] * 4 + [c_int, _P, c_size_t, _P]),
     'lsps_axpy': (c_int, [_P, _P, c_float, _P, c_long, _P]),
     'lsps_bnorm_workspace_bytes': (c_size_t, [c_int]),
     'lsps_bnorm_fwd': (c_int, [_P] * 8 + [c_int] * 4 + [c_float] * 3 + [_P, c_size_t, _P]),

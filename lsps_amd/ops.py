@@ -1706,6 +1706,190 @@ def act(x, kind, slope=0.0):
 
 
 # ------------------------------------------------------------------------------------------
+# layer normalisation; orthogonalised updates
+# ------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _on_device(what, t, *others):
+    """(context that makes the tensors' device the current one, its current stream).  The launch goes to the stream that is
+    current on the tensors' own device, whichever device the caller has made current."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        _lib.ptr(t)                                    # raises: no CPU fallback
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise _lib.LspsHipError("%s: tensors on %s and %s" % (what, t.device, o.device))
+    return torch.cuda.device(t.device), torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _scratch(nbytes, device):
+    """Scratch memory of one call, from torch's allocator: calls on two streams and two captured graphs get buffers of their own
+    (a captured one belongs to its graph's pool)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _ws(buf):
+    return (None, 0) if buf is None else (buf.data_ptr(), buf.numel())
+
+
+def _rows(t, rows, cols):
+    """`t` as rows of `cols` neighbouring elements at one pitch: (tensor, pitch).  Copies only what has no such form."""
+    try:
+        v = t.view(rows, cols)
+    except RuntimeError:
+        v = None
+    if v is None or (cols > 1 and v.stride(1) != 1) or (rows > 1 and v.stride(0) < cols):
+        v = t.contiguous().view(rows, cols)
+    return v, (v.stride(0) if rows > 1 else cols)
+
+
+class _LayerNormFn(torch.autograd.Function):
+    """nn.LayerNorm.  The statistics are saved, the normalised values are formed again in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, cols, eps):
+        L = _lib.lib()
+        rows = x.numel() // cols
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        xr = x
+        if rows:
+            w, b = (None if t is None else _c(t) for t in (w, b))
+            dev, st = _on_device('layer_norm', x, w, b)
+            xr, ldx = _rows(x, rows, cols)
+            dt = _DTYPES[x.dtype]
+            ws = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x.device) if cols > 16384 else None   # (the register variants need none)
+            with dev:
+                _lib.check(L.lsps_layernorm_fwd(xr.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                                rows, cols, ldx, dt, eps, *_ws(ws), st), 'layernorm_fwd')
+        ctx.cols, ctx.bshape = cols, None if b is None else b.shape
+        ctx.save_for_backward(x if xr.data_ptr() == x.data_ptr() else xr, w, mean, rstd)
+        ctx.xshape = x.shape
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        L = _lib.lib()
+        x, w, mean, rstd = ctx.saved_tensors
+        cols, rows = ctx.cols, mean.numel()
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(ctx.xshape, dtype=x.dtype, device=x.device) if need_x else None
+        alloc = torch.empty if rows else torch.zeros
+        dw = alloc(w.shape, dtype=torch.float32, device=x.device) if need_w else None
+        db = alloc(ctx.bshape, dtype=torch.float32, device=x.device) if need_b else None
+        if rows and (need_x or need_w or need_b):
+            xr, ldx = _rows(x, rows, cols)
+            gr, ldg = _rows(dy, rows, cols)
+            dev, st = _on_device('layer_norm', x, dy)
+            dt = _DTYPES[x.dtype]
+            ws = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x.device)
+            with dev:
+                _lib.check(L.lsps_layernorm_bwd(gr.data_ptr(), xr.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _lib.ptr(w),
+                                                None if dx is None else dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), rows, cols, ldx, ldg,
+                                                dt, *_ws(ws), st), 'layernorm_bwd')
+        return dx, dw, db, None, None
+
+
+def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
+    """nn.functional.layer_norm on the HIP kernels (csrc/layernorm.hip): `x` float32 or bfloat16 [..., *normalized_shape], `weight` and
+    `bias` float32 of `normalized_shape` or None.  Statistics and parameter gradients are float32; differentiable once.  Rows that lie
+    at a pitch (a slice of wider rows) are read where they are."""
+    shape = (int(normalized_shape),) if isinstance(normalized_shape, int) else tuple(int(n) for n in normalized_shape)
+    if not shape or tuple(x.shape[x.dim() - len(shape):]) != shape or min(shape) < 1:
+        raise _lib.LspsHipError("layer_norm: normalized_shape %s does not end the shape %s" % (shape, tuple(x.shape)))
+    if x.dtype not in _DTYPES:
+        raise _lib.LspsHipError("layer_norm: float32 or bfloat16 input expected, not %s" % x.dtype)
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32):
+            raise _lib.LspsHipError("layer_norm: %s of shape %s, %s (expected %s, float32)" % (name, tuple(t.shape), t.dtype, shape))
+    _on_device('layer_norm', x, weight, bias)
+    cols = 1
+    for n in shape:
+        cols *= n
+    return _LayerNormFn.apply(x, weight, bias, cols, float(eps))
+
+
+NS_COEFFS = (3.4445, -4.7750, 2.0315)     # quintic whose iterates send (0, 1] near 1 within five steps (the usual choice with Muon)
+
+
+def _coeffs(coeffs):
+    a, b, c = (float(v) for v in coeffs)
+    return a, b, c
+
+
+@torch.no_grad()
+def _newton_schulz(g, steps, coeffs, eps):
+    L = _lib.lib()
+    dev, st = _on_device('newton_schulz', g)
+    out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    if g.numel() == 0:
+        return out
+    g = _c(g)
+    rows, cols = g.shape[-2:]
+    count = g.numel() // (rows * cols)
+    ws = _scratch(L.lsps_newton_schulz_workspace_bytes(count, rows, cols, steps), g.device)
+    with dev:
+        _lib.check(L.lsps_newton_schulz(g.data_ptr(), out.data_ptr(), count, rows, cols, _DTYPES[g.dtype], steps, *coeffs, eps, *_ws(ws),
+                                        st), 'newton_schulz')
+    return out
+
+
+def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+    """Newton-Schulz iterate of the matrices [..., rows, cols] of `g` (float32 or bfloat16; the same type comes back): singular vectors
+    kept, singular values driven towards 1 (csrc/orthogonal.hip).  X = G / (|G|_F + eps), then `steps` times
+    X <- a X + (b A + c A^2) X, A = X X^T on the shorter side.  Float32-class arithmetic for either type.  No backward pass."""
+    if not isinstance(g, torch.Tensor) or g.dim() < 2:
+        raise _lib.LspsHipError("newton_schulz: matrices [..., rows, cols] expected")
+    if g.dtype not in _DTYPES:
+        raise _lib.LspsHipError("newton_schulz: float32 or bfloat16 expected, not %s" % g.dtype)
+    if g.requires_grad and torch.is_grad_enabled():
+        raise _lib.LspsHipError("newton_schulz has no backward pass: call it under torch.no_grad() or on a detached tensor")
+    return _newton_schulz(g, int(steps), _coeffs(coeffs), float(eps))
+
+
+def _disjoint(what, written, read):
+    """Refuses memory that one call would both write and use twice."""
+    spans = sorted([(t.data_ptr(), t.data_ptr() + 4 * t.numel(), True) for t in written] +
+                   [(t.data_ptr(), t.data_ptr() + 4 * t.numel(), False) for t in read])
+    end, end_written = 0, 0
+    for lo, hi, w in spans:
+        if lo < end_written or (w and lo < end):
+            raise _lib.LspsHipError("%s: tensors overlap" % what)
+        end = max(end, hi)
+        if w:
+            end_written = max(end_written, hi)
+
+
+def muon_step_(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, rms=0.2, grad_scale=1.0, steps=5,
+               coeffs=NS_COEFFS, eps=1e-7):
+    """One Muon step over lists of weights, gradients and momentum buffers (float32, contiguous, equal shapes), in place, all matrices
+    through the same launches.  A tensor of more than two dimensions is a matrix (shape[0], rest).  For every matrix
+    m <- momentum m + grad_scale g, G = nesterov ? grad_scale g + momentum m : m,
+    p <- p (1 - lr weight_decay) - lr rms sqrt(max(rows, cols)) newton_schulz(G).  (optim.FlatMuon: the optimizer around it.)"""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not (len(params) == len(grads) == len(momenta)):
+        raise _lib.LspsHipError("muon_step_: %d weights, %d gradients, %d momenta" % (len(params), len(grads), len(momenta)))
+    for p, g, m in zip(params, grads, momenta):
+        if p.dim() < 2 or p.shape != g.shape or p.shape != m.shape or p.numel() == 0:
+            raise _lib.LspsHipError("muon_step_: weight %s, gradient %s, momentum %s" % (tuple(p.shape), tuple(g.shape), tuple(m.shape)))
+    if not params:
+        return
+    L = _lib.lib()
+    dev, st = _on_device('muon_step_', params[0], *(params + grads + momenta))
+    mats = (_lib.LspsMuonMatrix * len(params))()
+    for k, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        mats[k] = _lib.LspsMuonMatrix(_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), p.shape[0], p.numel() // p.shape[0])
+    _disjoint('muon_step_', params + momenta, grads)
+    ws = _scratch(L.lsps_muon_workspace_bytes(mats, len(params), int(steps)), params[0].device)
+    with dev:
+        _lib.check(L.lsps_muon_step(mats, len(params), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(rms),
+                                    float(grad_scale), int(steps), *_coeffs(coeffs), float(eps), *_ws(ws), st), 'muon_step')
+    torch.autograd.graph.increment_version(params + momenta)       # written behind torch's back
+
+
+# ------------------------------------------------------------------------------------------
 # scoped cache of packed weight panels (lsps_pack_cache_begin / _end)
 # ------------------------------------------------------------------------------------------
 _pack_arenas = {}

@@ -19,7 +19,7 @@ import math
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, ops
 
 
 class FlatArena(object):
@@ -147,6 +147,10 @@ class FlatAdam(torch.optim.Optimizer):
         for p, t in zip(params, steps.tolist()):
             self.state[p]['step'] = int(t)
 
+    def _by_adam(self, p):
+        """Does `step` pass this parameter to lsps_adam_step?  (FlatMuon: not the matrices.)"""
+        return True
+
     @torch.no_grad()
     def step(self, closure=None):
         if self.arena is None:
@@ -164,7 +168,7 @@ class FlatAdam(torch.optim.Optimizer):
         lens = self._seg_len_host
         host = self._host
         for i, p in enumerate(params):
-            if a.touched[i]:
+            if a.touched[i] and self._by_adam(p):
                 st = self.state[p]
                 st['step'] = int(st['step']) + 1
                 t = st['step']
@@ -215,3 +219,80 @@ class FlatAdam(torch.optim.Optimizer):
                     view.copy_(st[key])
                 st[key] = view
             st['step'] = int(st['step'].item()) if torch.is_tensor(st.get('step')) else int(st.get('step', 0))
+
+
+class FlatMuon(FlatAdam):
+    """Muon over a FlatArena: weight matrices (conv weights as (out, in * taps)) take an orthogonalised momentum step, all of them in
+    one lsps_muon_step call; what has no two directions of more than one element (biases, gains, a one-row head) takes Adam as in
+    FlatAdam, from the same buffers (a matrix' momentum lives where exp_avg would; exp_avg_sq is not used for it).
+
+    `lr`, `betas`, `eps`: as FlatAdam (`eps`: Adam's).  A matrix moves by lr * rms in the root mean square of its entries, so `rms` = 0.2 suits
+    learning rates found for Adam.  `weight_decay` is coupled for the Adam part (FlatAdam's) and decoupled for matrices
+    (p *= 1 - lr * weight_decay): a term added to the gradient would lose its size in the orthogonalisation."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, momentum=0.95, nesterov=True, rms=0.2,
+                 ns_steps=5, ns_coeffs=ops.NS_COEFFS, ns_eps=1e-7):
+        super(FlatMuon, self).__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+        more = dict(momentum=momentum, nesterov=nesterov, rms=rms, ns_steps=ns_steps, ns_coeffs=tuple(ns_coeffs), ns_eps=ns_eps)
+        self.defaults.update(more)
+        self.param_groups[0].update(more)
+
+    @staticmethod
+    def is_matrix(p):
+        return p.dim() >= 2 and p.shape[0] > 1 and p.numel() > p.shape[0]
+
+    def _by_adam(self, p):
+        return not self.is_matrix(p)
+
+    def _keep_momentum(self, loaded):
+        """Leaves {step, momentum_buffer} as the state of each matrix; `loaded`: the momenta of a state dict (others start at zero:
+        a first moment of Adam's is no momentum of this one)."""
+        for p, o in zip(self.param_groups[0]['params'], self.arena.offsets):
+            if not self.is_matrix(p):
+                continue
+            st = self.state[p]
+            st.setdefault('step', 0)
+            view = self.flat_m[o:o + p.numel()].view(p.shape)
+            src = loaded.get(p)
+            if src is None:
+                view.zero_()
+            elif src.data_ptr() != view.data_ptr():
+                view.copy_(src)
+            for key in ('exp_avg', 'exp_avg_sq'):
+                st.pop(key, None)
+            st['momentum_buffer'] = view
+
+    def _momenta(self):
+        return dict((p, st['momentum_buffer']) for p, st in self.state.items() if st.get('momentum_buffer') is not None)
+
+    def attach(self):
+        loaded = self._momenta()
+        arena = super(FlatMuon, self).attach()
+        self._keep_momentum(loaded)
+        return arena
+
+    def load_state_dict(self, state_dict):
+        """Accepts a FlatMuon state dict; from a FlatAdam one the vectors' moments are taken and the momenta start at zero."""
+        more = dict((k, v) for k, v in self.param_groups[0].items() if k not in ('params', 'lr', 'betas', 'eps', 'weight_decay'))
+        super(FlatMuon, self).load_state_dict(state_dict)
+        for k, v in more.items():
+            self.param_groups[0].setdefault(k, v)
+        if self.arena is not None:
+            self._keep_momentum(self._momenta())
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        if self.arena is None:
+            raise _lib.LspsHipError("FlatMuon.step(): no arena — call trainer.cuda(gpu) first (no CPU fallback)")
+        g = self.param_groups[0]
+        a = self.arena
+        mats = [i for i, p in enumerate(g['params']) if a.touched[i] and self.is_matrix(p)]
+        if mats:
+            params = [g['params'][i] for i in mats]
+            ops.muon_step_([p.data for p in params], [p.grad for p in params], [self.state[p]['momentum_buffer'] for p in params],
+                           lr=g['lr'], momentum=g['momentum'], nesterov=g['nesterov'], weight_decay=g['weight_decay'], rms=g['rms'],
+                           grad_scale=self.grad_scale, steps=g['ns_steps'], coeffs=g['ns_coeffs'], eps=g['ns_eps'])
+            for p in params:
+                self.state[p]['step'] = int(self.state[p]['step']) + 1
+            a.generation += 1
+        return super(FlatMuon, self).step(closure)

@@ -506,6 +506,33 @@ class LeakyReLUBNLinear(nn.Module):
         return self.model[1](self.model[0](x), LRELU_SLOPE)
 
 
+class LayerNorm(nn.Module):
+    """Parameter holder + launcher for lsps_layernorm_* (torch's nn.LayerNorm: the same state-dict keys, eps 1e-5)."""
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True):
+        super(LayerNorm, self).__init__()
+        self.normalized_shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(self.normalized_shape)) if elementwise_affine else None
+        self.bias = nn.Parameter(torch.zeros(self.normalized_shape)) if elementwise_affine else None
+
+    def forward(self, x):
+        return ops.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
+
+
+class LeakyReLULNLinear(nn.Module):
+    """LReLU(LN(linear(x))): LeakyReLUBNLinear with statistics of the sample instead of the batch (any batch size, the same in
+    training and evaluation)."""
+
+    def __init__(self, n_in, n_out):
+        super(LeakyReLULNLinear, self).__init__()
+        self.model = nn.Sequential(Linear(n_in, n_out), LayerNorm(n_out), _Fused('LeakyReLU'))
+        self.model.apply(gaussian_weights_init)
+
+    def forward(self, x):
+        return ops.act(self.model[1](self.model[0](x)), ACT_LRELU, LRELU_SLOPE)
+
+
 class LeakyReLUBNNSResBlock(nn.Module):
     """x + BN(conv(LReLU(BN(conv(x))))), affine-free BN, convs without bias (common_net.py:183-199)."""
 

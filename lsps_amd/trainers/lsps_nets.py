@@ -10,7 +10,7 @@ import torch.nn as nn
 from .common_net import *  # noqa: F401,F403
 from .common_net import (ACT_LRELU, ACT_NONE, ACT_TANH, Conv2d, ConvTranspose2d, GaussianNoiseLayer,
                          LeakyINSResBlock, LeakyINSResNeXtBlock, LeakyReLUConv2d, LeakyReLUConvTranspose2d,
-                         LeakyReLULinear, Linear, _Fused, run_layers)
+                         LeakyReLULinear, LeakyReLULNLinear, Linear, _Fused, run_layers)
 from .. import ops
 from ..ops import ACT_SOFTPLUS
 
@@ -65,15 +65,22 @@ class Mapping(_Net):
 
 
 class poseVAE(_Net):
-    """Pose MLP: encode 108->50->(20,20) with reparameterisation, decode 20->50->108 (lsps_nets.py:34-83)."""
+    """Pose MLP: encode 108->50->(20,20) with reparameterisation, decode 20->50->108 (lsps_nets.py:34-83).
+    `norm: layer` in its parameters (not in the reference) puts a layer norm in front of both hidden LeakyReLUs."""
 
     def __init__(self, params):
         super(poseVAE, self).__init__()
         self.input_dim, self.z_dim, self.h_dim = params['input_dim'], params['z_dim'], params['h_dim']
-        self.en_fc1 = Linear(self.input_dim, self.h_dim, act=ACT_LRELU)      # + self.lrelu, :74
+        norm = params.get('norm', 'none')
+        if norm not in ('none', 'layer'):
+            raise ValueError("poseVAE: norm %r ('none' or 'layer')" % (norm,))
+        if norm == 'layer':
+            self.en_fc1 = LeakyReLULNLinear(self.input_dim, self.h_dim)
+        else:
+            self.en_fc1 = Linear(self.input_dim, self.h_dim, act=ACT_LRELU)  # + self.lrelu, :74
         self.en_mu = Linear(self.h_dim, self.z_dim)
         self.en_sigma = Linear(self.h_dim, self.z_dim, act=ACT_SOFTPLUS)     # + self.softplus, :76
-        self.de_fc1 = LeakyReLULinear(self.z_dim, self.h_dim)
+        self.de_fc1 = (LeakyReLULNLinear if norm == 'layer' else LeakyReLULinear)(self.z_dim, self.h_dim)
         self.de_fc2 = Linear(self.h_dim, self.input_dim)
         self.preset_parameters()
 

@@ -27,7 +27,7 @@ from .init import *  # noqa: F401,F403
 from .init import gaussian_weights_init
 from .. import dist as lsps_dist
 from .. import ops
-from ..optim import FlatAdam
+from ..optim import FlatAdam, FlatMuon
 
 _NETS = {'Mapping': Mapping, 'poseVAE': poseVAE, 'SharedDis': SharedDis, 'SharedResGen': SharedResGen,
          'SharedResXGen': SharedResXGen}
@@ -201,10 +201,15 @@ class LSPSTrainer(nn.Module):
         self.vae = _net(hyperparameters['vae'])
         self.map = _net(hyperparameters['map'])
         # optimizers / schedulers (lsps_trainer.py:26-34)
-        self.dis_opt = FlatAdam(self.dis.parameters(), lr=lr, betas=(0.5, 0.999), weight_decay=0.0001)
-        self.gen_opt = FlatAdam(list(self.gen.parameters()) + list(self.map.parameters()), lr=lr, betas=(0.5, 0.999),
-                                weight_decay=0.0001)
-        self.vae_opt = FlatAdam(self.vae.parameters(), lr=lr * 10., betas=(0.5, 0.999), weight_decay=0.001)
+        # `optimizer: muon` (not in the reference): weight matrices take orthogonalised updates, vectors stay with Adam
+        name = hyperparameters.get('optimizer', 'adam')
+        if name not in ('adam', 'muon'):
+            raise ValueError("optimizer %r ('adam' or 'muon')" % (name,))
+        Opt = FlatMuon if name == 'muon' else FlatAdam
+        self.dis_opt = Opt(self.dis.parameters(), lr=lr, betas=(0.5, 0.999), weight_decay=0.0001)
+        self.gen_opt = Opt(list(self.gen.parameters()) + list(self.map.parameters()), lr=lr, betas=(0.5, 0.999),
+                           weight_decay=0.0001)
+        self.vae_opt = Opt(self.vae.parameters(), lr=lr * 10., betas=(0.5, 0.999), weight_decay=0.001)
         MS = torch.optim.lr_scheduler.MultiStepLR
         self.dis_sch = MS(self.dis_opt, milestones=[200, 300, 400, 450], gamma=0.5)
         self.gen_sch = MS(self.gen_opt, milestones=[200, 300, 400, 450], gamma=0.5)
