@@ -1711,104 +1711,126 @@ def act(x, kind, slope=0.0):
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
-def _on_device(what, t, *others):
-    """(context that makes the tensors' device the current one, its current stream).  The launch goes to the stream that is
-    current on the tensors' own device, whichever device the caller has made current."""
+def _same_device(what, t, *others):
+    """Device index of `t` (a HIP tensor, or _lib.ptr raises); the other tensors have to be there too."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        _lib.ptr(t)                                    # raises: no CPU fallback
+        _lib.ptr(t)
+    index = t.get_device()
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != index:
             raise _lib.LspsHipError("%s: tensors on %s and %s" % (what, t.device, o.device))
-    return torch.cuda.device(t.device), torch.cuda.current_stream(t.device).cuda_stream
+    return index
 
 
-def _scratch(nbytes, device):
-    """Scratch memory of one call, from torch's allocator: calls on two streams and two captured graphs get buffers of their own
-    (a captured one belongs to its graph's pool)."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+# hipStream_t of a device's current stream: what torch.cuda.current_stream(index).cuda_stream is, without building a Stream object
+# (2.4 us; the small layer norms are bound by such calls)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _ws(buf):
-    return (None, 0) if buf is None else (buf.data_ptr(), buf.numel())
+def _launch(what, index, fn, *args):
+    """fn(*args, stream) on the stream that is current on device `index`, whichever device the caller has made current."""
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _scratch(nbytes, t):
+    """(buffer, pointer, bytes) of one call's scratch memory, from torch's allocator: calls on two streams and two captured graphs
+    get buffers of their own (a captured one belongs to its graph's pool)."""
+    if not nbytes:
+        return None, None, 0
+    buf = t.new_empty(nbytes, dtype=torch.uint8)
+    return buf, buf.data_ptr(), nbytes
 
 
 def _rows(t, rows, cols):
     """`t` as rows of `cols` neighbouring elements at one pitch: (tensor, pitch).  Copies only what has no such form."""
+    if t.is_contiguous():
+        return t, cols
     try:
         v = t.view(rows, cols)
     except RuntimeError:
         v = None
     if v is None or (cols > 1 and v.stride(1) != 1) or (rows > 1 and v.stride(0) < cols):
-        v = t.contiguous().view(rows, cols)
+        return t.contiguous(), cols
     return v, (v.stride(0) if rows > 1 else cols)
+
+
+LN_FWD_COLS = 16384       # rows up to here need no workspace in the forward (csrc/layernorm.hip)
 
 
 class _LayerNormFn(torch.autograd.Function):
     """nn.LayerNorm.  The statistics are saved, the normalised values are formed again in the backward."""
 
     @staticmethod
-    def forward(ctx, x, w, b, cols, eps):
-        L = _lib.lib()
+    def forward(ctx, x, w, b, index, cols, eps):
         rows = x.numel() // cols
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-        xr = x
-        if rows:
-            w, b = (None if t is None else _c(t) for t in (w, b))
-            dev, st = _on_device('layer_norm', x, w, b)
-            xr, ldx = _rows(x, rows, cols)
-            dt = _DTYPES[x.dtype]
-            ws = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x.device) if cols > 16384 else None   # (the register variants need none)
-            with dev:
-                _lib.check(L.lsps_layernorm_fwd(xr.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                                                rows, cols, ldx, dt, eps, *_ws(ws), st), 'layernorm_fwd')
-        ctx.cols, ctx.bshape = cols, None if b is None else b.shape
-        ctx.save_for_backward(x if xr.data_ptr() == x.data_ptr() else xr, w, mean, rstd)
-        ctx.xshape = x.shape
+        y = x.new_empty(x.shape)
+        stats = x.new_empty((2, rows), dtype=torch.float32)
+        ctx.cols = cols
+        if b is not None:
+            ctx.bshape = b.shape
+        if not rows:
+            ctx.save_for_backward(x, w, stats)
+            return y
+        L = _lib.lib()
+        dt = _DTYPES[x.dtype]
+        if w is not None:
+            w = _c(w)
+        if b is not None:
+            b = _c(b)
+        xr, ldx = _rows(x, rows, cols)
+        buf, ws, n = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x) if cols > LN_FWD_COLS else (None, None, 0)
+        sp = stats.data_ptr()
+        _launch('layernorm_fwd', index, L.lsps_layernorm_fwd, xr.data_ptr(), None if w is None else w.data_ptr(),
+                None if b is None else b.data_ptr(), y.data_ptr(), sp, sp + 4 * rows, rows, cols, ldx, dt, eps, ws, n)
+        ctx.save_for_backward(x if xr.data_ptr() == x.data_ptr() else xr, w, stats)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        L = _lib.lib()
-        x, w, mean, rstd = ctx.saved_tensors
-        cols, rows = ctx.cols, mean.numel()
+        x, w, stats = ctx.saved_tensors
+        cols, rows = ctx.cols, stats.shape[1]
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(ctx.xshape, dtype=x.dtype, device=x.device) if need_x else None
-        alloc = torch.empty if rows else torch.zeros
-        dw = alloc(w.shape, dtype=torch.float32, device=x.device) if need_w else None
-        db = alloc(ctx.bshape, dtype=torch.float32, device=x.device) if need_b else None
-        if rows and (need_x or need_w or need_b):
+        dx = dy.new_empty(dy.shape) if need_x else None
+        alloc = stats.new_empty if rows else stats.new_zeros
+        dw = alloc(w.shape) if need_w else None
+        db = alloc(ctx.bshape) if need_b else None
+        if rows:
+            L = _lib.lib()
+            dt = _DTYPES[x.dtype]
             xr, ldx = _rows(x, rows, cols)
             gr, ldg = _rows(dy, rows, cols)
-            dev, st = _on_device('layer_norm', x, dy)
-            dt = _DTYPES[x.dtype]
-            ws = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x.device)
-            with dev:
-                _lib.check(L.lsps_layernorm_bwd(gr.data_ptr(), xr.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _lib.ptr(w),
-                                                None if dx is None else dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), rows, cols, ldx, ldg,
-                                                dt, *_ws(ws), st), 'layernorm_bwd')
-        return dx, dw, db, None, None
+            buf, ws, n = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x)
+            sp = stats.data_ptr()
+            _launch('layernorm_bwd', x.get_device(), L.lsps_layernorm_bwd, gr.data_ptr(), xr.data_ptr(), sp, sp + 4 * rows,
+                    None if w is None else w.data_ptr(), dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                    db.data_ptr() if need_b else None, rows, cols, ldx, ldg, dt, ws, n)
+        return dx, dw, db, None, None, None
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     """nn.functional.layer_norm on the HIP kernels (csrc/layernorm.hip): `x` float32 or bfloat16 [..., *normalized_shape], `weight` and
     `bias` float32 of `normalized_shape` or None.  Statistics and parameter gradients are float32; differentiable once.  Rows that lie
     at a pitch (a slice of wider rows) are read where they are."""
-    shape = (int(normalized_shape),) if isinstance(normalized_shape, int) else tuple(int(n) for n in normalized_shape)
-    if not shape or tuple(x.shape[x.dim() - len(shape):]) != shape or min(shape) < 1:
-        raise _lib.LspsHipError("layer_norm: normalized_shape %s does not end the shape %s" % (shape, tuple(x.shape)))
-    if x.dtype not in _DTYPES:
-        raise _lib.LspsHipError("layer_norm: float32 or bfloat16 input expected, not %s" % x.dtype)
-    for name, t in (('weight', weight), ('bias', bias)):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32):
-            raise _lib.LspsHipError("layer_norm: %s of shape %s, %s (expected %s, float32)" % (name, tuple(t.shape), t.dtype, shape))
-    _on_device('layer_norm', x, weight, bias)
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     cols = 1
     for n in shape:
         cols *= n
-    return _LayerNormFn.apply(x, weight, bias, cols, float(eps))
+    if not shape or x.shape[-len(shape):] != shape or cols < 1:
+        raise _lib.LspsHipError("layer_norm: normalized_shape %s does not end the shape %s" % (shape, tuple(x.shape)))
+    if x.dtype not in _DTYPES:
+        raise _lib.LspsHipError("layer_norm: float32 or bfloat16 input expected, not %s" % x.dtype)
+    for t in (weight, bias):
+        if t is not None and (t.shape != shape or t.dtype != torch.float32):
+            raise _lib.LspsHipError("layer_norm: weight or bias of shape %s, %s (expected %s, float32)" % (tuple(t.shape), t.dtype, shape))
+    index = _same_device('layer_norm', x, weight, bias)
+    return _LayerNormFn.apply(x, weight, bias, index, cols, float(eps))
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)     # quintic whose iterates send (0, 1] near 1 within five steps (the usual choice with Muon)
@@ -1817,23 +1839,6 @@ NS_COEFFS = (3.4445, -4.7750, 2.0315)     # quintic whose iterates send (0, 1] n
 def _coeffs(coeffs):
     a, b, c = (float(v) for v in coeffs)
     return a, b, c
-
-
-@torch.no_grad()
-def _newton_schulz(g, steps, coeffs, eps):
-    L = _lib.lib()
-    dev, st = _on_device('newton_schulz', g)
-    out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-    if g.numel() == 0:
-        return out
-    g = _c(g)
-    rows, cols = g.shape[-2:]
-    count = g.numel() // (rows * cols)
-    ws = _scratch(L.lsps_newton_schulz_workspace_bytes(count, rows, cols, steps), g.device)
-    with dev:
-        _lib.check(L.lsps_newton_schulz(g.data_ptr(), out.data_ptr(), count, rows, cols, _DTYPES[g.dtype], steps, *coeffs, eps, *_ws(ws),
-                                        st), 'newton_schulz')
-    return out
 
 
 def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
@@ -1846,7 +1851,19 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         raise _lib.LspsHipError("newton_schulz: float32 or bfloat16 expected, not %s" % g.dtype)
     if g.requires_grad and torch.is_grad_enabled():
         raise _lib.LspsHipError("newton_schulz has no backward pass: call it under torch.no_grad() or on a detached tensor")
-    return _newton_schulz(g, int(steps), _coeffs(coeffs), float(eps))
+    index = _same_device('newton_schulz', g)
+    with torch.no_grad():
+        out = torch.empty_like(g, memory_format=torch.contiguous_format)
+        if g.numel() == 0:
+            return out
+        L = _lib.lib()
+        g = _c(g)
+        rows, cols = g.shape[-2:]
+        count = g.numel() // (rows * cols)
+        buf, ws, n = _scratch(L.lsps_newton_schulz_workspace_bytes(count, rows, cols, int(steps)), g)
+        _launch('newton_schulz', index, L.lsps_newton_schulz, g.data_ptr(), out.data_ptr(), count, rows, cols, _DTYPES[g.dtype], int(steps),
+                *_coeffs(coeffs), float(eps), ws, n)
+    return out
 
 
 def _disjoint(what, written, read):
@@ -1877,15 +1894,14 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     if not params:
         return
     L = _lib.lib()
-    dev, st = _on_device('muon_step_', params[0], *(params + grads + momenta))
+    index = _same_device('muon_step_', params[0], *(params + grads + momenta))
     mats = (_lib.LspsMuonMatrix * len(params))()
     for k, (p, g, m) in enumerate(zip(params, grads, momenta)):
         mats[k] = _lib.LspsMuonMatrix(_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), p.shape[0], p.numel() // p.shape[0])
     _disjoint('muon_step_', params + momenta, grads)
-    ws = _scratch(L.lsps_muon_workspace_bytes(mats, len(params), int(steps)), params[0].device)
-    with dev:
-        _lib.check(L.lsps_muon_step(mats, len(params), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(rms),
-                                    float(grad_scale), int(steps), *_coeffs(coeffs), float(eps), *_ws(ws), st), 'muon_step')
+    buf, ws, n = _scratch(L.lsps_muon_workspace_bytes(mats, len(params), int(steps)), params[0])
+    _launch('muon_step', index, L.lsps_muon_step, mats, len(params), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
+            float(rms), float(grad_scale), int(steps), *_coeffs(coeffs), float(eps), ws, n)
     torch.autograd.graph.increment_version(params + momenta)       # written behind torch's back
 
 

@@ -132,7 +132,8 @@ def muon_reference(p, g, m, lr, momentum, nesterov, wd, rms, gscale, steps=5):
 
 
 SETS = [[(50, 108)], [(50, 108), (20, 50), (50, 20), (108, 50)], [(64, 1, 7, 7), (128, 64, 3, 3), (20, 48, 2, 2), (1, 9), (9, 1), (256, 300)],
-        [(33 + i % 7, 20 + i) for i in range(70)]]
+        [(33 + i % 7, 20 + i) for i in range(70)],
+        [(30, 40), (40, 30), (30, 40), (200, 900), (70, 30), (200, 900), (520, 2100), (400, 420), (40, 30), (192, 500)]]
 
 
 @pytest.mark.parametrize('nesterov', [True, False])

@@ -84,12 +84,15 @@ def test_refusals_of_the_c_entry_points():
 
 def test_workspace_sizes_grow_with_the_call():
     h = _lib.lib()
-    one, many = h.lsps_newton_schulz_workspace_bytes(1, 256, 2304, 5), h.lsps_newton_schulz_workspace_bytes(28, 256, 2304, 5)
-    assert 4 * 4 * 256 * 2304 < one < 2 * (4 * 4 * 256 * 2304 + 5 * 4 * 256 * 256) and many < 28 * one
-    assert h.lsps_newton_schulz_workspace_bytes(1, 2304, 256, 5) == one                          # tall = wide
-    assert h.lsps_newton_schulz_workspace_bytes(1, 256, 2304, 3) < one                           # no second chain
-    mats = (_lib.LspsMuonMatrix * 70)(*[_lib.LspsMuonMatrix(0, 0, 0, 64, 64)] * 70)
-    assert h.lsps_muon_workspace_bytes(mats, 70, 5) == h.lsps_muon_workspace_bytes(mats, 64, 5)   # passes of 64 share it
+
+    def ns(*a):
+        return h.lsps_newton_schulz_workspace_bytes(*a)
+    assert ns(28, 256, 2304, 5) >= 28 * 4 * 2 * 256 * 2304                 # two limbs, two generations of X
+    assert ns(1, 2304, 256, 5) == ns(1, 256, 2304, 5)                      # tall = wide
+    assert ns(1, 256, 2304, 1) < ns(1, 256, 2304, 5) and ns(2, 100, 90, 5) > ns(1, 100, 90, 5)
+    mats = (_lib.LspsMuonMatrix * 1500)(*[_lib.LspsMuonMatrix(0, 0, 0, 64, 64)] * 1500)
+    one, many = h.lsps_muon_workspace_bytes(mats, 1024, 5), h.lsps_muon_workspace_bytes(mats, 1500, 5)
+    assert h.lsps_muon_workspace_bytes(mats, 1, 5) < one == many            # passes share it
 
 
 def test_flat_muon_sorts_parameters():
