@@ -15,12 +15,15 @@
 // the matrix' entries (22 significand bits; the entries are bounded by the spectral norm, which is a polynomial of values in
 // [0, 1], see ortho_bounds), and a product is three v_mfma_f32_32x32x16_f16 (hi hi + hi lo + lo hi, f32 accumulation; the
 // dropped lo lo is below 2^-22 of the product): f32-class results at a third of the f16 rate, 5 x the f32 MFMA rate.
-// Layout: [row][k / 8][hi 8 | lo 8], rows and columns padded with zeros to multiples of 64: a k-chunk of 32 is one 128-byte line
-// of a row, copied to LDS by 16-byte LDS-DMA whose source addresses carry the bank swizzle (unit ^ (row & 7)).
+// Layout of a matrix with R rows: [column / 32][R][(column % 32) / 8][hi 8 | lo 8], rows and columns padded with zeros to multiples
+// of 64: a 32-deep chunk of a row is one 128-byte line and the rows of a chunk follow each other, so that a tile's chunk is one
+// contiguous run over all L2 channels (rows at a power-of-two pitch all fell on one channel: 2100 instead of 768 cycles per chunk
+// of a 128 x 128 tile at 2048 x 2048).  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.
 // All matrices of a call go through one launch per product (the blocks find their matrix in a table in the workspace).
 #include <math.h>
 #include <string.h>
 
+#include "c8util.h"
 #include "common.h"
 
 namespace lsps {
@@ -28,37 +31,48 @@ namespace lsps {
 typedef _Float16 og_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 og_h4 __attribute__((ext_vector_type(4)));
 typedef float og_f16v __attribute__((ext_vector_type(16)));
+typedef float og_f4 __attribute__((ext_vector_type(4)));
 typedef float og_f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short og_u4u __attribute__((ext_vector_type(4), aligned(2)));
-typedef __attribute__((address_space(3))) void *og_lds;
-typedef const __attribute__((address_space(1))) void *og_glb;
 
-#define ORTHO_GROUPS 64        // groups of equal matrices per pass (the blocks search them with one ballot)
-#define ORTHO_CHAIN 3          // steps between two Gram matrices of the long side
+#define ORTHO_GROUPS 64        // shapes per pass (the blocks search them with one ballot)
+#define ORTHO_MATRICES 1024    // matrices with pointers of their own per pass
+#define ORTHO_CHAINS 3         // longest chain: steps between two Gram matrices of the long side
 #define ORTHO_NORM_BLOCK 16384 // elements per block of the norm pass
-#define ORTHO_TABLE_PART 32    // groups per table launch (passed by value: nothing on the host has to outlive the call)
-enum { OK_NORM, OK_SPLIT, OK_SYM64, OK_SYM128, OK_RECT64, OK_RECT128, ORTHO_KINDS };
-enum { OB_A, OB_S, OB_T, OB_R0, OB_R1, OB_SMALL, OB_X0 = OB_SMALL, OB_X1, OB_XT0, OB_XT1, OB_NONE };
+#define ORTHO_TABLE_PART 24    // groups, and
+#define ORTHO_PTR_PART 96      // matrices per table launch (passed by value: nothing on the host has to outlive the call)
+#define ORTHO_STEPS 64
+enum { OB_A, OB_S, OB_T, OB_R0, OB_R1, OB_SMALL, OB_X0 = OB_SMALL, OB_X1, OB_NONE };
 enum { OM_F32, OM_BF16, OM_MUON };
+enum { OL_SYM, OL_RECT, OL_LAST };
 
-struct OrthoGroup {
-  const void *g;       // count matrices of rows x cols, contiguous
+struct OrthoPtr {
+  const void *g;
   void *out;           // OM_MUON: the weights
   float *m;            // OM_MUON: the momentum
-  unsigned x_off, s_off;          // workspace offsets in 256-byte units: long-side matrices, M x M matrices
+};
+
+// `count` matrices of one shape
+struct OrthoGroup {
+  OrthoPtr base;                  // ptr < 0: the matrices lie one behind the other from here on
+  int ptr;                        // else: the first of their pointers in the table
+  unsigned x_off, s_off, p_off;   // workspace offsets in 256-byte units: long-side matrices, M x M matrices, partial products
   int norm_off;                   // first of the matrices' partial sums of squares
   int rows, cols, count;
+  int chain;                      // steps between two Gram matrices
   float step;                     // OM_MUON: lr rms sqrt(max(rows, cols))
-  int first[ORTHO_KINDS];         // blocks in front of this group, for each way of cutting it into blocks
 };
 
 struct OrthoTable {
   OrthoGroup g[ORTHO_GROUPS];
-  int first[ORTHO_KINDS][ORTHO_GROUPS];
+  OrthoPtr ptr[ORTHO_MATRICES];
 };
 
 struct OrthoPart {
   OrthoGroup g[ORTHO_TABLE_PART];
+};
+struct OrthoPtrPart {
+  OrthoPtr p[ORTHO_PTR_PART];
 };
 
 __host__ __device__ static inline int og_pad(int n) { return (n + 63) & ~63; }
@@ -67,46 +81,45 @@ __host__ __device__ static inline int og_long(const OrthoGroup &g) { return g.ro
 __host__ __device__ static inline int og_norm_blocks(const OrthoGroup &g) {
   return (int)(((long)g.rows * g.cols + ORTHO_NORM_BLOCK - 1) / ORTHO_NORM_BLOCK);
 }
-// blocks per matrix
-__host__ __device__ static inline int og_blocks(const OrthoGroup &g, int kind) {
-  const int M = og_pad(og_short(g)), N = og_pad(og_long(g));
-  switch (kind) {
-    case OK_NORM: return og_norm_blocks(g);
-    case OK_SPLIT: return (M / 64) * (N / 64);
-    case OK_SYM64: return (M / 64) * (M / 64 + 1) / 2;
-    case OK_SYM128: return ((M + 127) / 128) * ((M + 127) / 128 + 1) / 2;
-    case OK_RECT64: return (M / 64) * (N / 64);
-    default: return ((M + 127) / 128) * ((N + 127) / 128);
-  }
+__host__ __device__ static inline int og_split_blocks(const OrthoGroup &g) { return og_pad(g.rows) / 64 * (og_pad(g.cols) / 64); }
+// tiles of T x T per matrix of a product
+__host__ __device__ static inline int og_tiles(const OrthoGroup &g, int type, int T) {
+  const int m = (og_pad(og_short(g)) + T - 1) / T, n = (og_pad(og_long(g)) + T - 1) / T;
+  return type == OL_SYM ? m * (m + 1) / 2 : m * n;
 }
 
 __global__ void ortho_table_kernel(OrthoPart part, OrthoTable *t, int base, int n) {
-  const int i = threadIdx.x;
-  if (i >= n) return;
-  t->g[base + i] = part.g[i];
-  for (int k = 0; k < ORTHO_KINDS; ++k) t->first[k][base + i] = part.g[i].first[k];
+  if ((int)threadIdx.x < n) t->g[base + threadIdx.x] = part.g[threadIdx.x];
+}
+__global__ void ortho_ptr_kernel(OrthoPtrPart part, OrthoTable *t, int base, int n) {
+  if ((int)threadIdx.x < n) t->ptr[base + threadIdx.x] = part.p[threadIdx.x];
 }
 
-struct OrthoAt {
-  int grp, mat, tile;
+// first block of every group in a launch
+struct OrthoFirst {
+  int b[ORTHO_GROUPS];
 };
-// group, matrix and tile of block b: the group is the last one whose first block is not behind b
-__device__ __forceinline__ OrthoAt ortho_at(const OrthoTable *t, int n, int kind, int b) {
+// the group of block b: the last one whose first block is not behind it
+__device__ __forceinline__ int ortho_group_of(const OrthoFirst &first, int n, int b) {
   const int lane = threadIdx.x & 63;
-  const bool le = lane < n && t->first[kind][lane] <= b;
-  OrthoAt at;
-  at.grp = __builtin_amdgcn_readfirstlane(63 - __clzll(__ballot(le)));
-  const int per = og_blocks(t->g[at.grp], kind), rel = b - t->g[at.grp].first[kind];
-  at.mat = rel / per;
-  at.tile = rel - at.mat * per;
-  return at;
+  const bool le = lane < n && first.b[lane] <= b;
+  return __builtin_amdgcn_readfirstlane(63 - __clzll(__ballot(le)));
+}
+
+__device__ __forceinline__ OrthoPtr ortho_ptr(const OrthoTable *t, const OrthoGroup &g, int mat, int bytes) {
+  if (g.ptr >= 0) return t->ptr[g.ptr + mat];
+  const long o = (long)g.rows * g.cols * mat * bytes;
+  return OrthoPtr{(const char *)g.base.g + o, (char *)g.base.out + o, nullptr};
 }
 
 __device__ __forceinline__ char *ortho_buffer(char *ws, const OrthoGroup &g, int id, int mat) {
   const long M = og_pad(og_short(g)), N = og_pad(og_long(g));
   if (id < OB_SMALL) return ws + (size_t)g.s_off * 256 + ((long)id * g.count + mat) * M * M * 4;
-  const int which = id == OB_X0 ? 0 : id == OB_XT0 ? 1 : id == OB_X1 ? 2 : 3;
-  return ws + (size_t)g.x_off * 256 + ((long)which * g.count + mat) * M * N * 4;
+  return ws + (size_t)g.x_off * 256 + ((long)(id - OB_X0) * g.count + mat) * M * N * 4;
+}
+// byte of element (row, col) of a matrix of R rows: its hi limb (the lo limb is 16 bytes on)
+__device__ __forceinline__ long og_at(long R, int row, int col) {
+  return ((col >> 5) * R + row) * 128 + ((col >> 3) & 3) * 32 + (col & 7) * 2;
 }
 
 template <typename T>
@@ -136,13 +149,15 @@ struct OrthoMomentum {
 // the momentum is updated on the way.  Memory bound: 4 (Muon: 12) bytes per element.
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable *__restrict__ t, int n, double *__restrict__ sums,
-                                                         OrthoMomentum mo) {
+                                                         OrthoMomentum mo, OrthoFirst first) {
   __shared__ double red[4];
-  const OrthoAt at = ortho_at(t, n, OK_NORM, blockIdx.x);
-  const OrthoGroup &g = t->g[at.grp];
-  const long size = (long)g.rows * g.cols, lo = (long)at.tile * ORTHO_NORM_BLOCK;
-  const T *src = (const T *)g.g + at.mat * size;
-  float *m = MUON ? g.m + at.mat * size : nullptr;
+  const int grp = ortho_group_of(first, n, blockIdx.x);
+  const OrthoGroup g = t->g[grp];
+  const int rel = blockIdx.x - first.b[grp], nb = og_norm_blocks(g), mat = rel / nb, tile = rel - mat * nb;
+  const long size = (long)g.rows * g.cols, lo = (long)tile * ORTHO_NORM_BLOCK;
+  const OrthoPtr ptr = ortho_ptr(t, g, mat, sizeof(T));
+  const T *src = (const T *)ptr.g;
+  float *m = ptr.m;
   double s = 0.;
 #pragma unroll 4
   for (int i = 0; i < ORTHO_NORM_BLOCK / 1024; ++i) {
@@ -173,7 +188,7 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable *__res
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) sums[g.norm_off + at.mat * og_norm_blocks(g) + at.tile] = red[0] + red[1] + red[2] + red[3];
+  if (threadIdx.x == 0) sums[g.norm_off + rel] = red[0] + red[1] + red[2] + red[3];
 }
 
 __device__ __forceinline__ void og_split(float v, _Float16 &hi, _Float16 &lo) {
@@ -181,26 +196,28 @@ __device__ __forceinline__ void og_split(float v, _Float16 &hi, _Float16 &lo) {
   lo = (_Float16)(v - (float)hi);
 }
 
-// X0 as limbs, both ways round: X (short side in rows) and its transpose.  One 64 x 64 tile of G per block, through LDS.
+// X0 as limbs, the short side in rows.  One 64 x 64 tile of G per block, through LDS (turned round there for a tall G).
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ortho_split_kernel(const OrthoTable *__restrict__ t, int n, char *__restrict__ ws,
-                                                          const double *__restrict__ sums, OrthoMomentum mo, float eps, float scale) {
+                                                          const double *__restrict__ sums, OrthoMomentum mo, float eps, float scale,
+                                                          OrthoFirst first) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
-  const OrthoAt at = ortho_at(t, n, OK_SPLIT, blockIdx.x);
-  const OrthoGroup &g = t->g[at.grp];
+  const int grp = ortho_group_of(first, n, blockIdx.x);
+  const OrthoGroup g = t->g[grp];
+  const int rel = blockIdx.x - first.b[grp], per = og_split_blocks(g), mat = rel / per, tix = rel - mat * per;
   const int nb = og_norm_blocks(g);
-  const double *part = sums + g.norm_off + (long)at.mat * nb;
+  const double *part = sums + g.norm_off + (long)mat * nb;
   double s = 0.;
   for (int i = threadIdx.x; i < nb; i += 256) s += part[i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   const int tc = og_pad(g.cols) / 64;
-  const int r0 = at.tile / tc * 64, c0 = (at.tile - at.tile / tc * tc) * 64;
-  const long size = (long)g.rows * g.cols;
-  const T *src = (const T *)g.g + at.mat * size;
-  const float *m = MUON ? g.m + at.mat * size : nullptr;
+  const int r0 = tix / tc * 64, c0 = (tix - tix / tc * tc) * 64;
+  const OrthoPtr ptr = ortho_ptr(t, g, mat, sizeof(T));
+  const T *src = (const T *)ptr.g;
+  const float *m = ptr.m;
   float v[4][4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -223,166 +240,227 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const OrthoTable *__re
     for (int e = 0; e < 4; ++e) tile[(threadIdx.x >> 4) + k * 16][(threadIdx.x & 15) * 4 + e] = v[k][e] / norm * scale;
   __syncthreads();
   const bool tall = g.rows > g.cols;
-  char *d0 = ortho_buffer(ws, g, tall ? OB_XT0 : OB_X0, at.mat), *d1 = ortho_buffer(ws, g, tall ? OB_X0 : OB_XT0, at.mat);
-  const long p0 = (long)og_pad(g.cols) * 4, p1 = (long)og_pad(g.rows) * 4;     // row pitches in bytes
+  char *dst = ortho_buffer(ws, g, OB_X0, mat);
+  const int M = og_pad(og_short(g)), i0 = tall ? c0 : r0, j0 = tall ? r0 : c0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int u = threadIdx.x + k * 256, a = u >> 3, q = u & 7;
+    const int u = threadIdx.x + k * 256, i = u >> 3, j = (u & 7) * 8;
     og_h8 h, l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       _Float16 x, y;
-      og_split(tile[a][q * 8 + e], x, y);
+      og_split(tall ? tile[j + e][i] : tile[i][j + e], x, y);
       h[e] = x;
       l[e] = y;
     }
-    og_h8 *dst = reinterpret_cast<og_h8 *>(d0 + (r0 + a) * p0 + (c0 / 8 + q) * 32);
-    dst[0] = h;
-    dst[1] = l;
-  }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int u = threadIdx.x + k * 256, a = u >> 3, q = u & 7;
-    og_h8 h, l;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      _Float16 x, y;
-      og_split(tile[q * 8 + e][a], x, y);
-      h[e] = x;
-      l[e] = y;
-    }
-    og_h8 *dst = reinterpret_cast<og_h8 *>(d1 + (c0 + a) * p1 + (r0 / 8 + q) * 32);
-    dst[0] = h;
-    dst[1] = l;
+    og_h8 *o = reinterpret_cast<og_h8 *>(dst + og_at(M, i0 + i, j0 + j));
+    o[0] = h;
+    o[1] = l;
   }
 }
 
-// out = k0 (L R^T) + k1 E1 + k2 E2 on stored (scaled) values: the scales are folded into the factors
+// out = k0 (product) + k1 E1 + k2 E2 + diag I on stored (scaled) values: the scales are folded into the factors
 struct OrthoJob {
-  int l, r, e1, e2, out, mirror;
-  float k0, k1, k2;
+  int l, r, e1, e2, out;
+  float k0, k1, k2, diag;
 };
+// one launch: per chain length the product its groups are at (they walk their own lists side by side)
 struct OrthoLevel {
-  OrthoJob job[2];
-  int blocks;              // per job
-  int mode;                // of the last level: OM_*
-  float decay;             // 1 - lr wd
+  OrthoFirst first;
+  int kz[ORTHO_GROUPS];             // ranges the reduction of a group's product is split into
+  OrthoJob job[ORTHO_CHAINS][2];
+  int jobs[ORTHO_CHAINS], type[ORTHO_CHAINS];
+  int joining;                      // second launch of a split product: add the ranges up
+  int mode;                         // of the last level: OM_*
+  float decay;                      // 1 - lr wd
 };
 
-enum { OL_SYM, OL_RECT, OL_LAST };
-
-// One product per block: a T x T tile of L R^T, both with the reduction along their rows.  4 waves, 2 x 2, each (T/2) x (T/2)
-// in 32x32 MFMA tiles; the MFMA's row index is the tile's COLUMN, so a lane holds one row of the result and runs of 4 columns
-// (8-byte stores per limb).  LDS: two stages of a KC-deep chunk of both operands, filled by LDS-DMA while the other one is
-// multiplied; one barrier per chunk.
-//   OL_SYM : L R^T symmetric; tiles on and above the diagonal, the mirrored tile is stored from an LDS transpose
-//   OL_RECT: X of the next chain, stored both ways round
-//   OL_LAST: the result in the caller's layout and type, or the weight update
-template <int T, int KC, int LEVEL>
-__global__ __launch_bounds__(256) void ortho_product_kernel(const OrthoTable *__restrict__ t, int n, char *__restrict__ ws, OrthoLevel lv) {
-  constexpr int UPR = KC / 4, STAGE = T * KC * 4, PIECES = T * UPR / 256, RPP = 64 / UPR, WT = T / 2, FR = WT / 32, TP = 144;
-  constexpr int KIND = LEVEL == OL_SYM ? (T == 64 ? OK_SYM64 : OK_SYM128) : (T == 64 ? OK_RECT64 : OK_RECT128);
-  static_assert(4 * STAGE >= 4 * 32 * TP, "the transpose of the epilogue reuses the stages");
+// One product per block: a T x T tile.  WI x WJ waves, each (T / WI) x (T / WJ) in 32x32 MFMA tiles; the MFMA's row index is the tile's
+// COLUMN, so a lane holds one row of the result and runs of 4 columns (8-byte stores per limb).  hi hi has an accumulator of its
+// own: the small cross products, added to it, would cost it a rounding each (measured: that halves the error of the whole
+// iteration).  LDS: S stages of a KC-deep chunk of both operands, S - 1 of them requested ahead by LDS-DMA (from inline asm:
+// in front of a transposing read the compiler would wait for all requests); one barrier per chunk.
+//   OL_SYM : L R^T, symmetric: tiles on and above the diagonal, the mirrored tile is stored from an LDS transpose
+//   OL_RECT: L X, X of the next chain: the reduction runs down the rows of X, whose chunks are read transposed from LDS
+//   OL_LAST: the same, the result in the caller's layout and type, or the weight update
+// A product with few tiles and a long reduction is split into kz ranges of it: f32 partial tiles in the workspace, added in a
+// fixed order by a second launch of this kernel.
+template <int T, int KC, int S, int WI, int WJ>
+__global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(const OrthoTable *__restrict__ t, int n, char *__restrict__ ws, OrthoLevel lv) {
+  constexpr int WAVES = WI * WJ, SUB = KC / 32, STAGE = T * KC * 4, PIECES = T * SUB / 8 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = 144;
+  static_assert(S * 2 * STAGE >= WAVES * 32 * TP, "the transpose of the epilogue reuses the stages");
+  static_assert((S - 2) * 2 * PIECES < 64, "the range of s_waitcnt vmcnt");
   extern __shared__ __align__(1024) char smem[];
-  const int second = (int)blockIdx.x >= lv.blocks;
-  const OrthoJob job = lv.job[second];
-  const OrthoAt at = ortho_at(t, n, KIND, blockIdx.x - second * lv.blocks);
-  const OrthoGroup g = t->g[at.grp];
+  const int grp = ortho_group_of(lv.first, n, blockIdx.x);
+  const OrthoGroup g = t->g[grp];
+  const int cls = g.chain - 1, type = lv.type[cls], kz = lv.joining ? 1 : lv.kz[grp];
   const int M = og_pad(og_short(g)), N = og_pad(og_long(g));
+  const int per = og_tiles(g, type, T) * kz, total = per * g.count * lv.jobs[cls];
+  // consecutive blocks go to the eight XCDs in turn: block x + 8 y takes unit x q + y, so that an XCD's blocks share operands in its L2
+  const int rel = blockIdx.x - lv.first.b[grp], q8 = (total + 7) / 8, unit0 = (rel & 7) * q8 + (rel >> 3);
+  if ((rel >> 3) >= q8 || unit0 >= total) return;
+  const int second = unit0 >= per * g.count;
+  const OrthoJob job = lv.job[cls][second];
+  const int u1 = unit0 - second * per * g.count, mat = u1 / per, u2 = u1 - mat * per, z = u2 % kz, tile = u2 / kz;
   int bi, bj;
-  if (LEVEL == OL_SYM) {
-    bj = (int)((sqrtf(8.f * at.tile + 1.f) - 1.f) * 0.5f);
-    while ((bj + 1) * (bj + 2) / 2 <= at.tile) ++bj;
-    while (bj * (bj + 1) / 2 > at.tile) --bj;
-    bi = at.tile - bj * (bj + 1) / 2;
+  if (type == OL_SYM) {
+    bj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while ((bj + 1) * (bj + 2) / 2 <= tile) ++bj;
+    while (bj * (bj + 1) / 2 > tile) --bj;
+    bi = tile - bj * (bj + 1) / 2;
   } else {
-    const int tn = (N + T - 1) / T;
-    bi = at.tile / tn;
-    bj = at.tile - bi * tn;
+    const int tm = (M + T - 1) / T;                              // the row tiles of one column panel one after the other
+    bj = tile / tm;
+    bi = tile - bj * tm;
   }
-  const int cols = LEVEL == OL_SYM ? M : N;                      // of the result; rows: M
+  const int cols = type == OL_SYM ? M : N;                       // of the result; rows: M
   const int K = job.l >= OB_SMALL ? N : M;
-  const long pitch = (long)K * 4;
-  const char *L = ortho_buffer(ws, g, job.l, at.mat), *R = ortho_buffer(ws, g, job.r, at.mat);
+  const int chunks = K / KC, c0 = (int)((long)chunks * z / kz), c1 = (int)((long)chunks * (z + 1) / kz);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const char *lp[PIECES], *rp[PIECES];
+  const int wi = wave / WJ, wj = wave % WJ, l31 = lane & 31, lh = lane >> 5;
+  og_f16v acc[FI][FJ], acx[FI][FJ];
 #pragma unroll
-  for (int p = 0; p < PIECES; ++p) {
-    const int row = (wave + 4 * p) * RPP + lane / UPR, unit = (lane % UPR) ^ (row & 7);
-    const int li = bi * T + row < M ? bi * T + row : M - 1, rj = bj * T + row < cols ? bj * T + row : cols - 1;
-    lp[p] = L + li * pitch + unit * 16;
-    rp[p] = R + rj * pitch + unit * 16;
-  }
-  auto stage = [&](int buf) {
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = acx[i][j][e] = 0.f;
+  float *part = reinterpret_cast<float *>(ws + (size_t)g.p_off * 256);   // [mat][tile][z][fi][fj][q][thread][4]
+  if (!lv.joining) {
+    // a piece = 8 lines of 128 bytes = one DMA request of a wave: [sub-chunk of 32][line], line = row of the tile; for X in
+    // OL_RECT / OL_LAST: [32 columns][row of the chunk].  Unit u of line r lies at u ^ (r / 2): 16 lanes reading 16 consecutive
+    // lines, or four lines of the 64-bit transposing reads, touch all 64 banks once
+    const bool turned = type != OL_SYM;
+    const c8_i32x4 lrs = c8_rsrc_words(ortho_buffer(ws, g, job.l, mat), (unsigned)((long)M * K * 4));
+    const c8_i32x4 rrs = c8_rsrc_words(ortho_buffer(ws, g, job.r, mat), (unsigned)((long)M * (turned ? N : K) * 4));
+    unsigned lo[PIECES], ro[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      __builtin_amdgcn_global_load_lds((og_glb)lp[p], (og_lds)(smem + buf * 2 * STAGE + (wave + 4 * p) * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((og_glb)rp[p], (og_lds)(smem + buf * 2 * STAGE + STAGE + (wave + 4 * p) * 1024), 16, 0, 0);
-      lp[p] += KC * 4;
-      rp[p] += KC * 4;
+      const int line = (wave + WAVES * p) * 8 + (lane >> 3), sub = line / T, row = line % T, unit = ((lane & 7) ^ ((line >> 1) & 7)) * 16;
+      const int li = bi * T + row < M ? bi * T + row : M - 1;
+      lo[p] = (unsigned)((sub * M + li) * 128 + unit);
+      if (!turned) {
+        const int rj = bj * T + row < M ? bj * T + row : M - 1;
+        ro[p] = (unsigned)((sub * M + rj) * 128 + unit);
+      } else {                                                            // T / 32 column chunks of KC rows each
+        const int cc = line / KC, r = line % KC;
+        const int c = bj * (T / 32) + cc < N / 32 ? bj * (T / 32) + cc : N / 32 - 1;
+        ro[p] = (unsigned)((c * (long)M + r) * 128 + unit);
+      }
     }
-  };
-  const int wi = wave >> 1, wj = wave & 1, l31 = lane & 31, lh = lane >> 5;
-  og_f16v acc[FR][FR];
+    const unsigned lstep = (unsigned)M * SUB * 128, rstep = turned ? KC * 128 : lstep, lds0 = c8_lds_addr(smem);
+    auto stage = [&](int buf, int c) {
 #pragma unroll
-  for (int i = 0; i < FR; ++i)
+      for (int p = 0; p < PIECES; ++p) {
+        c8_dma16_asm(lrs, lds0 + buf * 2 * STAGE + (wave + WAVES * p) * 1024, lo[p], c * lstep);
+        c8_dma16_asm(rrs, lds0 + buf * 2 * STAGE + STAGE + (wave + WAVES * p) * 1024, ro[p], c * rstep);
+      }
+    };
+    const int n = c1 - c0;
 #pragma unroll
-    for (int j = 0; j < FR; ++j)
+    for (int c = 0; c < S - 1; ++c)
+      if (c < n) stage(c, c0 + c);
+    int at = 0;
+    for (int c = 0; c < n; ++c) {
+      // requests are served in order: those of the S - 2 chunks behind this one may still be on their way
+      if (c + S - 1 <= n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * 2 * PIECES) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();                                        // (__syncthreads may wait for all requests)
+      asm volatile("" ::: "memory");
+      if (c + S - 1 < n) stage(at == 0 ? S - 1 : at - 1, c0 + c + S - 1);  // the stage that was multiplied before this barrier
+      const char *sl = smem + at * 2 * STAGE, *sr = sl + STAGE;
+      at = at + 1 == S ? 0 : at + 1;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  stage(0);
-  const int chunks = K / KC;
-  for (int c = 0; c < chunks; ++c) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (c + 1 < chunks) stage((c + 1) & 1);
-    const char *sl = smem + (c & 1) * 2 * STAGE, *sr = sl + STAGE;
-#pragma unroll
-    for (int ks = 0; ks < KC / 16; ++ks) {
-      const int kg = ks * 2 + lh;
-      og_h8 lf[FR][2], rf[FR][2];
-#pragma unroll
-      for (int f = 0; f < FR; ++f)
+      for (int ks = 0; ks < KC / 16; ++ks) {
+        const int sub = ks >> 1, kg = (ks & 1) * 2 + lh;
+        og_h8 lf[FI][2], rf[FJ][2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int li = wi * WT + f * 32 + l31, rj = wj * WT + f * 32 + l31;
-          lf[f][q] = *reinterpret_cast<const og_h8 *>(sl + li * (UPR * 16) + (((kg * 2 + q) ^ (li & 7)) * 16));
-          rf[f][q] = *reinterpret_cast<const og_h8 *>(sr + rj * (UPR * 16) + (((kg * 2 + q) ^ (rj & 7)) * 16));
+#pragma unroll
+          for (int f = 0; f < FJ; ++f)
+            if (!turned) {
+              const int rj = (wj * FJ + f) * 32 + l31;
+              rf[f][q] = *reinterpret_cast<const og_h8 *>(sr + (sub * T + rj) * 128 + (((kg * 2 + q) ^ ((rj >> 1) & 7)) * 16));
+            } else {
+              // lane i of 16 points at 4 columns of row i / 4 and receives 4 rows of column i
+              const int r = ks * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2 + q;
+              const char *base = sr + ((wj * FJ + f) * KC + r) * 128 + (lane & 1) * 8;
+              rf[f][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)base + ((u ^ ((r >> 1) & 7)) * 16),
+                                                              (const unsigned char *)base + 512 + ((u ^ (((r + 4) >> 1) & 7)) * 16)));
+            }
+#pragma unroll
+          for (int f = 0; f < FI; ++f) {
+            const int li = (wi * FI + f) * 32 + l31;
+            lf[f][q] = *reinterpret_cast<const og_h8 *>(sl + (sub * T + li) * 128 + (((kg * 2 + q) ^ ((li >> 1) & 7)) * 16));
+          }
         }
 #pragma unroll
-      for (int i = 0; i < FR; ++i)
+        for (int i = 0; i < FI; ++i)
 #pragma unroll
-        for (int j = 0; j < FR; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][0], lf[i][1], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][1], lf[i][0], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][0], lf[i][0], acc[i][j], 0, 0, 0);
-        }
+          for (int j = 0; j < FJ; ++j) {
+            acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][0], lf[i][1], acx[i][j], 0, 0, 0);
+            acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][1], lf[i][0], acx[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][0], lf[i][0], acc[i][j], 0, 0, 0);
+          }
+      }
     }
+    if (kz > 1) {
+      og_f4 *dst = reinterpret_cast<og_f4 *>(part) + ((long)(mat * (per / kz) + tile) * kz + z) * (T * T / 4) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            og_f4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e] + acx[i][j][q * 4 + e];
+            dst[((i * FJ + j) * 4 + q) * WAVES * 64] = v;
+          }
+      return;
+    }
+  } else {
+    const int nz = lv.kz[grp];
+    const og_f4 *src = reinterpret_cast<const og_f4 *>(part) + (long)(mat * per + tile) * nz * (T * T / 4) + threadIdx.x;
+    for (int k = 0; k < nz; ++k, src += T * T / 4)
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const og_f4 v = src[((i * FJ + j) * 4 + q) * WAVES * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][q * 4 + e] += v[e];
+          }
   }
-  const char *e1 = job.e1 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e1, at.mat);
-  const char *e2 = job.e2 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e2, at.mat);
-  const long opitch = (long)cols * 4;
+  const char *e1 = job.e1 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e1, mat);
+  const char *e2 = job.e2 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e2, mat);
   auto stored = [&](const char *e, int i, int j, float (&v)[4]) {        // 4 stored values of row i from column j on
-    const og_h4 *p = reinterpret_cast<const og_h4 *>(e + i * opitch + (j >> 3) * 32 + (j & 7) * 2);
+    const og_h4 *p = reinterpret_cast<const og_h4 *>(e + og_at(M, i, j));
     const og_h4 h = p[0], l = p[2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = (float)h[k] + (float)l[k];
   };
-  if (LEVEL != OL_LAST) __syncthreads();                                 // the stages become the waves' transpose buffers
+  const bool last = type == OL_LAST, mirrored = type == OL_SYM && bi != bj;
+  const OrthoPtr ptr = ortho_ptr(t, g, mat, lv.mode == OM_BF16 ? 2 : 4);
+  const int m = og_short(g), nn = og_long(g);
+  const bool tall = g.rows > g.cols;
+  char *out = last ? nullptr : ortho_buffer(ws, g, job.out, mat);
+  if (mirrored) __syncthreads();                                         // the stages become the waves' transpose buffers
   char *tp = smem + wave * 32 * TP;
 #pragma unroll
-  for (int fi = 0; fi < FR; ++fi)
+  for (int fi = 0; fi < FI; ++fi)
 #pragma unroll
-    for (int fj = 0; fj < FR; ++fj) {
-      const int i0 = bi * T + wi * WT + fi * 32, j0 = bj * T + wj * WT + fj * 32, i = i0 + l31;
+    for (int fj = 0; fj < FJ; ++fj) {
+      const int i0 = bi * T + (wi * FI + fi) * 32, j0 = bj * T + (wj * FJ + fj) * 32, i = i0 + l31;
       if (i0 >= M || j0 >= cols) continue;                               // (T = 128 on an odd number of 64-row halves)
-      const bool mirrored = LEVEL == OL_RECT || (LEVEL == OL_SYM && bi != bj);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int j = j0 + q * 8 + lh * 4;
         float v[4], x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = job.k0 * acc[fi][fj][q * 4 + k];
+        for (int k = 0; k < 4; ++k) v[k] = job.k0 * (acc[fi][fj][q * 4 + k] + acx[fi][fj][q * 4 + k]);
         if (e1) {
           stored(e1, i, j, x);
 #pragma unroll
@@ -393,16 +471,17 @@ __global__ __launch_bounds__(256) void ortho_product_kernel(const OrthoTable *__
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = fmaf(job.k2, x[k], v[k]);
         }
-        if constexpr (LEVEL != OL_LAST) {
+        if (!last) {
           og_h4 h, l;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
+            if (i == j + k) v[k] += job.diag;
             _Float16 a, b;
             og_split(v[k], a, b);
             h[k] = a;
             l[k] = b;
           }
-          og_h4 *p = reinterpret_cast<og_h4 *>(ortho_buffer(ws, g, job.out, at.mat) + i * opitch + (j >> 3) * 32 + (j & 7) * 2);
+          og_h4 *p = reinterpret_cast<og_h4 *>(out + og_at(M, i, j));
           p[0] = h;
           p[2] = l;
           if (mirrored) {
@@ -413,35 +492,40 @@ __global__ __launch_bounds__(256) void ortho_product_kernel(const OrthoTable *__
               *reinterpret_cast<_Float16 *>(d + 64) = l[k];
             }
           }
-        } else {
-          const int m = og_short(g), nn = og_long(g);
-          const bool tall = g.rows > g.cols;
-          const long size = (long)g.rows * g.cols;
-          if (i < m) {
+        } else if (i < m) {
+          if (!tall && j + 4 <= nn && lv.mode != OM_BF16) {
+            og_f4u *o = reinterpret_cast<og_f4u *>((float *)ptr.out + (long)i * nn + j);
+            og_f4u y;
+            if (lv.mode == OM_MUON) {
+              const og_f4u w = *o;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) y[k] = fmaf(-g.step, v[k], w[k] * lv.decay);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) y[k] = v[k];
+            }
+            *o = y;
+          } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               if (j + k < nn) {
-                const long o = at.mat * size + (tall ? (long)(j + k) * m + i : (long)i * nn + j + k);
-                if (lv.mode == OM_F32) ((float *)g.out)[o] = v[k];
-                else if (lv.mode == OM_BF16) ((__bf16 *)g.out)[o] = (__bf16)v[k];       // the one rounding of the result
-                else ((float *)g.out)[o] = fmaf(-g.step, v[k], ((float *)g.out)[o] * lv.decay);
+                const long o = tall ? (long)(j + k) * m + i : (long)i * nn + j + k;
+                if (lv.mode == OM_F32) ((float *)ptr.out)[o] = v[k];
+                else if (lv.mode == OM_BF16) ((__bf16 *)ptr.out)[o] = (__bf16)v[k];       // the one rounding of the result
+                else ((float *)ptr.out)[o] = fmaf(-g.step, v[k], ((float *)ptr.out)[o] * lv.decay);
               }
           }
         }
       }
-      if constexpr (LEVEL != OL_LAST) {
-        if (mirrored) {
-          char *dst = ortho_buffer(ws, g, job.mirror, at.mat);
-          const long mp = (long)M * 4;                                   // the mirrored matrix has the result's rows as columns
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (mirrored) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const int u = lane + s * 64, jr = u >> 3, ig = (u & 7) >> 1, limb = u & 1;
-            const og_h8 x = *reinterpret_cast<const og_h8 *>(tp + jr * TP + limb * 64 + ig * 16);
-            *reinterpret_cast<og_h8 *>(dst + (j0 + jr) * mp + (i0 / 8 + ig) * 32 + limb * 16) = x;
-          }
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int s = 0; s < 4; ++s) {
+          const int u = lane + s * 64, jr = u >> 3, ig = (u & 7) >> 1, limb = u & 1;
+          const og_h8 x = *reinterpret_cast<const og_h8 *>(tp + jr * TP + limb * 64 + ig * 16);
+          *reinterpret_cast<og_h8 *>(out + og_at(M, j0 + jr, i0 + ig * 8) + limb * 16) = x;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
     }
 }
@@ -456,21 +540,32 @@ struct OrthoCall {
   OrthoMomentum mo;
 };
 
+// Steps between two Gram matrices.  Longer chains save products with the long side (worth it from N = 2 M on; the M x M products
+// they add cost more below) and carry rounding further.  Error of five steps against 64 bits, relative, plain f32 iteration / chains
+// of 1 / 2 / 3:  256 x 2304: 3.4e-6 / 1.6e-6 / 2.2e-6 / 3.5e-6   600 x 600: 2.5e-6 / 1.0e-6 / 1.7e-6 / 5.7e-6
+//                128 x 576: 1.8e-6 / 0.9e-6 / 3.1e-6 / 3.8e-6    50 x 108: 1.3e-6 / 1.2e-6 / 8.0e-6 / 4.0e-6
+static int ortho_chain(const OrthoGroup &g) {
+  const int M = og_short(g), N = og_long(g);
+  if (M < 192 || N < 2 * M) return 1;
+  return N < 4 * M ? 2 : 3;
+}
+
 // Bounds of the matrices' spectral norms (hence of their entries) along the iteration: every one of them is a polynomial of
-// X0's singular values, which lie in [0, 1].  bx: X; ba, bs, bt, br: A, S, T = A P, R of one chain.  False if the coefficients
-// let the iteration grow out of hand (or are not finite).
+// X0's singular values, which lie in [0, 1].  The scales that put them into the range of f16 limbs: X before and behind a chain,
+// A, S, T = A P and R at its steps, Q = a^n I + R at its end (s for a chain of one step).
 struct OrthoScale {
-  float x[ORTHO_CHAIN + 1], a[ORTHO_CHAIN], s[ORTHO_CHAIN], t[ORTHO_CHAIN], r[ORTHO_CHAIN];
+  float x[2], a[ORTHO_CHAINS], s[ORTHO_CHAINS], t[ORTHO_CHAINS], r[ORTHO_CHAINS], q;
 };
-#define ORTHO_SAMPLES 1025
+#define ORTHO_SAMPLES 257
 #define ORTHO_GROWTH 1e4
 static bool ortho_scale_of(double bound, float *scale) {
   if (!(bound <= ORTHO_GROWTH)) return false;
   if (bound < 1e-6) bound = 1e-6;
-  *scale = (float)exp2(floor(log2(16384. / bound)));     // a factor of 4 below the largest f16 for rounding and between the samples
+  *scale = (float)exp2(floor(log2(16384. / bound)));     // a factor of 4 below the largest f16: rounding, and between the samples
   return true;
 }
-// one chain of n steps from the singular values sv (advanced to those behind the chain)
+// one chain of n steps from the singular values sv (advanced to those behind the chain).  False if the coefficients let the
+// iteration grow out of hand (or are not finite).
 static bool ortho_bounds(double *sv, int n, const OrthoCall &c, OrthoScale *o) {
   double r[ORTHO_SAMPLES], lam[ORTHO_SAMPLES], most = 0.;
   for (int i = 0; i < ORTHO_SAMPLES; ++i) {
@@ -496,153 +591,213 @@ static bool ortho_bounds(double *sv, int n, const OrthoCall &c, OrthoScale *o) {
       return false;
     an *= c.a;
   }
+  double mq = 0.;
   most = 0.;
   for (int i = 0; i < ORTHO_SAMPLES; ++i) {
+    mq = fmax(mq, fabs(an + r[i]));
     sv[i] *= an + r[i];
     if (!isfinite(sv[i])) return false;
     most = fmax(most, fabs(sv[i]));
   }
-  return ortho_scale_of(most, &o->x[1]);
+  return ortho_scale_of(mq, &o->q) && ortho_scale_of(most, &o->x[1]);
 }
 
-static void ortho_samples(double *sv) {
-  for (int i = 0; i < ORTHO_SAMPLES; ++i) sv[i] = 1.00001 * pow((double)i / (ORTHO_SAMPLES - 1), 3.);    // denser towards 0
-}
+// the products of one chain length, in order
+struct OrthoPlan {
+  struct {
+    OrthoJob job[2];
+    int jobs, type;
+  } level[3 * ORTHO_STEPS + ORTHO_STEPS];
+  int levels;
+  float x0;                         // scale of X0
+};
 
-static bool ortho_converges(const OrthoCall &c) {
+static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
   double sv[ORTHO_SAMPLES];
+  for (int i = 0; i < ORTHO_SAMPLES; ++i) {                              // denser towards 0
+    const double u = (double)i / (ORTHO_SAMPLES - 1);
+    sv[i] = 1.00001 * u * u * u;
+  }
+  p->levels = 0;
+  auto add = [p](int type, const OrthoJob &job) {
+    p->level[p->levels].type = type;
+    p->level[p->levels].jobs = 1;
+    p->level[p->levels++].job[0] = job;
+  };
   OrthoScale sc;
-  ortho_samples(sv);
-  for (int left = c.steps; left > 0;) {
-    const int n = left < ORTHO_CHAIN ? left : ORTHO_CHAIN;
-    if (!ortho_bounds(sv, n, c, &sc)) return false;
-    left -= n;
+  for (int left = c.steps, set = 0; left > 0; set ^= 1) {
+    const int chain = left < most ? left : most;
+    if (!ortho_bounds(sv, chain, c, &sc)) return false;
+    if (left == c.steps) p->x0 = sc.x[0];
+    const int x = set ? OB_X1 : OB_X0;
+    add(OL_SYM, OrthoJob{x, x, OB_NONE, OB_NONE, OB_A, sc.a[0] / (sc.x[0] * sc.x[0]), 0.f, 0.f, 0.f});
+    int r = OB_R0;                                                         // R of the first step is its S
+    float rs = sc.s[0], an = c.a;                                          // R's scale; a^k
+    for (int k = 0; k < chain; ++k) {
+      const bool more = k + 1 < chain;
+      const float sa = sc.a[k], ss = k || more ? sc.s[k] : sc.q;
+      const int s = k ? OB_S : OB_R0;
+      // S = b A + c A A (the whole chain's Q = a I + S if it is one step)
+      add(OL_SYM, OrthoJob{OB_A, OB_A, OB_A, OB_NONE, s, c.c * ss / (sa * sa), c.b * ss / sa, 0.f, k || more ? 0.f : an * ss});
+      if (!k && !more) rs = ss;
+      OrthoJob todo[2];
+      int jobs = 0;
+      if (more)                                                                                                    // T = a A + A S
+        todo[jobs++] = OrthoJob{OB_A, s, OB_A, OB_NONE, OB_T, sc.t[k] / (sa * ss), c.a * sc.t[k] / sa, 0.f, 0.f};
+      if (k) {                                                                            // R = a R + a^k S + R S (+ a^(k+1) I: Q)
+        const int to = r == OB_R0 ? OB_R1 : OB_R0;
+        const float sr = more ? sc.r[k] : sc.q;
+        todo[jobs++] = OrthoJob{r, s, r, s, to, sr / (rs * ss), c.a * sr / rs, an * sr / ss, more ? 0.f : an * c.a * sr};
+        r = to;
+        rs = sr;
+        an *= c.a;
+      }
+      if (jobs) {
+        add(OL_SYM, todo[0]);
+        p->level[p->levels - 1].job[1] = todo[1];
+        p->level[p->levels - 1].jobs = jobs;
+      }
+      if (more)                                                                                                    // A = a T + T S
+        add(OL_SYM, OrthoJob{OB_T, s, OB_T, OB_NONE, OB_A, sc.a[k + 1] / (sc.t[k] * ss), c.a * sc.a[k + 1] / sc.t[k], 0.f, 0.f});
+    }
+    left -= chain;
+    const float to = left > 0 ? sc.x[1] : 1.f;                                                                     // X = Q X
+    add(left > 0 ? OL_RECT : OL_LAST, OrthoJob{r, x, OB_NONE, OB_NONE, set ? OB_X0 : OB_X1, to / (rs * sc.x[0]), 0.f, 0.f, 0.f});
   }
   return true;
 }
 
+// ranges of the reduction: a product whose tiles leave CUs idle splits a long reduction, down to 256 columns of it a range
+#define ORTHO_KZ 32
+static int ortho_kz(int K, long own, long tiles) {
+  long z = 256 / (tiles > 0 ? tiles : 1);
+  if (own <= 16 && z < K / 1024) z = K / 1024;             // few tiles in the company of many: not the launch's last ones
+  if (z > K / 256) z = K / 256;
+  if (z > ORTHO_KZ) z = ORTHO_KZ;
+  return z < 2 ? 1 : (int)z;
+}
+
 struct OrthoLayout {
   size_t sums, data, bytes;
-  int total[ORTHO_KINDS];
+  OrthoFirst norm, split;
+  int norm_blocks, split_blocks;
+  int tile;                         // of the products
+  int kz[ORTHO_GROUPS];             // of the Gram matrices
 };
 
-// workspace: table | partial sums of squares | per group X, X^T (twice when the chain restarts) | per group the M x M matrices
+// workspace: table | partial sums of squares | per group X (two when there is more than one chain), the M x M matrices, the partial
+// Gram matrices
 static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
   OrthoLayout lo;
   memset(&lo, 0, sizeof lo);
   lo.sums = align_up(sizeof(OrthoTable), 256);
-  long parts = 0;
+  long parts = 0, tiles = 0;
   for (int i = 0; i < n; ++i) {
-    for (int k = 0; k < ORTHO_KINDS; ++k) {
-      g[i].first[k] = lo.total[k];
-      lo.total[k] += g[i].count * og_blocks(g[i], k);
-    }
+    g[i].chain = ortho_chain(g[i]);
+    lo.norm.b[i] = lo.norm_blocks;
+    lo.split.b[i] = lo.split_blocks;
+    lo.norm_blocks += g[i].count * og_norm_blocks(g[i]);
+    lo.split_blocks += g[i].count * og_split_blocks(g[i]);
     g[i].norm_off = (int)parts;
     parts += (long)g[i].count * og_norm_blocks(g[i]);
+    tiles += (long)g[i].count * og_tiles(g[i], OL_SYM, 64);
   }
   size_t at = lo.sums + align_up(parts * sizeof(double), 256);
   for (int i = 0; i < n; ++i) {
     const size_t M = og_pad(og_short(g[i])), N = og_pad(og_long(g[i]));
     g[i].x_off = (unsigned)(at / 256);
-    at += M * N * 4 * g[i].count * (steps > ORTHO_CHAIN ? 4 : 2);        // multiples of 64 x 64 x 4 bytes
+    at += M * N * 4 * g[i].count * (steps > g[i].chain ? 2 : 1);         // multiples of 64 x 64 x 4 bytes
     g[i].s_off = (unsigned)(at / 256);
     at += M * M * 4 * g[i].count * OB_SMALL;
+    g[i].p_off = (unsigned)(at / 256);
+    lo.kz[i] = ortho_kz((int)N, (long)g[i].count * og_tiles(g[i], OL_SYM, 64), tiles);
+    if (lo.kz[i] > 1) at += (size_t)lo.kz[i] * g[i].count * og_tiles(g[i], OL_SYM, 64) * 64 * 64 * 4;
   }
   lo.bytes = at;
   return lo;
 }
 
-template <int T, int KC, int LEVEL>
-static int ortho_launch(const OrthoTable *t, int n, char *ws, const OrthoLevel &lv, int jobs, hipStream_t st) {
-  const int lds = 4 * T * KC * 4;
-  if (const int rc = lds_optin(reinterpret_cast<const void *>(&ortho_product_kernel<T, KC, LEVEL>), lds, "ortho_product_kernel")) return rc;
-  hipLaunchKernelGGL((ortho_product_kernel<T, KC, LEVEL>), dim3(lv.blocks * jobs), dim3(256), lds, st, t, n, ws, lv);
+template <int T, int KC, int S, int WI, int WJ>
+static int ortho_launch(const OrthoTable *t, int n, char *ws, const OrthoLevel &lv, int blocks, hipStream_t st) {
+  const int lds = S * 2 * T * KC * 4;
+  if (const int rc = lds_optin(reinterpret_cast<const void *>(&ortho_product_kernel<T, KC, S, WI, WJ>), lds, "ortho_product_kernel")) return rc;
+  hipLaunchKernelGGL((ortho_product_kernel<T, KC, S, WI, WJ>), dim3(blocks), dim3(WI * WJ * 64), lds, st, t, n, ws, lv);
   return 0;
 }
 
-// 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs
-template <int LEVEL>
-static int ortho_product(const OrthoTable *t, int n, char *ws, const OrthoLayout &lo, OrthoLevel lv, int jobs, hipStream_t st) {
-  const int k128 = LEVEL == OL_SYM ? OK_SYM128 : OK_RECT128, k64 = LEVEL == OL_SYM ? OK_SYM64 : OK_RECT64;
-  if (lo.total[k128] * jobs >= 256) {
-    lv.blocks = lo.total[k128];
-    return ortho_launch<128, 32, LEVEL>(t, n, ws, lv, jobs, st);
-  }
-  lv.blocks = lo.total[k64];
-  return ortho_launch<64, 64, LEVEL>(t, n, ws, lv, jobs, st);
-}
-
-// one pass over at most ORTHO_GROUPS groups
-static int ortho_run(OrthoGroup *g, int n, const OrthoCall &c, char *ws, hipStream_t st) {
+// one pass over at most ORTHO_GROUPS groups and ORTHO_MATRICES pointers
+static int ortho_run(OrthoGroup *g, int n, const OrthoPtr *ptrs, int nptr, const OrthoCall &c, char *ws, hipStream_t st) {
   const OrthoLayout lo = ortho_layout(g, n, c.steps);
   OrthoTable *table = (OrthoTable *)ws;
   double *sums = (double *)(ws + lo.sums);
+  static thread_local OrthoPlan plan[ORTHO_CHAINS];
+  bool used[ORTHO_CHAINS] = {false};
+  int levels = 0;
+  float x0 = 1.f;
+  for (int i = 0; i < n; ++i) used[g[i].chain - 1] = true;
+  for (int k = 0; k < ORTHO_CHAINS; ++k)
+    if (used[k]) {
+      LSPS_CHECK_ARG(ortho_plan(&plan[k], k + 1, c), "newton_schulz: coefficients");
+      if (plan[k].levels > levels) levels = plan[k].levels;
+      x0 = plan[k].x0;                                                   // (the same for every chain length)
+    }
   for (int i = 0; i < n; i += ORTHO_TABLE_PART) {
     OrthoPart part;
     const int k = n - i < ORTHO_TABLE_PART ? n - i : ORTHO_TABLE_PART;
     memcpy(part.g, g + i, k * sizeof(OrthoGroup));
     hipLaunchKernelGGL(ortho_table_kernel, dim3(1), dim3(64), 0, st, part, table, i, k);
   }
-  double sv[ORTHO_SAMPLES];
-  OrthoScale sc;
-  ortho_samples(sv);
-  int left = c.steps, set = 0;
-  int chain = left < ORTHO_CHAIN ? left : ORTHO_CHAIN;
-  LSPS_CHECK_ARG(ortho_bounds(sv, chain, c, &sc), "newton_schulz: coefficients");
-  if (c.mode == OM_MUON) {
-    hipLaunchKernelGGL((ortho_norm_kernel<float, true>), dim3(lo.total[OK_NORM]), dim3(256), 0, st, table, n, sums, c.mo);
-    hipLaunchKernelGGL((ortho_split_kernel<float, true>), dim3(lo.total[OK_SPLIT]), dim3(256), 0, st, table, n, ws, sums, c.mo, c.eps, sc.x[0]);
-  } else if (!c.bf16) {
-    hipLaunchKernelGGL((ortho_norm_kernel<float, false>), dim3(lo.total[OK_NORM]), dim3(256), 0, st, table, n, sums, c.mo);
-    hipLaunchKernelGGL((ortho_split_kernel<float, false>), dim3(lo.total[OK_SPLIT]), dim3(256), 0, st, table, n, ws, sums, c.mo, c.eps, sc.x[0]);
-  } else {
-    hipLaunchKernelGGL((ortho_norm_kernel<__bf16, false>), dim3(lo.total[OK_NORM]), dim3(256), 0, st, table, n, sums, c.mo);
-    hipLaunchKernelGGL((ortho_split_kernel<__bf16, false>), dim3(lo.total[OK_SPLIT]), dim3(256), 0, st, table, n, ws, sums, c.mo, c.eps, sc.x[0]);
+  for (int i = 0; i < nptr; i += ORTHO_PTR_PART) {
+    OrthoPtrPart part;
+    const int k = nptr - i < ORTHO_PTR_PART ? nptr - i : ORTHO_PTR_PART;
+    memcpy(part.p, ptrs + i, k * sizeof(OrthoPtr));
+    hipLaunchKernelGGL(ortho_ptr_kernel, dim3(1), dim3(128), 0, st, part, table, i, k);
   }
-  while (left > 0) {
-    const OrthoJob none = {OB_A, OB_A, OB_NONE, OB_NONE, OB_A, OB_A, 0.f, 0.f, 0.f};
-    OrthoLevel lv = {{none, none}, 0, c.mode, c.decay};
-    const int x = set ? OB_X1 : OB_X0, xt = set ? OB_XT1 : OB_XT0;
-    lv.job[0] = OrthoJob{x, x, OB_NONE, OB_NONE, OB_A, OB_A, sc.a[0] / (sc.x[0] * sc.x[0]), 0.f, 0.f};
-    if (const int rc = ortho_product<OL_SYM>(table, n, ws, lo, lv, 1, st)) return rc;
-    int r = OB_R0;                                                         // R of the first step is its S
-    float rs = sc.s[0];                                                    // its scale
-    float an = c.a;                                                        // a^k
-    for (int k = 0; k < chain; ++k) {
-      const bool more = k + 1 < chain;
-      const float sa = sc.a[k], ss = sc.s[k];
-      const int s = k ? OB_S : OB_R0;
-      // S = b A + c A A
-      lv.job[0] = OrthoJob{OB_A, OB_A, OB_A, OB_NONE, s, s, c.c * ss / (sa * sa), c.b * ss / sa, 0.f};
-      if (const int rc = ortho_product<OL_SYM>(table, n, ws, lo, lv, 1, st)) return rc;
-      int jobs = 0;
-      if (more)                                                            // T = a A + A S
-        lv.job[jobs++] = OrthoJob{OB_A, s, OB_A, OB_NONE, OB_T, OB_T, sc.t[k] / (sa * ss), c.a * sc.t[k] / sa, 0.f};
-      if (k) {                                                             // R = a R + a^k S + R S
-        const int to = r == OB_R0 ? OB_R1 : OB_R0;
-        lv.job[jobs++] = OrthoJob{r, s, r, s, to, to, sc.r[k] / (rs * ss), c.a * sc.r[k] / rs, an * sc.r[k] / ss};
-        r = to;
-        rs = sc.r[k];
-        an *= c.a;
+#define ORTHO_PRE(T, MUON)                                                                                                        \
+  do {                                                                                                                            \
+    hipLaunchKernelGGL((ortho_norm_kernel<T, MUON>), dim3(lo.norm_blocks), dim3(256), 0, st, table, n, sums, c.mo, lo.norm);      \
+    hipLaunchKernelGGL((ortho_split_kernel<T, MUON>), dim3(lo.split_blocks), dim3(256), 0, st, table, n, ws, sums, c.mo, c.eps,   \
+                       x0, lo.split);                                                                                             \
+  } while (0)
+  if (c.mode == OM_MUON) ORTHO_PRE(float, true);
+  else if (!c.bf16) ORTHO_PRE(float, false);
+  else ORTHO_PRE(__bf16, false);
+#undef ORTHO_PRE
+  for (int l = 0; l < levels; ++l) {
+    OrthoLevel lv;
+    memset(&lv, 0, sizeof lv);
+    lv.mode = c.mode;
+    lv.decay = c.decay;
+    for (int k = 0; k < ORTHO_CHAINS; ++k)
+      if (used[k] && l < plan[k].levels) {
+        lv.type[k] = plan[k].level[l].type;
+        lv.jobs[k] = plan[k].level[l].jobs;
+        memcpy(lv.job[k], plan[k].level[l].job, sizeof lv.job[k]);
       }
-      if (jobs)
-        if (const int rc = ortho_product<OL_SYM>(table, n, ws, lo, lv, jobs, st)) return rc;
-      if (!more) break;
-      // A = a T + T S
-      lv.job[0] = OrthoJob{OB_T, s, OB_T, OB_NONE, OB_A, OB_A, sc.a[k + 1] / (sc.t[k] * ss), c.a * sc.a[k + 1] / sc.t[k], 0.f};
-      if (const int rc = ortho_product<OL_SYM>(table, n, ws, lo, lv, 1, st)) return rc;
+    // 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs
+    long b128 = 0;
+    for (int i = 0; i < n; ++i) {
+      const int k = g[i].chain - 1;
+      b128 += (long)g[i].count * lv.jobs[k] * og_tiles(g[i], lv.type[k], 128);
     }
-    left -= chain;
-    const float sx = sc.x[0], sx1 = sc.x[1];
-    if (left > 0) {                                                        // X = a^n X + R X, both ways round
-      lv.job[0] = OrthoJob{r, xt, x, OB_NONE, set ? OB_X0 : OB_X1, set ? OB_XT0 : OB_XT1, sx1 / (rs * sx), an * sx1 / sx, 0.f};
-      if (const int rc = ortho_product<OL_RECT>(table, n, ws, lo, lv, 1, st)) return rc;
-      set ^= 1;
-      chain = left < ORTHO_CHAIN ? left : ORTHO_CHAIN;
-      LSPS_CHECK_ARG(ortho_bounds(sv, chain, c, &sc), "newton_schulz: coefficients");
-    } else {
-      lv.job[0] = OrthoJob{r, xt, x, OB_NONE, OB_NONE, OB_NONE, 1.f / (rs * sx), an / sx, 0.f};
-      if (const int rc = ortho_product<OL_LAST>(table, n, ws, lo, lv, 1, st)) return rc;
+    const int T = b128 >= 256 ? 128 : 64;
+    bool split = false;
+    for (int pass = 0; pass < 2; ++pass) {
+      int blocks = 0;
+      lv.joining = pass;
+      for (int i = 0; i < n; ++i) {
+        const int k = g[i].chain - 1;
+        const bool gram = lv.jobs[k] && lv.type[k] == OL_SYM && lv.job[k][0].l >= OB_SMALL && T == 64;
+        lv.kz[i] = gram ? lo.kz[i] : 1;
+        split |= lv.kz[i] > 1;
+        lv.first.b[i] = blocks;
+        const long units = (long)g[i].count * lv.jobs[k] * og_tiles(g[i], lv.type[k], T) * (pass ? lv.kz[i] > 1 : lv.kz[i]);
+        blocks += (int)((units + 7) / 8 * 8);
+      }
+      if (!blocks) break;
+      const int rc = T == 128 ? ortho_launch<128, 32, 2, 2, 4>(table, n, ws, lv, blocks, st) : ortho_launch<64, 32, 3, 2, 2>(table, n, ws, lv, blocks, st);
+      if (rc) return rc;
+      if (!split) break;
     }
   }
   LSPS_CHECK_LAUNCH("newton_schulz");
@@ -655,21 +810,28 @@ using namespace lsps;
 
 extern "C" {
 
+static bool ortho_sane(const OrthoGroup &g) {
+  return g.rows > 0 && g.cols > 0 && g.count > 0 && g.rows <= 1 << 20 && g.cols <= 1 << 20 &&
+         (double)og_pad(g.rows) * og_pad(g.cols) <= (double)(1 << 29) &&      // a matrix of limbs: 32-bit offsets
+         (double)og_pad(g.rows) * og_pad(g.cols) * g.count <= (double)(1L << 36);
+}
+
 static int ortho_check(const char *what, OrthoGroup *g, int n, const OrthoCall &c, const void *ws, size_t ws_bytes) {
-  LSPS_CHECK_ARG(c.steps >= 1 && c.steps <= 64, "%s: %d steps (1 to 64)", what, c.steps);
+  LSPS_CHECK_ARG(c.steps >= 1 && c.steps <= ORTHO_STEPS, "%s: %d steps (1 to %d)", what, c.steps, ORTHO_STEPS);
   LSPS_CHECK_ARG(c.eps >= 0.f, "%s: eps %g", what, (double)c.eps);
-  LSPS_CHECK_ARG(ortho_converges(c), "%s: the iteration with (%g, %g, %g) leaves the range of its 16-bit limbs on [0, 1]", what, (double)c.a,
-                 (double)c.b, (double)c.c);
-  long blocks[ORTHO_KINDS] = {0};
+  static thread_local OrthoPlan plan;
+  bool used[ORTHO_CHAINS] = {false};
+  for (int i = 0; i < n; ++i) used[ortho_chain(g[i]) - 1] = true;
+  for (int k = 1; k <= ORTHO_CHAINS; ++k)
+    LSPS_CHECK_ARG(!used[k - 1] || ortho_plan(&plan, k, c), "%s: the iteration with (%g, %g, %g) leaves the range of its 16-bit limbs on [0, 1]", what,
+                   (double)c.a, (double)c.b, (double)c.c);
+  double blocks = 0;
   for (int i = 0; i < n; ++i) {
-    LSPS_CHECK_ARG(g[i].rows > 0 && g[i].cols > 0 && g[i].count > 0 && g[i].rows <= 1 << 20 && g[i].cols <= 1 << 20,
-                   "%s: %d matrices of %d x %d", what, g[i].count, g[i].rows, g[i].cols);
-    LSPS_CHECK_ARG((long)og_pad(g[i].rows) * og_pad(g[i].cols) <= 1L << 34, "%s: a matrix of %d x %d", what, g[i].rows, g[i].cols);
-    for (int k = 0; k < ORTHO_KINDS; ++k) {
-      blocks[k] += (long)g[i].count * og_blocks(g[i], k);
-      LSPS_CHECK_ARG(blocks[k] < 1L << 22, "%s: too many matrices for one call", what);
-    }
+    LSPS_CHECK_ARG(ortho_sane(g[i]), "%s: %d matrices of %d x %d", what, g[i].count, g[i].rows, g[i].cols);
+    // the finest launch: 64 x 64 tiles, two jobs or split reductions
+    blocks += (double)g[i].count * ((double)og_pad(g[i].rows) / 64 * og_pad(g[i].cols) / 64 + 8) * 2;
   }
+  LSPS_CHECK_ARG(blocks < (double)(1L << 23), "%s: too many matrices for one call", what);
   const size_t need = ortho_layout(g, n, c.steps).bytes;
   LSPS_CHECK_ARG(!((uintptr_t)ws & 15), "%s: the workspace is not 16-byte aligned", what);
   if (!ws || ws_bytes < need) {
@@ -685,12 +847,8 @@ static OrthoGroup ortho_group(int count, int rows, int cols) {
   g.count = count;
   g.rows = rows;
   g.cols = cols;
+  g.ptr = -1;
   return g;
-}
-
-static bool ortho_sane(const OrthoGroup &g) {
-  return g.rows > 0 && g.cols > 0 && g.count > 0 && g.rows <= 1 << 20 && g.cols <= 1 << 20 &&
-         (double)og_pad(g.rows) * og_pad(g.cols) * g.count <= 1e12;
 }
 
 size_t lsps_newton_schulz_workspace_bytes(int count, int rows, int cols, int steps) {
@@ -705,38 +863,60 @@ int lsps_newton_schulz(const void *g, void *out, int count, int rows, int cols, 
   LSPS_CHECK_ARG(g && out, "newton_schulz: null pointer");
   LSPS_CHECK_ARG(dtype == LSPS_F32 || dtype == LSPS_BF16, "newton_schulz: dtype %d (LSPS_F32 or LSPS_BF16)", dtype);
   OrthoGroup grp = ortho_group(count, rows, cols);
-  grp.g = g;
-  grp.out = out;
+  grp.base.g = g;
+  grp.base.out = out;
   const OrthoCall call = {steps, a, b, c, eps, dtype == LSPS_F32 ? OM_F32 : OM_BF16, dtype == LSPS_BF16, 1.f, {0.f, 1.f, 0}};
   if (const int rc = ortho_check("newton_schulz", &grp, 1, call, ws, ws_bytes)) return rc;
-  return ortho_run(&grp, 1, call, (char *)ws, (hipStream_t)stream);
+  return ortho_run(&grp, 1, nullptr, 0, call, (char *)ws, (hipStream_t)stream);
 }
 
-// the matrices of one pass: the largest of the call first, so that the long blocks of a product start first
-static int muon_pass(const LspsMuonMatrix *mats, int n, int at, float lr, float rms, OrthoGroup *g) {
-  const int k = n - at < ORTHO_GROUPS ? n - at : ORTHO_GROUPS;
-  for (int i = 0; i < k; ++i) {
-    const LspsMuonMatrix &m = mats[at + i];
-    OrthoGroup q = ortho_group(1, m.rows, m.cols);
-    q.g = m.g;
-    q.out = m.p;
-    q.m = m.m;
-    q.step = lr * rms * sqrtf((float)(m.rows > m.cols ? m.rows : m.cols));
-    int j = i;
-    for (; j > 0 && og_long(g[j - 1]) < og_long(q); --j) g[j] = g[j - 1];
-    g[j] = q;
+// The next pass of a Muon step from matrix `at` on: as many as fit ORTHO_GROUPS shapes and ORTHO_MATRICES pointers, sorted into
+// shapes, the longest shapes first (the long blocks of a product start first).  Returns the number of matrices taken.
+struct MuonPass {
+  OrthoGroup g[ORTHO_GROUPS];
+  OrthoPtr ptr[ORTHO_MATRICES];
+  int n, taken;
+};
+static void muon_pass(const LspsMuonMatrix *mats, int n, int at, float lr, float rms, MuonPass *p) {
+  int shape[ORTHO_MATRICES];
+  p->n = p->taken = 0;
+  for (; at + p->taken < n && p->taken < ORTHO_MATRICES; ++p->taken) {
+    const LspsMuonMatrix &m = mats[at + p->taken];
+    int k = 0;
+    while (k < p->n && (p->g[k].rows != m.rows || p->g[k].cols != m.cols)) ++k;
+    if (k == p->n) {
+      if (p->n == ORTHO_GROUPS) break;
+      p->g[p->n] = ortho_group(0, m.rows, m.cols);
+      p->g[p->n++].step = lr * rms * sqrtf((float)(m.rows > m.cols ? m.rows : m.cols));
+    }
+    ++p->g[k].count;
+    shape[p->taken] = k;
   }
-  return k;
+  int order[ORTHO_GROUPS], next = 0;
+  for (int i = 0; i < p->n; ++i) {
+    int j = i;
+    for (; j > 0 && og_long(p->g[order[j - 1]]) < og_long(p->g[i]); --j) order[j] = order[j - 1];
+    order[j] = i;
+  }
+  OrthoGroup sorted[ORTHO_GROUPS];
+  for (int i = 0; i < p->n; ++i) {
+    sorted[i] = p->g[order[i]];
+    sorted[i].ptr = next;
+    for (int k = 0; k < p->taken; ++k)
+      if (shape[k] == order[i]) p->ptr[next++] = OrthoPtr{mats[at + k].g, mats[at + k].p, mats[at + k].m};
+  }
+  memcpy(p->g, sorted, p->n * sizeof(OrthoGroup));
 }
 
 size_t lsps_muon_workspace_bytes(const LspsMuonMatrix *mats, int n, int steps) {
+  static thread_local MuonPass p;
   size_t most = 0;
   if (!mats || n < 1 || steps < 1) return 0;
   for (int i = 0; i < n; ++i)
     if (!ortho_sane(ortho_group(1, mats[i].rows, mats[i].cols))) return 0;
-  for (int at = 0; at < n; at += ORTHO_GROUPS) {
-    OrthoGroup g[ORTHO_GROUPS];
-    const size_t need = ortho_layout(g, muon_pass(mats, n, at, 0.f, 0.f, g), steps).bytes;
+  for (int at = 0; at < n; at += p.taken) {
+    muon_pass(mats, n, at, 0.f, 0.f, &p);
+    const size_t need = ortho_layout(p.g, p.n, steps).bytes;
     if (need > most) most = need;
   }
   return most;
@@ -744,18 +924,25 @@ size_t lsps_muon_workspace_bytes(const LspsMuonMatrix *mats, int n, int steps) {
 
 int lsps_muon_step(const LspsMuonMatrix *mats, int n, float lr, float momentum, int nesterov, float weight_decay, float rms, float grad_scale,
                    int steps, float a, float b, float c, float eps, void *ws, size_t ws_bytes, void *stream) {
+  static thread_local MuonPass p;
   (void)hipGetLastError();   // clear stale sticky errors left by other users of the runtime
   LSPS_CHECK_ARG(mats && n > 0, "muon_step: no matrices");
   LSPS_CHECK_ARG(isfinite(lr) && isfinite(weight_decay) && isfinite(rms) && isfinite(grad_scale) && momentum >= 0.f && momentum < 1.f,
                  "muon_step: lr %g, momentum %g, weight decay %g, rms %g, gradient scale %g", (double)lr, (double)momentum,
                  (double)weight_decay, (double)rms, (double)grad_scale);
-  for (int i = 0; i < n; ++i) LSPS_CHECK_ARG(mats[i].p && mats[i].g && mats[i].m, "muon_step: null pointer in matrix %d", i);
+  for (int i = 0; i < n; ++i) {
+    LSPS_CHECK_ARG(mats[i].p && mats[i].g && mats[i].m, "muon_step: null pointer in matrix %d", i);
+    LSPS_CHECK_ARG(ortho_sane(ortho_group(1, mats[i].rows, mats[i].cols)), "muon_step: matrix %d of %d x %d", i, mats[i].rows, mats[i].cols);
+  }
   const OrthoCall call = {steps, a, b, c, eps, OM_MUON, false, 1.f - lr * weight_decay, {momentum, grad_scale, nesterov != 0}};
-  OrthoGroup g[ORTHO_GROUPS];
-  for (int at = 0; at < n; at += ORTHO_GROUPS)
-    if (const int rc = ortho_check("muon_step", g, muon_pass(mats, n, at, lr, rms, g), call, ws, ws_bytes)) return rc;
-  for (int at = 0; at < n; at += ORTHO_GROUPS)
-    if (const int rc = ortho_run(g, muon_pass(mats, n, at, lr, rms, g), call, (char *)ws, (hipStream_t)stream)) return rc;
+  for (int at = 0; at < n; at += p.taken) {
+    muon_pass(mats, n, at, lr, rms, &p);
+    if (const int rc = ortho_check("muon_step", p.g, p.n, call, ws, ws_bytes)) return rc;
+  }
+  for (int at = 0; at < n; at += p.taken) {
+    muon_pass(mats, n, at, lr, rms, &p);
+    if (const int rc = ortho_run(p.g, p.n, p.ptr, p.taken, call, (char *)ws, (hipStream_t)stream)) return rc;
+  }
   return 0;
 }
 
