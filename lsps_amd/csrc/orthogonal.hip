@@ -19,7 +19,8 @@
 // of 64: a 32-deep chunk of a row is one 128-byte line and the rows of a chunk follow each other, so that a tile's chunk is one
 // contiguous run over all L2 channels (rows at a power-of-two pitch all fell on one channel: 2100 instead of 768 cycles per chunk
 // of a 128 x 128 tile at 2048 x 2048).  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.
-// All matrices of a call go through one launch per product (the blocks find their matrix in a table in the workspace).
+// All matrices of a call go through one launch per product (a block finds its group of equal matrices in the kernel's arguments).
+#include <limits.h>
 #include <math.h>
 #include <string.h>
 
@@ -35,11 +36,10 @@ typedef float og_f4 __attribute__((ext_vector_type(4)));
 typedef float og_f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short og_u4u __attribute__((ext_vector_type(4), aligned(2)));
 
-#define ORTHO_GROUPS 64        // shapes per pass (the blocks search them with one ballot)
+#define ORTHO_GROUPS 16        // shapes per pass (they travel in the kernels' arguments)
 #define ORTHO_MATRICES 1024    // matrices with pointers of their own per pass
 #define ORTHO_CHAINS 3         // longest chain: steps between two Gram matrices of the long side
 #define ORTHO_NORM_BLOCK 16384 // elements per block of the norm pass
-#define ORTHO_TABLE_PART 24    // groups, and
 #define ORTHO_PTR_PART 96      // matrices per table launch (passed by value: nothing on the host has to outlive the call)
 #define ORTHO_STEPS 64
 enum { OB_A, OB_S, OB_T, OB_R0, OB_R1, OB_SMALL, OB_X0 = OB_SMALL, OB_X1, OB_NONE };
@@ -52,25 +52,22 @@ struct OrthoPtr {
   float *m;            // OM_MUON: the momentum
 };
 
-// `count` matrices of one shape
+// `count` matrices of one shape, and what one launch does with them.  48 bytes: a lane fetches a group's
 struct OrthoGroup {
-  OrthoPtr base;                  // ptr < 0: the matrices lie one behind the other from here on
-  int ptr;                        // else: the first of their pointers in the table
-  unsigned x_off, s_off, p_off;   // workspace offsets in 256-byte units: long-side matrices, M x M matrices, partial products
-  int norm_off;                   // first of the matrices' partial sums of squares
+  int first;                      // blocks in front of the group's
+  int aux;                        // norm and split passes: partial sums of squares in front of the group's; a product: ranges of its reduction
+  int type, jobs;                 // a product: OL_*, and how many of them
   int rows, cols, count;
-  int chain;                      // steps between two Gram matrices
+  int ptr;                        // first of the matrices' pointers in the table; < 0: they lie one behind the other
+  unsigned x_off, s_off, p_off;   // workspace offsets in 256-byte units: long-side matrices, M x M matrices, partial products
   float step;                     // OM_MUON: lr rms sqrt(max(rows, cols))
 };
-
-struct OrthoTable {
-  OrthoGroup g[ORTHO_GROUPS];
-  OrthoPtr ptr[ORTHO_MATRICES];
+struct OrthoGroups {
+  OrthoGroup g[ORTHO_GROUPS];     // (first = INT_MAX behind the last one)
+  OrthoPtr base;                  // the only group's matrices if they lie one behind the other
+  const OrthoPtr *table;
 };
 
-struct OrthoPart {
-  OrthoGroup g[ORTHO_TABLE_PART];
-};
 struct OrthoPtrPart {
   OrthoPtr p[ORTHO_PTR_PART];
 };
@@ -88,28 +85,35 @@ __host__ __device__ static inline int og_tiles(const OrthoGroup &g, int type, in
   return type == OL_SYM ? m * (m + 1) / 2 : m * n;
 }
 
-__global__ void ortho_table_kernel(OrthoPart part, OrthoTable *t, int base, int n) {
-  if ((int)threadIdx.x < n) t->g[base + threadIdx.x] = part.g[threadIdx.x];
-}
-__global__ void ortho_ptr_kernel(OrthoPtrPart part, OrthoTable *t, int base, int n) {
-  if ((int)threadIdx.x < n) t->ptr[base + threadIdx.x] = part.p[threadIdx.x];
+__global__ void ortho_ptr_kernel(OrthoPtrPart part, OrthoPtr *t, int base, int n) {
+  if ((int)threadIdx.x < n) t[base + threadIdx.x] = part.p[threadIdx.x];
 }
 
-// first block of every group in a launch
-struct OrthoFirst {
-  int b[ORTHO_GROUPS];
-};
-// the group of block b: the last one whose first block is not behind it
-__device__ __forceinline__ int ortho_group_of(const OrthoFirst &first, int n, int b) {
+template <typename T>
+__device__ __forceinline__ T og_readlane(const T &v, int lane) {
+  constexpr int W = sizeof(T) / 4;
+  int w[W];
+  __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+  for (int i = 0; i < W; ++i) w[i] = __builtin_amdgcn_readlane(w[i], lane);
+  T r;
+  __builtin_memcpy(&r, w, sizeof(T));
+  return r;
+}
+
+// The group of block b (the last one whose first block is not behind it): lane i looks at group i, so that one trip to the
+// arguments' memory brings them all (through a table and its index it was three, 1.2 us of every launch).
+__device__ __forceinline__ OrthoGroup ortho_group_of(const OrthoGroups &gs, int b, int &index) {
   const int lane = threadIdx.x & 63;
-  const bool le = lane < n && first.b[lane] <= b;
-  return __builtin_amdgcn_readfirstlane(63 - __clzll(__ballot(le)));
+  const OrthoGroup mine = gs.g[lane < ORTHO_GROUPS ? lane : 0];
+  index = __builtin_amdgcn_readfirstlane(63 - __clzll(__ballot(lane < ORTHO_GROUPS && mine.first <= b)));
+  return og_readlane(mine, index);
 }
 
-__device__ __forceinline__ OrthoPtr ortho_ptr(const OrthoTable *t, const OrthoGroup &g, int mat, int bytes) {
-  if (g.ptr >= 0) return t->ptr[g.ptr + mat];
+__device__ __forceinline__ OrthoPtr ortho_ptr(const OrthoGroups &gs, const OrthoGroup &g, int mat, int bytes) {
+  if (g.ptr >= 0) return gs.table[g.ptr + mat];
   const long o = (long)g.rows * g.cols * mat * bytes;
-  return OrthoPtr{(const char *)g.base.g + o, (char *)g.base.out + o, nullptr};
+  return OrthoPtr{(const char *)gs.base.g + o, (char *)gs.base.out + o, nullptr};
 }
 
 __device__ __forceinline__ char *ortho_buffer(char *ws, const OrthoGroup &g, int id, int mat) {
@@ -148,14 +152,13 @@ struct OrthoMomentum {
 // sums of squares of G in 64 bits (squares of f32 values neither overflow nor vanish there), one partial sum per block; Muon:
 // the momentum is updated on the way.  Memory bound: 4 (Muon: 12) bytes per element.
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable *__restrict__ t, int n, double *__restrict__ sums,
-                                                         OrthoMomentum mo, OrthoFirst first) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroups gs, double *__restrict__ sums, OrthoMomentum mo) {
   __shared__ double red[4];
-  const int grp = ortho_group_of(first, n, blockIdx.x);
-  const OrthoGroup g = t->g[grp];
-  const int rel = blockIdx.x - first.b[grp], nb = og_norm_blocks(g), mat = rel / nb, tile = rel - mat * nb;
+  int grp;
+  const OrthoGroup g = ortho_group_of(gs, blockIdx.x, grp);
+  const int rel = blockIdx.x - g.first, nb = og_norm_blocks(g), mat = rel / nb, tile = rel - mat * nb;
   const long size = (long)g.rows * g.cols, lo = (long)tile * ORTHO_NORM_BLOCK;
-  const OrthoPtr ptr = ortho_ptr(t, g, mat, sizeof(T));
+  const OrthoPtr ptr = ortho_ptr(gs, g, mat, sizeof(T));
   const T *src = (const T *)ptr.g;
   float *m = ptr.m;
   double s = 0.;
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable *__res
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) sums[g.norm_off + rel] = red[0] + red[1] + red[2] + red[3];
+  if (threadIdx.x == 0) sums[g.aux + rel] = red[0] + red[1] + red[2] + red[3];
 }
 
 __device__ __forceinline__ void og_split(float v, _Float16 &hi, _Float16 &lo) {
@@ -198,16 +201,15 @@ __device__ __forceinline__ void og_split(float v, _Float16 &hi, _Float16 &lo) {
 
 // X0 as limbs, the short side in rows.  One 64 x 64 tile of G per block, through LDS (turned round there for a tall G).
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_split_kernel(const OrthoTable *__restrict__ t, int n, char *__restrict__ ws,
-                                                          const double *__restrict__ sums, OrthoMomentum mo, float eps, float scale,
-                                                          OrthoFirst first) {
+__global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroups gs, char *__restrict__ ws, const double *__restrict__ sums,
+                                                          OrthoMomentum mo, float eps, float scale) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
-  const int grp = ortho_group_of(first, n, blockIdx.x);
-  const OrthoGroup g = t->g[grp];
-  const int rel = blockIdx.x - first.b[grp], per = og_split_blocks(g), mat = rel / per, tix = rel - mat * per;
+  int grp;
+  const OrthoGroup g = ortho_group_of(gs, blockIdx.x, grp);
+  const int rel = blockIdx.x - g.first, per = og_split_blocks(g), mat = rel / per, tix = rel - mat * per;
   const int nb = og_norm_blocks(g);
-  const double *part = sums + g.norm_off + (long)mat * nb;
+  const double *part = sums + g.aux + (long)mat * nb;
   double s = 0.;
   for (int i = threadIdx.x; i < nb; i += 256) s += part[i];
 #pragma unroll
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const OrthoTable *__re
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   const int tc = og_pad(g.cols) / 64;
   const int r0 = tix / tc * 64, c0 = (tix - tix / tc * tc) * 64;
-  const OrthoPtr ptr = ortho_ptr(t, g, mat, sizeof(T));
+  const OrthoPtr ptr = ortho_ptr(gs, g, mat, sizeof(T));
   const T *src = (const T *)ptr.g;
   const float *m = ptr.m;
   float v[4][4];
@@ -264,13 +266,10 @@ struct OrthoJob {
   int l, r, e1, e2, out;
   float k0, k1, k2, diag;
 };
-// one launch: per chain length the product its groups are at (they walk their own lists side by side)
 struct OrthoLevel {
-  OrthoFirst first;
-  int kz[ORTHO_GROUPS];             // ranges the reduction of a group's product is split into
-  OrthoJob job[ORTHO_CHAINS][2];
-  int jobs[ORTHO_CHAINS], type[ORTHO_CHAINS];
-  int joining;                      // second launch of a split product: add the ranges up
+  OrthoGroups gs;
+  OrthoJob job[ORTHO_GROUPS * 2];   // of group i: 2 i, 2 i + 1
+  int joining;                      // second launch of a split product: the ranges it was split into
   int mode;                         // of the last level: OM_*
   float decay;                      // 1 - lr wd
 };
@@ -286,21 +285,23 @@ struct OrthoLevel {
 // A product with few tiles and a long reduction is split into kz ranges of it: f32 partial tiles in the workspace, added in a
 // fixed order by a second launch of this kernel.
 template <int T, int KC, int S, int WI, int WJ>
-__global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(const OrthoTable *__restrict__ t, int n, char *__restrict__ ws, OrthoLevel lv) {
+__global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
   constexpr int WAVES = WI * WJ, SUB = KC / 32, STAGE = T * KC * 4, PIECES = T * SUB / 8 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = 144;
   static_assert(S * 2 * STAGE >= WAVES * 32 * TP, "the transpose of the epilogue reuses the stages");
   static_assert((S - 2) * 2 * PIECES < 64, "the range of s_waitcnt vmcnt");
   extern __shared__ __align__(1024) char smem[];
-  const int grp = ortho_group_of(lv.first, n, blockIdx.x);
-  const OrthoGroup g = t->g[grp];
-  const int cls = g.chain - 1, type = lv.type[cls], kz = lv.joining ? 1 : lv.kz[grp];
+  const int lane = threadIdx.x & 63;
+  const OrthoJob mine = lv.job[lane < 2 * ORTHO_GROUPS ? lane : 0];
+  int grp;
+  const OrthoGroup g = ortho_group_of(lv.gs, blockIdx.x, grp);
+  const int type = g.type, kz = lv.joining ? 1 : g.aux;
   const int M = og_pad(og_short(g)), N = og_pad(og_long(g));
-  const int per = og_tiles(g, type, T) * kz, total = per * g.count * lv.jobs[cls];
+  const int per = og_tiles(g, type, T) * kz, total = per * g.count * g.jobs;
   // consecutive blocks go to the eight XCDs in turn: block x + 8 y takes unit x q + y, so that an XCD's blocks share operands in its L2
-  const int rel = blockIdx.x - lv.first.b[grp], q8 = (total + 7) / 8, unit0 = (rel & 7) * q8 + (rel >> 3);
+  const int rel = blockIdx.x - g.first, q8 = (total + 7) / 8, unit0 = (rel & 7) * q8 + (rel >> 3);
   if ((rel >> 3) >= q8 || unit0 >= total) return;
   const int second = unit0 >= per * g.count;
-  const OrthoJob job = lv.job[cls][second];
+  const OrthoJob job = og_readlane(mine, __builtin_amdgcn_readfirstlane(grp * 2 + second));
   const int u1 = unit0 - second * per * g.count, mat = u1 / per, u2 = u1 - mat * per, z = u2 % kz, tile = u2 / kz;
   int bi, bj;
   if (type == OL_SYM) {
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(const Or
   const int cols = type == OL_SYM ? M : N;                       // of the result; rows: M
   const int K = job.l >= OB_SMALL ? N : M;
   const int chunks = K / KC, c0 = (int)((long)chunks * z / kz), c1 = (int)((long)chunks * (z + 1) / kz);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ, l31 = lane & 31, lh = lane >> 5;
   og_f16v acc[FI][FJ], acx[FI][FJ];
 #pragma unroll
@@ -326,6 +327,23 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(const Or
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = acx[i][j][e] = 0.f;
   float *part = reinterpret_cast<float *>(ws + (size_t)g.p_off * 256);   // [mat][tile][z][fi][fj][q][thread][4]
+  const char *e1 = job.e1 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e1, mat);
+  const char *e2 = job.e2 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e2, mat);
+  // one fragment per wave: E1 and E2 are fetched in front of the product, whose first requests they precede
+  constexpr bool EARLY = FI * FJ == 1;
+  og_h4 eh[EARLY ? 8 : 1], el[EARLY ? 8 : 1];
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const char *e = q < 4 ? e1 : e2;
+      const int i = (bi * WI + wi) * 32 + l31, j = (bj * WJ + wj) * 32 + (q & 3) * 8 + lh * 4;
+      if (e) {
+        const og_h4 *p = reinterpret_cast<const og_h4 *>(e + og_at(M, i, j));
+        eh[q] = p[0];
+        el[q] = p[2];
+      }
+    }
+  }
   if (!lv.joining) {
     // a piece = 8 lines of 128 bytes = one DMA request of a wave: [sub-chunk of 32][line], line = row of the tile; for X in
     // OL_RECT / OL_LAST: [32 columns][row of the chunk].  Unit u of line r lies at u ^ (r / 2): 16 lanes reading 16 consecutive
@@ -420,7 +438,7 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(const Or
       return;
     }
   } else {
-    const int nz = lv.kz[grp];
+    const int nz = g.aux;
     const og_f4 *src = reinterpret_cast<const og_f4 *>(part) + (long)(mat * per + tile) * nz * (T * T / 4) + threadIdx.x;
     for (int k = 0; k < nz; ++k, src += T * T / 4)
 #pragma unroll
@@ -434,16 +452,21 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(const Or
             for (int e = 0; e < 4; ++e) acc[i][j][q * 4 + e] += v[e];
           }
   }
-  const char *e1 = job.e1 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e1, mat);
-  const char *e2 = job.e2 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e2, mat);
-  auto stored = [&](const char *e, int i, int j, float (&v)[4]) {        // 4 stored values of row i from column j on
-    const og_h4 *p = reinterpret_cast<const og_h4 *>(e + og_at(M, i, j));
-    const og_h4 h = p[0], l = p[2];
+  auto stored = [&](int which, int q, int i, int j, float (&v)[4]) {     // 4 stored values of row i from column j on
+    og_h4 h, l;
+    if constexpr (EARLY) {
+      h = eh[which * 4 + q];
+      l = el[which * 4 + q];
+    } else {
+      const og_h4 *p = reinterpret_cast<const og_h4 *>((which ? e2 : e1) + og_at(M, i, j));
+      h = p[0];
+      l = p[2];
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = (float)h[k] + (float)l[k];
   };
   const bool last = type == OL_LAST, mirrored = type == OL_SYM && bi != bj;
-  const OrthoPtr ptr = ortho_ptr(t, g, mat, lv.mode == OM_BF16 ? 2 : 4);
+  const OrthoPtr ptr = ortho_ptr(lv.gs, g, mat, lv.mode == OM_BF16 ? 2 : 4);
   const int m = og_short(g), nn = og_long(g);
   const bool tall = g.rows > g.cols;
   char *out = last ? nullptr : ortho_buffer(ws, g, job.out, mat);
@@ -462,12 +485,12 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(const Or
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = job.k0 * (acc[fi][fj][q * 4 + k] + acx[fi][fj][q * 4 + k]);
         if (e1) {
-          stored(e1, i, j, x);
+          stored(0, q, i, j, x);
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = fmaf(job.k1, x[k], v[k]);
         }
         if (e2) {
-          stored(e2, i, j, x);
+          stored(1, q, i, j, x);
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = fmaf(job.k2, x[k], v[k]);
         }
@@ -678,35 +701,33 @@ static int ortho_kz(int K, long own, long tiles) {
 }
 
 struct OrthoLayout {
-  size_t sums, data, bytes;
-  OrthoFirst norm, split;
-  int norm_blocks, split_blocks;
-  int tile;                         // of the products
+  size_t sums, bytes;
+  int chain[ORTHO_GROUPS];
   int kz[ORTHO_GROUPS];             // of the Gram matrices
+  int norm_first[ORTHO_GROUPS], split_first[ORTHO_GROUPS];
+  int norm_blocks, split_blocks;
 };
 
-// workspace: table | partial sums of squares | per group X (two when there is more than one chain), the M x M matrices, the partial
-// Gram matrices
+// workspace: pointers | partial sums of squares | per group X (two when there is more than one chain), the M x M matrices, the
+// partial Gram matrices
 static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
   OrthoLayout lo;
   memset(&lo, 0, sizeof lo);
-  lo.sums = align_up(sizeof(OrthoTable), 256);
-  long parts = 0, tiles = 0;
+  lo.sums = align_up(sizeof(OrthoPtr) * ORTHO_MATRICES, 256);
+  long tiles = 0;
   for (int i = 0; i < n; ++i) {
-    g[i].chain = ortho_chain(g[i]);
-    lo.norm.b[i] = lo.norm_blocks;
-    lo.split.b[i] = lo.split_blocks;
+    lo.chain[i] = ortho_chain(g[i]);
+    lo.norm_first[i] = lo.norm_blocks;
+    lo.split_first[i] = lo.split_blocks;
     lo.norm_blocks += g[i].count * og_norm_blocks(g[i]);
     lo.split_blocks += g[i].count * og_split_blocks(g[i]);
-    g[i].norm_off = (int)parts;
-    parts += (long)g[i].count * og_norm_blocks(g[i]);
     tiles += (long)g[i].count * og_tiles(g[i], OL_SYM, 64);
   }
-  size_t at = lo.sums + align_up(parts * sizeof(double), 256);
+  size_t at = lo.sums + align_up(lo.norm_blocks * sizeof(double), 256);
   for (int i = 0; i < n; ++i) {
     const size_t M = og_pad(og_short(g[i])), N = og_pad(og_long(g[i]));
     g[i].x_off = (unsigned)(at / 256);
-    at += M * N * 4 * g[i].count * (steps > g[i].chain ? 2 : 1);         // multiples of 64 x 64 x 4 bytes
+    at += M * N * 4 * g[i].count * (steps > lo.chain[i] ? 2 : 1);        // multiples of 64 x 64 x 4 bytes
     g[i].s_off = (unsigned)(at / 256);
     at += M * M * 4 * g[i].count * OB_SMALL;
     g[i].p_off = (unsigned)(at / 256);
@@ -718,86 +739,84 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
 }
 
 template <int T, int KC, int S, int WI, int WJ>
-static int ortho_launch(const OrthoTable *t, int n, char *ws, const OrthoLevel &lv, int blocks, hipStream_t st) {
+static int ortho_launch(char *ws, const OrthoLevel &lv, int blocks, hipStream_t st) {
   const int lds = S * 2 * T * KC * 4;
   if (const int rc = lds_optin(reinterpret_cast<const void *>(&ortho_product_kernel<T, KC, S, WI, WJ>), lds, "ortho_product_kernel")) return rc;
-  hipLaunchKernelGGL((ortho_product_kernel<T, KC, S, WI, WJ>), dim3(blocks), dim3(WI * WJ * 64), lds, st, t, n, ws, lv);
+  hipLaunchKernelGGL((ortho_product_kernel<T, KC, S, WI, WJ>), dim3(blocks), dim3(WI * WJ * 64), lds, st, ws, lv);
   return 0;
 }
 
 // one pass over at most ORTHO_GROUPS groups and ORTHO_MATRICES pointers
-static int ortho_run(OrthoGroup *g, int n, const OrthoPtr *ptrs, int nptr, const OrthoCall &c, char *ws, hipStream_t st) {
+static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr *ptrs, int nptr, const OrthoCall &c, char *ws, hipStream_t st) {
   const OrthoLayout lo = ortho_layout(g, n, c.steps);
-  OrthoTable *table = (OrthoTable *)ws;
   double *sums = (double *)(ws + lo.sums);
   static thread_local OrthoPlan plan[ORTHO_CHAINS];
   bool used[ORTHO_CHAINS] = {false};
   int levels = 0;
   float x0 = 1.f;
-  for (int i = 0; i < n; ++i) used[g[i].chain - 1] = true;
+  for (int i = 0; i < n; ++i) used[lo.chain[i] - 1] = true;
   for (int k = 0; k < ORTHO_CHAINS; ++k)
     if (used[k]) {
       LSPS_CHECK_ARG(ortho_plan(&plan[k], k + 1, c), "newton_schulz: coefficients");
       if (plan[k].levels > levels) levels = plan[k].levels;
       x0 = plan[k].x0;                                                   // (the same for every chain length)
     }
-  for (int i = 0; i < n; i += ORTHO_TABLE_PART) {
-    OrthoPart part;
-    const int k = n - i < ORTHO_TABLE_PART ? n - i : ORTHO_TABLE_PART;
-    memcpy(part.g, g + i, k * sizeof(OrthoGroup));
-    hipLaunchKernelGGL(ortho_table_kernel, dim3(1), dim3(64), 0, st, part, table, i, k);
-  }
   for (int i = 0; i < nptr; i += ORTHO_PTR_PART) {
     OrthoPtrPart part;
     const int k = nptr - i < ORTHO_PTR_PART ? nptr - i : ORTHO_PTR_PART;
     memcpy(part.p, ptrs + i, k * sizeof(OrthoPtr));
-    hipLaunchKernelGGL(ortho_ptr_kernel, dim3(1), dim3(128), 0, st, part, table, i, k);
+    hipLaunchKernelGGL(ortho_ptr_kernel, dim3(1), dim3(128), 0, st, part, (OrthoPtr *)ws, i, k);
   }
-#define ORTHO_PRE(T, MUON)                                                                                                        \
-  do {                                                                                                                            \
-    hipLaunchKernelGGL((ortho_norm_kernel<T, MUON>), dim3(lo.norm_blocks), dim3(256), 0, st, table, n, sums, c.mo, lo.norm);      \
-    hipLaunchKernelGGL((ortho_split_kernel<T, MUON>), dim3(lo.split_blocks), dim3(256), 0, st, table, n, ws, sums, c.mo, c.eps,   \
-                       x0, lo.split);                                                                                             \
+  OrthoLevel lv;
+  memset(&lv, 0, sizeof lv);
+  lv.mode = c.mode;
+  lv.decay = c.decay;
+  lv.gs.base = base;
+  lv.gs.table = (const OrthoPtr *)ws;
+  for (int i = 0; i < ORTHO_GROUPS; ++i) {
+    if (i < n) lv.gs.g[i] = g[i];
+    lv.gs.g[i].first = i < n ? lo.norm_first[i] : INT_MAX;
+    lv.gs.g[i].aux = lo.norm_first[i];
+  }
+  OrthoGroups split = lv.gs;
+  for (int i = 0; i < n; ++i) split.g[i].first = lo.split_first[i];
+#define ORTHO_PRE(T, MUON)                                                                                                            \
+  do {                                                                                                                                \
+    hipLaunchKernelGGL((ortho_norm_kernel<T, MUON>), dim3(lo.norm_blocks), dim3(256), 0, st, lv.gs, sums, c.mo);                      \
+    hipLaunchKernelGGL((ortho_split_kernel<T, MUON>), dim3(lo.split_blocks), dim3(256), 0, st, split, ws, sums, c.mo, c.eps, x0);     \
   } while (0)
   if (c.mode == OM_MUON) ORTHO_PRE(float, true);
   else if (!c.bf16) ORTHO_PRE(float, false);
   else ORTHO_PRE(__bf16, false);
 #undef ORTHO_PRE
   for (int l = 0; l < levels; ++l) {
-    OrthoLevel lv;
-    memset(&lv, 0, sizeof lv);
-    lv.mode = c.mode;
-    lv.decay = c.decay;
-    for (int k = 0; k < ORTHO_CHAINS; ++k)
-      if (used[k] && l < plan[k].levels) {
-        lv.type[k] = plan[k].level[l].type;
-        lv.jobs[k] = plan[k].level[l].jobs;
-        memcpy(lv.job[k], plan[k].level[l].job, sizeof lv.job[k]);
-      }
-    // 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs
     long b128 = 0;
     for (int i = 0; i < n; ++i) {
-      const int k = g[i].chain - 1;
-      b128 += (long)g[i].count * lv.jobs[k] * og_tiles(g[i], lv.type[k], 128);
+      const OrthoPlan &p = plan[lo.chain[i] - 1];
+      lv.gs.g[i].type = l < p.levels ? p.level[l].type : OL_SYM;
+      lv.gs.g[i].jobs = l < p.levels ? p.level[l].jobs : 0;
+      if (l < p.levels) memcpy(lv.job + 2 * i, p.level[l].job, sizeof p.level[l].job);
+      b128 += (long)g[i].count * lv.gs.g[i].jobs * og_tiles(g[i], lv.gs.g[i].type, 128);
     }
+    // 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs
     const int T = b128 >= 256 ? 128 : 64;
-    bool split = false;
+    bool split_any = false;
     for (int pass = 0; pass < 2; ++pass) {
       int blocks = 0;
       lv.joining = pass;
       for (int i = 0; i < n; ++i) {
-        const int k = g[i].chain - 1;
-        const bool gram = lv.jobs[k] && lv.type[k] == OL_SYM && lv.job[k][0].l >= OB_SMALL && T == 64;
-        lv.kz[i] = gram ? lo.kz[i] : 1;
-        split |= lv.kz[i] > 1;
-        lv.first.b[i] = blocks;
-        const long units = (long)g[i].count * lv.jobs[k] * og_tiles(g[i], lv.type[k], T) * (pass ? lv.kz[i] > 1 : lv.kz[i]);
+        OrthoGroup &q = lv.gs.g[i];
+        const bool gram = q.jobs && q.type == OL_SYM && lv.job[2 * i].l >= OB_SMALL && T == 64;
+        q.aux = gram ? lo.kz[i] : 1;
+        split_any |= q.aux > 1;
+        q.first = blocks;
+        const long units = (long)q.count * q.jobs * og_tiles(q, q.type, T) * (pass ? q.aux > 1 : q.aux);
         blocks += (int)((units + 7) / 8 * 8);
       }
       if (!blocks) break;
-      const int rc = T == 128 ? ortho_launch<128, 32, 2, 2, 4>(table, n, ws, lv, blocks, st) : ortho_launch<64, 32, 3, 2, 2>(table, n, ws, lv, blocks, st);
+      const int rc = T == 128 ? ortho_launch<128, 32, 2, 2, 4>(ws, lv, blocks, st) : ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st);
       if (rc) return rc;
-      if (!split) break;
+      if (!split_any) break;
     }
   }
   LSPS_CHECK_LAUNCH("newton_schulz");
@@ -863,11 +882,9 @@ int lsps_newton_schulz(const void *g, void *out, int count, int rows, int cols, 
   LSPS_CHECK_ARG(g && out, "newton_schulz: null pointer");
   LSPS_CHECK_ARG(dtype == LSPS_F32 || dtype == LSPS_BF16, "newton_schulz: dtype %d (LSPS_F32 or LSPS_BF16)", dtype);
   OrthoGroup grp = ortho_group(count, rows, cols);
-  grp.base.g = g;
-  grp.base.out = out;
   const OrthoCall call = {steps, a, b, c, eps, dtype == LSPS_F32 ? OM_F32 : OM_BF16, dtype == LSPS_BF16, 1.f, {0.f, 1.f, 0}};
   if (const int rc = ortho_check("newton_schulz", &grp, 1, call, ws, ws_bytes)) return rc;
-  return ortho_run(&grp, 1, nullptr, 0, call, (char *)ws, (hipStream_t)stream);
+  return ortho_run(&grp, 1, OrthoPtr{g, out, nullptr}, nullptr, 0, call, (char *)ws, (hipStream_t)stream);
 }
 
 // The next pass of a Muon step from matrix `at` on: as many as fit ORTHO_GROUPS shapes and ORTHO_MATRICES pointers, sorted into
@@ -941,7 +958,7 @@ int lsps_muon_step(const LspsMuonMatrix *mats, int n, float lr, float momentum, 
   }
   for (int at = 0; at < n; at += p.taken) {
     muon_pass(mats, n, at, lr, rms, &p);
-    if (const int rc = ortho_run(p.g, p.n, p.ptr, p.taken, call, (char *)ws, (hipStream_t)stream)) return rc;
+    if (const int rc = ortho_run(p.g, p.n, OrthoPtr{nullptr, nullptr, nullptr}, p.ptr, p.taken, call, (char *)ws, (hipStream_t)stream)) return rc;
   }
   return 0;
 }
