@@ -262,6 +262,18 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroups gs, char *
 }
 
 // out = k0 (product) + k1 E1 + k2 E2 + diag I on stored (scaled) values: the scales are folded into the factors
+__device__ __forceinline__ void og_result(void *out, long o, float v, int mode, float step, float decay) {
+  if (mode == OM_F32) ((float *)out)[o] = v;
+  else if (mode == OM_BF16) ((__bf16 *)out)[o] = (__bf16)v;               // the one rounding of the result
+  else ((float *)out)[o] = fmaf(-step, v, ((float *)out)[o] * decay);
+}
+
+struct OgTrue {
+  static constexpr bool value = true;
+};
+struct OgFalse {
+  static constexpr bool value = false;
+};
 struct OrthoJob {
   int l, r, e1, e2, out;
   float k0, k1, k2, diag;
@@ -285,10 +297,10 @@ struct OrthoLevel {
 // A product with few tiles and a long reduction is split into kz ranges of it: f32 partial tiles in the workspace, added in a
 // fixed order by a second launch of this kernel.
 template <int T, int KC, int S, int WI, int WJ>
-__global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
+__global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
   constexpr int WAVES = WI * WJ, SUB = KC / 32, STAGE = T * KC * 4, PIECES = T * SUB / 8 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = 144;
   static_assert(S * 2 * STAGE >= WAVES * 32 * TP, "the transpose of the epilogue reuses the stages");
-  static_assert((S - 2) * 2 * PIECES < 64, "the range of s_waitcnt vmcnt");
+  static_assert((S - 1) * 2 * PIECES < 64, "the range of s_waitcnt vmcnt");
   extern __shared__ __align__(1024) char smem[];
   const int lane = threadIdx.x & 63;
   const OrthoJob mine = lv.job[lane < 2 * ORTHO_GROUPS ? lane : 0];
@@ -374,53 +386,82 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(char *__
         c8_dma16_asm(rrs, lds0 + buf * 2 * STAGE + STAGE + (wave + WAVES * p) * 1024, ro[p], c * rstep);
       }
     };
-    const int n = c1 - c0;
-#pragma unroll
-    for (int c = 0; c < S - 1; ++c)
-      if (c < n) stage(c, c0 + c);
-    int at = 0;
-    for (int c = 0; c < n; ++c) {
-      // requests are served in order: those of the S - 2 chunks behind this one may still be on their way
-      if (c + S - 1 <= n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * 2 * PIECES) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();                                        // (__syncthreads may wait for all requests)
-      asm volatile("" ::: "memory");
-      if (c + S - 1 < n) stage(at == 0 ? S - 1 : at - 1, c0 + c + S - 1);  // the stage that was multiplied before this barrier
-      const char *sl = smem + at * 2 * STAGE, *sr = sl + STAGE;
-      at = at + 1 == S ? 0 : at + 1;
-#pragma unroll
-      for (int ks = 0; ks < KC / 16; ++ks) {
-        const int sub = ks >> 1, kg = (ks & 1) * 2 + lh;
-        og_h8 lf[FI][2], rf[FJ][2];
+    // Fragments are read from LDS one half chunk ahead of their MFMAs, across the barrier too: the barrier of chunk c comes when its
+    // last fragments are in registers, so its stage is free for chunk c + S, and chunk c + 1 has landed
+    static_assert(KC == 32, "two halves per chunk");
+    og_h8 lf[2][FI][2], rf[2][FJ][2];
+    auto product = [&](auto turn) {
+      auto load = [&](int h, const char *sl) {
+        const char *sr = sl + STAGE;
+        const int kg = h * 2 + lh;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
           for (int f = 0; f < FJ; ++f)
-            if (!turned) {
+            if constexpr (!turn.value) {
               const int rj = (wj * FJ + f) * 32 + l31;
-              rf[f][q] = *reinterpret_cast<const og_h8 *>(sr + (sub * T + rj) * 128 + (((kg * 2 + q) ^ ((rj >> 1) & 7)) * 16));
+              rf[h][f][q] = *reinterpret_cast<const og_h8 *>(sr + rj * 128 + (((kg * 2 + q) ^ ((rj >> 1) & 7)) * 16));
             } else {
               // lane i of 16 points at 4 columns of row i / 4 and receives 4 rows of column i
-              const int r = ks * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2 + q;
-              const char *base = sr + ((wj * FJ + f) * KC + r) * 128 + (lane & 1) * 8;
-              rf[f][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)base + ((u ^ ((r >> 1) & 7)) * 16),
-                                                              (const unsigned char *)base + 512 + ((u ^ (((r + 4) >> 1) & 7)) * 16)));
+              const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2 + q;
+              const char *at = sr + ((wj * FJ + f) * KC + r) * 128 + (lane & 1) * 8;
+              rf[h][f][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)at + ((u ^ ((r >> 1) & 7)) * 16),
+                                                                 (const unsigned char *)at + 512 + ((u ^ (((r + 4) >> 1) & 7)) * 16)));
             }
 #pragma unroll
           for (int f = 0; f < FI; ++f) {
             const int li = (wi * FI + f) * 32 + l31;
-            lf[f][q] = *reinterpret_cast<const og_h8 *>(sl + (sub * T + li) * 128 + (((kg * 2 + q) ^ ((li >> 1) & 7)) * 16));
+            lf[h][f][q] = *reinterpret_cast<const og_h8 *>(sl + li * 128 + (((kg * 2 + q) ^ ((li >> 1) & 7)) * 16));
           }
         }
+      };
+      auto multiply = [&](int h) {
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
-          for (int j = 0; j < FJ; ++j) {
-            acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][0], lf[i][1], acx[i][j], 0, 0, 0);
-            acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][1], lf[i][0], acx[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[j][0], lf[i][0], acc[i][j], 0, 0, 0);
-          }
+          for (int j = 0; j < FJ; ++j) acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[h][j][0], lf[h][i][1], acx[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int j = 0; j < FJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[h][j][0], lf[h][i][0], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int j = 0; j < FJ; ++j) acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[h][j][1], lf[h][i][0], acx[i][j], 0, 0, 0);
+      };
+      const int n = c1 - c0;
+#pragma unroll
+      for (int c = 0; c < S; ++c)
+        if (c < n) stage(c, c0 + c);
+      // requests are served in order: those of the S - 1 chunks behind the first may still be on their way
+      if (n >= S) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * 2 * PIECES) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      load(0, smem);
+      int at = 0;
+      for (int c = 0; c < n; ++c) {
+        load(1, smem + at * 2 * STAGE);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + 1 < n) {
+          // chunks c + 1 ... c + S - 1 are requested
+          if (n - 2 - c >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * 2 * PIECES) : "memory");
+          else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          if (c + S < n) stage(at, c0 + c + S);
+          at = at + 1 == S ? 0 : at + 1;
+          load(0, smem + at * 2 * STAGE);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        multiply(1);
       }
+    };
+    if (c0 < c1) {
+      if (turned) product(OgTrue());
+      else product(OgFalse());
     }
     if (kz > 1) {
       og_f4 *dst = reinterpret_cast<og_f4 *>(part) + ((long)(mat * (per / kz) + tile) * kz + z) * (T * T / 4) + threadIdx.x;
@@ -531,12 +572,7 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(char *__
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (j + k < nn) {
-                const long o = tall ? (long)(j + k) * m + i : (long)i * nn + j + k;
-                if (lv.mode == OM_F32) ((float *)ptr.out)[o] = v[k];
-                else if (lv.mode == OM_BF16) ((__bf16 *)ptr.out)[o] = (__bf16)v[k];       // the one rounding of the result
-                else ((float *)ptr.out)[o] = fmaf(-g.step, v[k], ((float *)ptr.out)[o] * lv.decay);
-              }
+              if (j + k < nn) og_result(ptr.out, tall ? (long)(j + k) * m + i : (long)i * nn + j + k, v[k], lv.mode, g.step, lv.decay);
           }
         }
       }
@@ -551,6 +587,183 @@ __global__ __launch_bounds__(WI * WJ * 64, 2) void ortho_product_kernel(char *__
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
     }
+}
+
+// ---- small matrices: the whole iteration in one workgroup ----------------------------------------------------------------
+#define ORTHO_SMALL_M 64
+#define ORTHO_SMALL_N 448      // 14 chunks of 8 KB next to A and Q, 16 KB each
+struct OrthoSmallStep {
+  float gram, s0, s1, diag, x;      // factors of A; of A A, A and I in Q = a I + b A + c A A; of Q X
+};
+struct OrthoSmall {
+  OrthoGroups gs;
+  OrthoSmallStep step[ORTHO_STEPS];
+  OrthoMomentum mo;
+  int steps, mode;
+  float decay, eps, x0;
+};
+
+// byte of 16-byte unit u of row r of a chunk of 64 rows x 32 columns in LDS
+__device__ __forceinline__ int og_unit(int r, int u) { return r * 128 + ((u ^ ((r >> 1) & 7)) << 4); }
+
+// One matrix per workgroup, M <= 64 <= and N <= 448 after padding: X, A and Q stay in LDS as limbs, the three products of a step
+// follow each other with a barrier between them (through launches they take ~5 us each at these sizes).  4 waves; A and Q: one
+// 32 x 32 tile each; X <- Q X: a wave owns whole chunks of 32 columns, so it can write where it has read.
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256) void ortho_small_kernel(OrthoSmall c) {
+  extern __shared__ __align__(1024) char smem[];
+  __shared__ double red[4];
+  int grp;
+  const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
+  const int mat = blockIdx.x - g.first;
+  const OrthoPtr ptr = ortho_ptr(c.gs, g, mat, sizeof(T));
+  const int m = og_short(g), n = og_long(g), chunks = (n + 31) / 32;
+  const bool tall = g.rows > g.cols;
+  char *A = smem, *Q = smem + 16384, *X = smem + 32768;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, lh = lane >> 5;
+  // G as f32, 8 columns in the place of their two units; lanes run along the rows of G
+  const T *src = (const T *)ptr.g;
+  const int groups = chunks * 4;                                 // of 8 columns
+  double sum = 0.;
+  for (int t = threadIdx.x; t < 64 * groups; t += 256) {
+    const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = q * 8 + e;
+      const bool in = i < m && j < n;
+      const long o = tall ? (long)j * m + i : (long)i * n + j;
+      v[e] = in ? (float)src[o] : 0.f;
+      if constexpr (MUON) {
+        if (in) {
+          v[e] *= c.mo.gscale;
+          const float mm = fmaf(c.mo.mu, ptr.m[o], v[e]);
+          ptr.m[o] = mm;
+          v[e] = c.mo.nesterov ? fmaf(c.mo.mu, mm, v[e]) : mm;
+        }
+      }
+      sum += (double)v[e] * (double)v[e];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const og_f4 f = {v[h * 4], v[h * 4 + 1], v[h * 4 + 2], v[h * 4 + 3]};
+      *reinterpret_cast<og_f4 *>(X + (q >> 2) * 8192 + og_unit(i, (q & 3) * 2 + h)) = f;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) red[wave] = sum;
+  __syncthreads();
+  const float norm = (float)(sqrt(red[0] + red[1] + red[2] + red[3]) + (double)c.eps);
+  for (int t = threadIdx.x; t < 64 * groups; t += 256) {         // every thread turns what it stored into limbs
+    const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
+    char *p0 = X + (q >> 2) * 8192 + og_unit(i, (q & 3) * 2), *p1 = X + (q >> 2) * 8192 + og_unit(i, (q & 3) * 2 + 1);
+    const og_f4 f0 = *reinterpret_cast<og_f4 *>(p0), f1 = *reinterpret_cast<og_f4 *>(p1);
+    og_h8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      _Float16 a, b;
+      og_split((e < 4 ? f0[e] : f1[e - 4]) / norm * c.x0, a, b);
+      h[e] = a;
+      l[e] = b;
+    }
+    *reinterpret_cast<og_h8 *>(p0) = h;
+    *reinterpret_cast<og_h8 *>(p1) = l;
+  }
+  const int ti = (wave >> 1) * 32, tj = (wave & 1) * 32;         // this wave's tile of A and Q
+  for (int k = 0; k < c.steps; ++k) {
+    const OrthoSmallStep st = c.step[k];
+    auto frag = [&](const char *chunk, int row, int half, int limb) {      // 8 columns of a row: half-chunk `half`
+      return *reinterpret_cast<const og_h8 *>(chunk + og_unit(row, (half * 2 + lh) * 2 + limb));
+    };
+    auto put = [&](char *chunk, int row, int q, const float (&v)[4]) {     // 4 values of a row from column 8 q + 4 lh on
+      og_h4 h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        _Float16 a, b;
+        og_split(v[e], a, b);
+        h[e] = a;
+        l[e] = b;
+      }
+      *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2) + lh * 8) = h;
+      *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2 + 1) + lh * 8) = l;
+    };
+    // A = X X^T, then Q = a I + b A + c A A; small cross products apart from hi hi, as in ortho_product_kernel
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const char *in = which ? A : X;
+      og_f16v acc, acx;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] = acx[e] = 0.f;
+      __syncthreads();
+#pragma unroll 4
+      for (int h = 0; h < (which ? 4 : chunks * 2); ++h) {
+        const char *chunk = in + (h >> 1) * 8192;
+        const og_h8 ih = frag(chunk, ti + l31, h & 1, 0), il = frag(chunk, ti + l31, h & 1, 1);
+        const og_h8 jh = frag(chunk, tj + l31, h & 1, 0), jl = frag(chunk, tj + l31, h & 1, 1);
+        acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, il, acx, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, ih, acc, 0, 0, 0);
+        acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jl, ih, acx, 0, 0, 0);
+      }
+      char *chunk = (which ? Q : A) + (tj >> 5) * 8192;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+        const char *e1 = A + (tj >> 5) * 8192;
+        const og_h4 eh = *reinterpret_cast<const og_h4 *>(e1 + og_unit(ti + l31, q * 2) + lh * 8);
+        const og_h4 el = *reinterpret_cast<const og_h4 *>(e1 + og_unit(ti + l31, q * 2 + 1) + lh * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = acc[q * 4 + e] + acx[q * 4 + e];
+          if (which) v[e] = st.s0 * p + st.s1 * ((float)eh[e] + (float)el[e]) + (ti + l31 == tj + q * 8 + lh * 4 + e ? st.diag : 0.f);
+          else v[e] = st.gram * p;
+        }
+        put(chunk, ti + l31, q, v);
+      }
+    }
+    __syncthreads();
+    // X = Q X: the reduction runs down the rows of X (transposing reads)
+    for (int ch = wave; ch < chunks; ch += 4) {
+      char *chunk = X + ch * 8192;
+      og_f16v acc[2], acx[2];
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[f][e] = acx[f][e] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2;
+        og_h8 x[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          x[q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)chunk + og_unit(r, u + q) + (lane & 1) * 8,
+                                                      (const unsigned char *)chunk + og_unit(r + 4, u + q) + (lane & 1) * 8));
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const og_h8 ih = frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 0), il = frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 1);
+          acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], il, acx[f], 0, 0, 0);
+          acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], ih, acc[f], 0, 0, 0);
+          acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[1], ih, acx[f], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = f * 32 + l31, j = ch * 32 + q * 8 + lh * 4;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = st.x * (acc[f][q * 4 + e] + acx[f][q * 4 + e]);
+          if (k + 1 < c.steps) {
+            put(chunk, i, q, v);
+          } else if (i < m) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (j + e < n) og_result(ptr.out, tall ? (long)(j + e) * m + i : (long)i * n + j + e, v[e], c.mode, g.step, c.decay);
+          }
+        }
+    }
+  }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -631,17 +844,17 @@ struct OrthoPlan {
     OrthoJob job[2];
     int jobs, type;
   } level[3 * ORTHO_STEPS + ORTHO_STEPS];
-  int levels;
+  int levels;                       // 0: not asked for yet
   float x0;                         // scale of X0
 };
 
 static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
+  p->levels = 0;
   double sv[ORTHO_SAMPLES];
   for (int i = 0; i < ORTHO_SAMPLES; ++i) {                              // denser towards 0
     const double u = (double)i / (ORTHO_SAMPLES - 1);
     sv[i] = 1.00001 * u * u * u;
   }
-  p->levels = 0;
   auto add = [p](int type, const OrthoJob &job) {
     p->level[p->levels].type = type;
     p->level[p->levels].jobs = 1;
@@ -702,6 +915,7 @@ static int ortho_kz(int K, long own, long tiles) {
 
 struct OrthoLayout {
   size_t sums, bytes;
+  bool small;                       // every matrix fits ortho_small_kernel
   int chain[ORTHO_GROUPS];
   int kz[ORTHO_GROUPS];             // of the Gram matrices
   int norm_first[ORTHO_GROUPS], split_first[ORTHO_GROUPS];
@@ -714,6 +928,13 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
   OrthoLayout lo;
   memset(&lo, 0, sizeof lo);
   lo.sums = align_up(sizeof(OrthoPtr) * ORTHO_MATRICES, 256);
+  lo.small = true;
+  for (int i = 0; i < n; ++i) lo.small = lo.small && og_short(g[i]) <= ORTHO_SMALL_M && og_long(g[i]) <= ORTHO_SMALL_N;
+  if (lo.small) {
+    for (int i = 0; i < n; ++i) lo.chain[i] = 1;
+    lo.bytes = lo.sums;
+    return lo;
+  }
   long tiles = 0;
   for (int i = 0; i < n; ++i) {
     lo.chain[i] = ortho_chain(g[i]);
@@ -747,20 +968,14 @@ static int ortho_launch(char *ws, const OrthoLevel &lv, int blocks, hipStream_t 
 }
 
 // one pass over at most ORTHO_GROUPS groups and ORTHO_MATRICES pointers
-static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr *ptrs, int nptr, const OrthoCall &c, char *ws, hipStream_t st) {
+static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr *ptrs, int nptr, const OrthoCall &c, const OrthoPlan *plan,
+                     char *ws, hipStream_t st) {
   const OrthoLayout lo = ortho_layout(g, n, c.steps);
   double *sums = (double *)(ws + lo.sums);
-  static thread_local OrthoPlan plan[ORTHO_CHAINS];
-  bool used[ORTHO_CHAINS] = {false};
   int levels = 0;
-  float x0 = 1.f;
-  for (int i = 0; i < n; ++i) used[lo.chain[i] - 1] = true;
-  for (int k = 0; k < ORTHO_CHAINS; ++k)
-    if (used[k]) {
-      LSPS_CHECK_ARG(ortho_plan(&plan[k], k + 1, c), "newton_schulz: coefficients");
-      if (plan[k].levels > levels) levels = plan[k].levels;
-      x0 = plan[k].x0;                                                   // (the same for every chain length)
-    }
+  const float x0 = plan[lo.chain[0] - 1].x0;                             // (the same for every chain length)
+  for (int i = 0; i < n; ++i)
+    if (plan[lo.chain[i] - 1].levels > levels) levels = plan[lo.chain[i] - 1].levels;
   for (int i = 0; i < nptr; i += ORTHO_PTR_PART) {
     OrthoPtrPart part;
     const int k = nptr - i < ORTHO_PTR_PART ? nptr - i : ORTHO_PTR_PART;
@@ -778,6 +993,33 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     lv.gs.g[i].first = i < n ? lo.norm_first[i] : INT_MAX;
     lv.gs.g[i].aux = lo.norm_first[i];
   }
+  if (lo.small) {
+    OrthoSmall sm;
+    memset(&sm, 0, sizeof sm);
+    sm.gs = lv.gs;
+    sm.mo = c.mo;
+    sm.steps = c.steps;
+    sm.mode = c.mode;
+    sm.decay = c.decay;
+    sm.eps = c.eps;
+    sm.x0 = x0;
+    int blocks = 0, most = 0;
+    for (int i = 0; i < n; ++i) {
+      sm.gs.g[i].first = blocks;
+      blocks += g[i].count;
+      if (og_long(g[i]) > most) most = og_long(g[i]);
+    }
+    for (int k = 0; k < c.steps; ++k) {
+      const OrthoJob *a = plan[0].level[3 * k].job, *q = plan[0].level[3 * k + 1].job, *x = plan[0].level[3 * k + 2].job;
+      sm.step[k] = OrthoSmallStep{a->k0, q->k0, q->k1, q->diag, x->k0};
+    }
+    const int lds = 32768 + (most + 31) / 32 * 8192;
+    auto kernel = c.mode == OM_MUON ? ortho_small_kernel<float, true> : c.bf16 ? ortho_small_kernel<__bf16, false> : ortho_small_kernel<float, false>;
+    if (const int rc = lds_optin(reinterpret_cast<const void *>(kernel), 32768 + ORTHO_SMALL_N / 32 * 8192, "ortho_small_kernel")) return rc;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), lds, st, sm);
+    LSPS_CHECK_LAUNCH("newton_schulz");
+    return 0;
+  }
   OrthoGroups split = lv.gs;
   for (int i = 0; i < n; ++i) split.g[i].first = lo.split_first[i];
 #define ORTHO_PRE(T, MUON)                                                                                                            \
@@ -791,15 +1033,19 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
 #undef ORTHO_PRE
   for (int l = 0; l < levels; ++l) {
     long b128 = 0;
+    bool square = true;
     for (int i = 0; i < n; ++i) {
       const OrthoPlan &p = plan[lo.chain[i] - 1];
       lv.gs.g[i].type = l < p.levels ? p.level[l].type : OL_SYM;
       lv.gs.g[i].jobs = l < p.levels ? p.level[l].jobs : 0;
       if (l < p.levels) memcpy(lv.job + 2 * i, p.level[l].job, sizeof p.level[l].job);
+      square = square && lv.gs.g[i].type == OL_SYM;
       b128 += (long)g[i].count * lv.gs.g[i].jobs * og_tiles(g[i], lv.gs.g[i].type, 128);
     }
-    // 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs
-    const int T = b128 >= 256 ? 128 : 64;
+    // 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs, the symmetric products (whose
+    // tiles on the diagonal do both halves' work) two per CU.  2048 x 9216: 1586 us with 256 for all, 1574 so; 64 x 256 x 2304:
+    // 710 / 680; 2048 x 2048, 256 tiles of Q X: 788, 845 with 500 for all
+    const int T = b128 >= (square ? 500 : 256) ? 128 : 64;
     bool split_any = false;
     for (int pass = 0; pass < 2; ++pass) {
       int blocks = 0;
@@ -814,7 +1060,11 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
         blocks += (int)((units + 7) / 8 * 8);
       }
       if (!blocks) break;
-      const int rc = T == 128 ? ortho_launch<128, 32, 2, 2, 4>(ws, lv, blocks, st) : ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st);
+      // 64 x 64 tiles: up to two blocks per CU a third stage hides more latency than more resident blocks would (1024 x 4608: 415 us,
+      // 492 with two stages), from then on they do (2048 x 9216: 1574, 1475 with two)
+      const int rc = T == 128       ? ortho_launch<128, 32, 2, 2, 4>(ws, lv, blocks, st)
+                     : blocks > 512 ? ortho_launch<64, 32, 2, 2, 2>(ws, lv, blocks, st)
+                                    : ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st);
       if (rc) return rc;
       if (!split_any) break;
     }
@@ -835,15 +1085,17 @@ static bool ortho_sane(const OrthoGroup &g) {
          (double)og_pad(g.rows) * og_pad(g.cols) * g.count <= (double)(1L << 36);
 }
 
-static int ortho_check(const char *what, OrthoGroup *g, int n, const OrthoCall &c, const void *ws, size_t ws_bytes) {
+// this thread's plans, none made yet
+static OrthoPlan *ortho_plans() {
+  static thread_local OrthoPlan plan[ORTHO_CHAINS];
+  for (int k = 0; k < ORTHO_CHAINS; ++k) plan[k].levels = 0;
+  return plan;
+}
+
+// checks one pass; plan[k]: made for the chain lengths that it needs, kept for the call's other passes
+static int ortho_check(const char *what, OrthoGroup *g, int n, const OrthoCall &c, OrthoPlan *plan, const void *ws, size_t ws_bytes) {
   LSPS_CHECK_ARG(c.steps >= 1 && c.steps <= ORTHO_STEPS, "%s: %d steps (1 to %d)", what, c.steps, ORTHO_STEPS);
   LSPS_CHECK_ARG(c.eps >= 0.f, "%s: eps %g", what, (double)c.eps);
-  static thread_local OrthoPlan plan;
-  bool used[ORTHO_CHAINS] = {false};
-  for (int i = 0; i < n; ++i) used[ortho_chain(g[i]) - 1] = true;
-  for (int k = 1; k <= ORTHO_CHAINS; ++k)
-    LSPS_CHECK_ARG(!used[k - 1] || ortho_plan(&plan, k, c), "%s: the iteration with (%g, %g, %g) leaves the range of its 16-bit limbs on [0, 1]", what,
-                   (double)c.a, (double)c.b, (double)c.c);
   double blocks = 0;
   for (int i = 0; i < n; ++i) {
     LSPS_CHECK_ARG(ortho_sane(g[i]), "%s: %d matrices of %d x %d", what, g[i].count, g[i].rows, g[i].cols);
@@ -851,10 +1103,15 @@ static int ortho_check(const char *what, OrthoGroup *g, int n, const OrthoCall &
     blocks += (double)g[i].count * ((double)og_pad(g[i].rows) / 64 * og_pad(g[i].cols) / 64 + 8) * 2;
   }
   LSPS_CHECK_ARG(blocks < (double)(1L << 23), "%s: too many matrices for one call", what);
-  const size_t need = ortho_layout(g, n, c.steps).bytes;
+  const OrthoLayout lo = ortho_layout(g, n, c.steps);
+  for (int i = 0; i < n; ++i) {
+    OrthoPlan *p = plan + lo.chain[i] - 1;
+    LSPS_CHECK_ARG(p->levels || ortho_plan(p, lo.chain[i], c), "%s: the iteration with (%g, %g, %g) leaves the range of its 16-bit limbs on [0, 1]",
+                   what, (double)c.a, (double)c.b, (double)c.c);
+  }
   LSPS_CHECK_ARG(!((uintptr_t)ws & 15), "%s: the workspace is not 16-byte aligned", what);
-  if (!ws || ws_bytes < need) {
-    set_error("%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
+  if (!ws || ws_bytes < lo.bytes) {
+    set_error("%s: workspace of %zu bytes, %zu needed", what, ws_bytes, lo.bytes);
     return LSPS_E_WS;
   }
   return 0;
@@ -883,8 +1140,9 @@ int lsps_newton_schulz(const void *g, void *out, int count, int rows, int cols, 
   LSPS_CHECK_ARG(dtype == LSPS_F32 || dtype == LSPS_BF16, "newton_schulz: dtype %d (LSPS_F32 or LSPS_BF16)", dtype);
   OrthoGroup grp = ortho_group(count, rows, cols);
   const OrthoCall call = {steps, a, b, c, eps, dtype == LSPS_F32 ? OM_F32 : OM_BF16, dtype == LSPS_BF16, 1.f, {0.f, 1.f, 0}};
-  if (const int rc = ortho_check("newton_schulz", &grp, 1, call, ws, ws_bytes)) return rc;
-  return ortho_run(&grp, 1, OrthoPtr{g, out, nullptr}, nullptr, 0, call, (char *)ws, (hipStream_t)stream);
+  OrthoPlan *plan = ortho_plans();
+  if (const int rc = ortho_check("newton_schulz", &grp, 1, call, plan, ws, ws_bytes)) return rc;
+  return ortho_run(&grp, 1, OrthoPtr{g, out, nullptr}, nullptr, 0, call, plan, (char *)ws, (hipStream_t)stream);
 }
 
 // The next pass of a Muon step from matrix `at` on: as many as fit ORTHO_GROUPS shapes and ORTHO_MATRICES pointers, sorted into
@@ -952,13 +1210,14 @@ int lsps_muon_step(const LspsMuonMatrix *mats, int n, float lr, float momentum, 
     LSPS_CHECK_ARG(ortho_sane(ortho_group(1, mats[i].rows, mats[i].cols)), "muon_step: matrix %d of %d x %d", i, mats[i].rows, mats[i].cols);
   }
   const OrthoCall call = {steps, a, b, c, eps, OM_MUON, false, 1.f - lr * weight_decay, {momentum, grad_scale, nesterov != 0}};
+  OrthoPlan *plan = ortho_plans();
   for (int at = 0; at < n; at += p.taken) {
     muon_pass(mats, n, at, lr, rms, &p);
-    if (const int rc = ortho_check("muon_step", p.g, p.n, call, ws, ws_bytes)) return rc;
+    if (const int rc = ortho_check("muon_step", p.g, p.n, call, plan, ws, ws_bytes)) return rc;
   }
   for (int at = 0; at < n; at += p.taken) {
     muon_pass(mats, n, at, lr, rms, &p);
-    if (const int rc = ortho_run(p.g, p.n, OrthoPtr{nullptr, nullptr, nullptr}, p.ptr, p.taken, call, (char *)ws, (hipStream_t)stream)) return rc;
+    if (const int rc = ortho_run(p.g, p.n, OrthoPtr{nullptr, nullptr, nullptr}, p.ptr, p.taken, call, plan, (char *)ws, (hipStream_t)stream)) return rc;
   }
   return 0;
 }

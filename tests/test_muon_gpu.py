@@ -46,7 +46,7 @@ def grads(count, rows, cols, seed=0, size=1e-3):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 9), (2, 9, 1), (1, 2, 3), (3, 20, 50), (1, 50, 108), (2, 64, 64), (2, 64, 49), (1, 65, 63), (1, 128, 129),
-          (2, 130, 65), (5, 100, 333), (1, 333, 1021), (2, 256, 256), (1, 257, 700), (1, 20, 8192), (3, 8192, 20), (70, 33, 40), (1, 512, 513),
+          (2, 130, 65), (5, 100, 333), (1, 333, 1021), (2, 256, 256), (1, 257, 700), (1, 20, 8192), (3, 8192, 20), (70, 33, 40), (1, 512, 513), (3, 64, 448), (2, 449, 64), (2, 448, 30), (300, 5, 31),
           (40, 192, 200), (1, 1024, 1100), (20, 448, 1000)]
 
 

@@ -90,7 +90,7 @@ def test_workspace_sizes_grow_with_the_call():
     assert ns(28, 256, 2304, 5) >= 28 * 4 * 2 * 256 * 2304                 # two limbs, two generations of X
     assert ns(1, 2304, 256, 5) == ns(1, 256, 2304, 5)                      # tall = wide
     assert ns(1, 256, 2304, 1) < ns(1, 256, 2304, 5) and ns(2, 100, 90, 5) > ns(1, 100, 90, 5)
-    mats = (_lib.LspsMuonMatrix * 1500)(*[_lib.LspsMuonMatrix(0, 0, 0, 64, 64)] * 1500)
+    mats = (_lib.LspsMuonMatrix * 1500)(*[_lib.LspsMuonMatrix(0, 0, 0, 70, 80)] * 1500)
     one, many = h.lsps_muon_workspace_bytes(mats, 1024, 5), h.lsps_muon_workspace_bytes(mats, 1500, 5)
     assert h.lsps_muon_workspace_bytes(mats, 1, 5) < one == many            # passes share it
 
