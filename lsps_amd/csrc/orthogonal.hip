@@ -299,7 +299,7 @@ struct OrthoLevel {
 template <int T, int KC, int S, int WI, int WJ>
 __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
   constexpr int WAVES = WI * WJ, SUB = KC / 32, STAGE = T * KC * 4, PIECES = T * SUB / 8 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = 144;
-  static_assert(S * 2 * STAGE >= WAVES * 32 * TP, "the transpose of the epilogue reuses the stages");
+  static_assert(S * 2 * STAGE >= WAVES * 32 * TP, "the exchange buffers of the epilogue lie in the stages");
   static_assert((S - 1) * 2 * PIECES < 64, "the range of s_waitcnt vmcnt");
   extern __shared__ __align__(1024) char smem[];
   const int lane = threadIdx.x & 63;
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
   const int m = og_short(g), nn = og_long(g);
   const bool tall = g.rows > g.cols;
   char *out = last ? nullptr : ortho_buffer(ws, g, job.out, mat);
-  if (mirrored) __syncthreads();                                         // the stages become the waves' transpose buffers
+  if (!last) __syncthreads();                                            // the stages become the waves' exchange buffers
   char *tp = smem + wave * 32 * TP;
 #pragma unroll
   for (int fi = 0; fi < FI; ++fi)
@@ -519,6 +519,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
     for (int fj = 0; fj < FJ; ++fj) {
       const int i0 = bi * T + (wi * FI + fi) * 32, j0 = bj * T + (wj * FJ + fj) * 32, i = i0 + l31;
       if (i0 >= M || j0 >= cols) continue;                               // (T = 128 on an odd number of 64-row halves)
+      og_h4 hq[4], lq[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int j = j0 + q * 8 + lh * 4;
@@ -545,17 +546,10 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
             h[k] = a;
             l[k] = b;
           }
-          og_h4 *p = reinterpret_cast<og_h4 *>(out + og_at(M, i, j));
-          p[0] = h;
-          p[2] = l;
-          if (mirrored) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              char *d = tp + (q * 8 + lh * 4 + k) * TP + l31 * 2;
-              *reinterpret_cast<_Float16 *>(d) = h[k];
-              *reinterpret_cast<_Float16 *>(d + 64) = l[k];
-            }
-          }
+          *reinterpret_cast<og_h4 *>(tp + l31 * TP + q * 32 + lh * 8) = h;
+          *reinterpret_cast<og_h4 *>(tp + l31 * TP + q * 32 + 16 + lh * 8) = l;
+          hq[q] = h;
+          lq[q] = l;
         } else if (i < m) {
           if (!tall && j + 4 <= nn && lv.mode != OM_BF16) {
             og_f4u *o = reinterpret_cast<og_f4u *>((float *)ptr.out + (long)i * nn + j);
@@ -576,15 +570,34 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
           }
         }
       }
-      if (mirrored) {
+      if (!last) {
+        // 32 rows x 128 bytes of the result lie one behind the other: 16 bytes per lane, four full stores
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        char *o = out + og_at(M, i0, j0);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const int u = lane + s * 64, jr = u >> 3, ig = (u & 7) >> 1, limb = u & 1;
-          const og_h8 x = *reinterpret_cast<const og_h8 *>(tp + jr * TP + limb * 64 + ig * 16);
-          *reinterpret_cast<og_h8 *>(out + og_at(M, j0 + jr, i0 + ig * 8) + limb * 16) = x;
+          const int u = lane + s * 64;
+          *reinterpret_cast<og_h8 *>(o + u * 16) = *reinterpret_cast<const og_h8 *>(tp + (u >> 3) * TP + (u & 7) * 16);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (mirrored) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              char *d = tp + (q * 8 + lh * 4 + k) * TP + (l31 >> 3) * 32 + (l31 & 7) * 2;
+              *reinterpret_cast<_Float16 *>(d) = hq[q][k];
+              *reinterpret_cast<_Float16 *>(d + 16) = lq[q][k];
+            }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          char *m = out + og_at(M, j0, i0);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const int u = lane + s * 64;
+            *reinterpret_cast<og_h8 *>(m + u * 16) = *reinterpret_cast<const og_h8 *>(tp + (u >> 3) * TP + (u & 7) * 16);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
       }
     }
 }
