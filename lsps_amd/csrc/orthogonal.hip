@@ -39,7 +39,7 @@ typedef unsigned short og_u4u __attribute__((ext_vector_type(4), aligned(2)));
 #define ORTHO_GROUPS 16        // shapes per pass (they travel in the kernels' arguments)
 #define ORTHO_MATRICES 1024    // matrices with pointers of their own per pass
 #define ORTHO_CHAINS 3         // longest chain: steps between two Gram matrices of the long side
-#define ORTHO_NORM_BLOCK 16384 // elements per block of the norm pass
+#define ORTHO_NORM_BLOCK 8192 // elements per block of the norm pass
 #define ORTHO_PTR_PART 96      // matrices per table launch (passed by value: nothing on the host has to outlive the call)
 #define ORTHO_STEPS 64
 enum { OB_A, OB_S, OB_T, OB_R0, OB_R1, OB_SMALL, OB_X0 = OB_SMALL, OB_X1, OB_NONE };
@@ -268,6 +268,14 @@ __device__ __forceinline__ void og_result(void *out, long o, float v, int mode, 
   else ((float *)out)[o] = fmaf(-step, v, ((float *)out)[o] * decay);
 }
 
+// a / b for 0 <= a < 2^23, b > 0: a tenth of the instructions of an integer division, all of them in a block's first microsecond
+__device__ __forceinline__ int og_div(int a, int b) {
+  int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+  q -= q * b > a;
+  q += (q + 1) * b <= a;
+  return __builtin_amdgcn_readfirstlane(q);
+}
+
 struct OgTrue {
   static constexpr bool value = true;
 };
@@ -314,7 +322,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
   if ((rel >> 3) >= q8 || unit0 >= total) return;
   const int second = unit0 >= per * g.count;
   const OrthoJob job = og_readlane(mine, __builtin_amdgcn_readfirstlane(grp * 2 + second));
-  const int u1 = unit0 - second * per * g.count, mat = u1 / per, u2 = u1 - mat * per, z = u2 % kz, tile = u2 / kz;
+  const int u1 = unit0 - second * per * g.count, mat = og_div(u1, per), u2 = u1 - mat * per, tile = og_div(u2, kz), z = u2 - tile * kz;
   int bi, bj;
   if (type == OL_SYM) {
     bj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
@@ -323,12 +331,12 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
     bi = tile - bj * (bj + 1) / 2;
   } else {
     const int tm = (M + T - 1) / T;                              // the row tiles of one column panel one after the other
-    bj = tile / tm;
+    bj = og_div(tile, tm);
     bi = tile - bj * tm;
   }
   const int cols = type == OL_SYM ? M : N;                       // of the result; rows: M
   const int K = job.l >= OB_SMALL ? N : M;
-  const int chunks = K / KC, c0 = (int)((long)chunks * z / kz), c1 = (int)((long)chunks * (z + 1) / kz);
+  const int chunks = K / KC, c0 = og_div(chunks * z, kz), c1 = og_div(chunks * (z + 1), kz);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ, l31 = lane & 31, lh = lane >> 5;
   og_f16v acc[FI][FJ], acx[FI][FJ];
@@ -341,21 +349,23 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
   float *part = reinterpret_cast<float *>(ws + (size_t)g.p_off * 256);   // [mat][tile][z][fi][fj][q][thread][4]
   const char *e1 = job.e1 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e1, mat);
   const char *e2 = job.e2 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e2, mat);
-  // one fragment per wave: E1 and E2 are fetched in front of the product, whose first requests they precede
+  // one fragment per wave: E1 and E2 are fetched behind the product's first requests
   constexpr bool EARLY = FI * FJ == 1;
   og_h4 eh[EARLY ? 8 : 1], el[EARLY ? 8 : 1];
-  if constexpr (EARLY) {
+  auto early = [&]() {
+    if constexpr (EARLY) {
+      const long at = og_at(M, (bi * WI + wi) * 32 + l31, (bj * WJ + wj) * 32 + lh * 4);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const char *e = q < 4 ? e1 : e2;
-      const int i = (bi * WI + wi) * 32 + l31, j = (bj * WJ + wj) * 32 + (q & 3) * 8 + lh * 4;
-      if (e) {
-        const og_h4 *p = reinterpret_cast<const og_h4 *>(e + og_at(M, i, j));
-        eh[q] = p[0];
-        el[q] = p[2];
+      for (int q = 0; q < 8; ++q) {
+        const char *e = q < 4 ? e1 : e2;
+        if (e) {
+          const og_h4 *p = reinterpret_cast<const og_h4 *>(e + at + (q & 3) * 32);
+          eh[q] = p[0];
+          el[q] = p[2];
+        }
       }
     }
-  }
+  };
   if (!lv.joining) {
     // a piece = 8 lines of 128 bytes = one DMA request of a wave: [sub-chunk of 32][line], line = row of the tile; for X in
     // OL_RECT / OL_LAST: [32 columns][row of the chunk].  Unit u of line r lies at u ^ (r / 2): 16 lanes reading 16 consecutive
@@ -433,6 +443,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
 #pragma unroll
       for (int c = 0; c < S; ++c)
         if (c < n) stage(c, c0 + c);
+      if (kz == 1) early();
       // requests are served in order: those of the S - 1 chunks behind the first may still be on their way
       if (n >= S) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * 2 * PIECES) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -479,6 +490,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
       return;
     }
   } else {
+    early();
     const int nz = g.aux;
     const og_f4 *src = reinterpret_cast<const og_f4 *>(part) + (long)(mat * per + tile) * nz * (T * T / 4) + threadIdx.x;
     for (int k = 0; k < nz; ++k, src += T * T / 4)
