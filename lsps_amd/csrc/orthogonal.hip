@@ -7,9 +7,9 @@
 // Gram matrix and, from step to step, R <- a R + a^n S + R S and A <- A P^2 with P = a I + S: products of M x M matrices only,
 // every one of them symmetric (they are polynomials of one symmetric matrix), so only the tiles on and above the diagonal are
 // computed.  Two products with the long side (A, and the last one) per restart instead of two per step: 3 M^2 N + O(M^3)
-// operations instead of 15 M^2 N for five steps.  A is formed anew from X after at most ORTHO_CHAIN steps: an error d of A is
-// one of |b| / a (a^2)^k d, relatively, in the directions of small singular values after k more steps, so three steps cost
-// what the plain iteration in f32 costs (measured: no larger error than it) and five do not.
+// operations instead of 15 M^2 N for five steps.  A is formed anew from X after at most ORTHO_CHAINS steps: an error d of A is
+// one of |b| / a (a^2)^k d, relatively, in the directions of small singular values after k more steps, so that chains of three
+// cost about what the plain iteration in f32 costs and longer ones more (ortho_chain has the measurements).
 //
 // Operands.  Every matrix lives in the workspace as two f16 limbs, v s = hi + lo with a power of two s chosen from a bound of
 // the matrix' entries (22 significand bits; the entries are bounded by the spectral norm, which is a polynomial of values in
@@ -801,14 +801,18 @@ struct OrthoCall {
   OrthoMomentum mo;
 };
 
-// Steps between two Gram matrices.  Longer chains save products with the long side (worth it from N = 2 M on; the M x M products
-// they add cost more below) and carry rounding further.  Error of five steps against 64 bits, relative, plain f32 iteration / chains
-// of 1 / 2 / 3:  256 x 2304: 3.4e-6 / 1.6e-6 / 2.2e-6 / 3.5e-6   600 x 600: 2.5e-6 / 1.0e-6 / 1.7e-6 / 5.7e-6
-//                128 x 576: 1.8e-6 / 0.9e-6 / 3.1e-6 / 3.8e-6    50 x 108: 1.3e-6 / 1.2e-6 / 8.0e-6 / 4.0e-6
-static int ortho_chain(const OrthoGroup &g) {
+// Steps between two Gram matrices.  Longer chains save products with the long side and add M x M products, so they pay from N = 2 M
+// on, and only where the long side's products fill the chip (`tiles`: 128 x 128 tiles of Q X of the whole pass; below, the number of
+// launches counts, and chains of one have the fewest).  They carry rounding further, the more the smaller M.  Five steps with chains
+// of 1 / 2 / 3, time and relative error against 64 bits, and the error of the plain iteration in f32:
+//   28 x 256 x 2304  438 / 369 / 332 us    1.5 / 1.7 / 3.0e-6  (3.4e-6)      4 x 256 x 1152   161 / 163 / 159 us    1.2 / 1.8 / 3.0e-6  (2.7e-6)
+//   2048 x 9216     2250 / 1708 / 1444     1.8 / 1.8 / 2.6e-6  (5.4e-6)      3 x 333 x 1021   171 / 181 / 180       1.2 / 1.6 / 2.7e-6  (2.7e-6)
+//   20 x 200 x 1000  226 / 212 / 208       1.3 / 2.1 / 3.7e-6  (2.5e-6)      1500 x 2000      476 / 500 / 492       1.3 / 1.3 / 4.1e-6  (3.6e-6)
+//   20 x 160 x 600   165 / 165 / 166       1.0 / 2.5 / 4.4e-6  (2.1e-6)      4 x 128 x 576    134 / 139 / 138       0.6 / 2.8 / 3.5e-6  (1.8e-6)
+static int ortho_chain(const OrthoGroup &g, long tiles) {
   const int M = og_short(g), N = og_long(g);
-  if (M < 192 || N < 2 * M) return 1;
-  return N < 4 * M ? 2 : 3;
+  if (tiles < 256 || M < 192 || N < 2 * M) return 1;
+  return M < 256 || N < 4 * M ? 2 : 3;
 }
 
 // Bounds of the matrices' spectral norms (hence of their entries) along the iteration: every one of them is a polynomial of
@@ -960,9 +964,10 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
     lo.bytes = lo.sums;
     return lo;
   }
-  long tiles = 0;
+  long tiles = 0, rect = 0;
+  for (int i = 0; i < n; ++i) rect += (long)g[i].count * og_tiles(g[i], OL_RECT, 128);
   for (int i = 0; i < n; ++i) {
-    lo.chain[i] = ortho_chain(g[i]);
+    lo.chain[i] = ortho_chain(g[i], rect);
     lo.norm_first[i] = lo.norm_blocks;
     lo.split_first[i] = lo.split_blocks;
     lo.norm_blocks += g[i].count * og_norm_blocks(g[i]);

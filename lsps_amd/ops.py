@@ -1889,6 +1889,8 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     if not (len(params) == len(grads) == len(momenta)):
         raise _lib.LspsHipError("muon_step_: %d weights, %d gradients, %d momenta" % (len(params), len(grads), len(momenta)))
     for p, g, m in zip(params, grads, momenta):
+        if not all(isinstance(t, torch.Tensor) for t in (p, g, m)):
+            raise _lib.LspsHipError("muon_step_: a weight, gradient or momentum is no tensor")
         if p.dim() < 2 or p.shape != g.shape or p.shape != m.shape or p.numel() == 0:
             raise _lib.LspsHipError("muon_step_: weight %s, gradient %s, momentum %s" % (tuple(p.shape), tuple(g.shape), tuple(m.shape)))
     if not params:

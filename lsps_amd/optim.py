@@ -289,7 +289,8 @@ class FlatMuon(FlatAdam):
         mats = [i for i, p in enumerate(g['params']) if a.touched[i] and self.is_matrix(p)]
         if mats:
             params = [g['params'][i] for i in mats]
-            ops.muon_step_([p.data for p in params], [p.grad for p in params], [self.state[p]['momentum_buffer'] for p in params],
+            flat = lambda buf: [buf[a.offsets[i]:a.offsets[i] + p.numel()].view(p.shape) for i, p in zip(mats, params)]      # noqa: E731
+            ops.muon_step_(flat(a.flat_p), flat(a.flat_g), flat(self.flat_m),
                            lr=g['lr'], momentum=g['momentum'], nesterov=g['nesterov'], weight_decay=g['weight_decay'], rms=g['rms'],
                            grad_scale=self.grad_scale, steps=g['ns_steps'], coeffs=g['ns_coeffs'], eps=g['ns_eps'])
             for p in params:

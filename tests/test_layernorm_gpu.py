@@ -232,6 +232,24 @@ def test_other_stream_and_two_graphs():
             assert all(torch.equal(p, q) for p, q in zip(out, w))
 
 
+@pytest.mark.parametrize('rows,cols', [(540001, 4096), (55000, 40001)])
+def test_beyond_32_bits(rows, cols):
+    """More than 2^31 elements: the first and the last rows, and the parameter gradients of a gradient that is zero but there."""
+    from lsps_amd import ops
+    _, _, w, b = make(1, cols, torch.float32)
+    ends = torch.tensor([0, 1, rows - 2, rows - 1], device='cuda')
+    x = torch.empty(rows, cols, device='cuda', dtype=torch.bfloat16).normal_()
+    dy = torch.zeros_like(x)
+    dy[ends] = torch.randn(4, cols, device='cuda').bfloat16()
+    leaves = [x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)]
+    y = ops.layer_norm(x, cols, w, b)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    xe, we, be = x.detach()[ends], w.detach(), b.detach()
+    check_forward(y.detach()[ends], xe, we, be)
+    check_backward(dx[ends], dw, db, xe, dy[ends], we, be)
+    assert not dx[2:rows - 2:997].any()
+
+
 def test_differentiable_once():
     from lsps_amd import ops
     x = torch.randn(4, 10, device='cuda', requires_grad=True)

@@ -47,7 +47,9 @@ def grads(count, rows, cols, seed=0, size=1e-3):
 
 SHAPES = [(1, 1, 1), (2, 1, 9), (2, 9, 1), (1, 2, 3), (3, 20, 50), (1, 50, 108), (2, 64, 64), (2, 64, 49), (1, 65, 63), (1, 128, 129),
           (2, 130, 65), (5, 100, 333), (1, 333, 1021), (2, 256, 256), (1, 257, 700), (1, 20, 8192), (3, 8192, 20), (70, 33, 40), (1, 512, 513), (3, 64, 448), (2, 449, 64), (2, 448, 30), (300, 5, 31),
-          (40, 192, 200), (1, 1024, 1100), (20, 448, 1000)]
+          (40, 192, 200), (1, 1024, 1100), (20, 448, 1000),
+          # 128 x 128 tiles with odd 64-row halves, symmetric and not; chains of two and three
+          (40, 520, 600), (40, 200, 930), (16, 260, 1100)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
@@ -205,6 +207,15 @@ def test_streams_and_graphs():
         run(1)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(p + m, want[k])) and torch.equal(out, ns)
+
+
+def test_beyond_32_bits():
+    """A stack whose working matrices pass 4 GiB: the last matrix is the one computed alone."""
+    from lsps_amd import ops
+    g = torch.randn(300, 1024, 1000, device='cuda')
+    out = ops.newton_schulz(g)
+    for k in (0, 299):
+        check(out[k], g[k])
 
 
 def test_version_counters_move():
