@@ -17,8 +17,13 @@
 // dropped lo lo is below 2^-22 of the product): f32-class results at a third of the f16 rate, 5 x the f32 MFMA rate.
 // Layout of a matrix with R rows: [column / 32][R][(column % 32) / 8][hi 8 | lo 8], rows and columns padded with zeros to multiples
 // of 64: a 32-deep chunk of a row is one 128-byte line and the rows of a chunk follow each other, so that a tile's chunk is one
-// contiguous run over all L2 channels (rows at a power-of-two pitch all fell on one channel: 2100 instead of 768 cycles per chunk
-// of a 128 x 128 tile at 2048 x 2048).  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.
+// contiguous run.  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.  X is kept one way round only:
+// Q X reads it transposed from LDS (28 x 256 x 2304: 407 us; with X^T beside X, 451).
+//
+// Times (MI355X): 28 x 256 x 2304 333 us (prologue 41, two Gram matrices 2 x 31, twelve 256 x 256 products 9 to 15 each, Q X 47 and
+// 40), 2048 x 9216 1443 us.  The 256 x 256 products are latency: 2 us from launch to launch, 1.6 to the first request, 1 to its
+// arrival, 2.5 for the product, 1.7 for the result.  The large ones run at 0.5 (symmetric) to 0.9 PFLOP/s of f16 MFMAs (a large
+// library product: 1.17): their blocks leave CUs idle (528 tiles, 256 CUs), and L2 to LDS carries 10 to 13 TB/s beside the MFMAs.
 // All matrices of a call go through one launch per product (a block finds its group of equal matrices in the kernel's arguments).
 #include <limits.h>
 #include <math.h>
@@ -39,7 +44,7 @@ typedef unsigned short og_u4u __attribute__((ext_vector_type(4), aligned(2)));
 #define ORTHO_GROUPS 16        // shapes per pass (they travel in the kernels' arguments)
 #define ORTHO_MATRICES 1024    // matrices with pointers of their own per pass
 #define ORTHO_CHAINS 3         // longest chain: steps between two Gram matrices of the long side
-#define ORTHO_NORM_BLOCK 8192 // elements per block of the norm pass
+#define ORTHO_NORM_BLOCK 8192  // elements per block of the norm pass
 #define ORTHO_PTR_PART 96      // matrices per table launch (passed by value: nothing on the host has to outlive the call)
 #define ORTHO_STEPS 64
 enum { OB_A, OB_S, OB_T, OB_R0, OB_R1, OB_SMALL, OB_X0 = OB_SMALL, OB_X1, OB_NONE };
@@ -932,12 +937,15 @@ static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
   return true;
 }
 
-// ranges of the reduction: a product whose tiles leave CUs idle splits a long reduction, down to 256 columns of it a range
-#define ORTHO_KZ 32
+// Ranges of a Gram matrix' reduction.  A product whose tiles leave CUs idle splits a long reduction into ranges of 256 columns (512
+// of the longest), at the price of the launch that adds them up.  Five steps: 3 x 333 x 1021 171 us with ranges of 256, 180 of 512, 189 of
+// 1024; 20 x 8192 149 us with 16 ranges, 166 with 32, 209 with 4; 4 x 128 x 576 122 us unsplit, 139 in two.
+#define ORTHO_KZ 16
 static int ortho_kz(int K, long own, long tiles) {
   long z = 256 / (tiles > 0 ? tiles : 1);
   if (own <= 16 && z < K / 1024) z = K / 1024;             // few tiles in the company of many: not the launch's last ones
-  if (z > K / 256) z = K / 256;
+  const long most = K < 768 ? 1 : K <= 1536 ? K / 256 : K / 512;
+  if (z > most) z = most;
   if (z > ORTHO_KZ) z = ORTHO_KZ;
   return z < 2 ? 1 : (int)z;
 }
