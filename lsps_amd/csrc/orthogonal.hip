@@ -61,7 +61,7 @@ struct OrthoPtr {
 struct OrthoGroup {
   int first;                      // blocks in front of the group's
   int aux;                        // norm and split passes: partial sums of squares in front of the group's; a product: ranges of its reduction
-  int type, jobs;                 // a product: OL_*, and how many of them
+  int type, jobs;                 // a product: OL_*, and how many of them; panels: jobs = 32-column chunks of one
   int rows, cols, count;
   int ptr;                        // first of the matrices' pointers in the table; < 0: they lie one behind the other
   unsigned x_off, s_off, p_off;   // workspace offsets in 256-byte units: long-side matrices, M x M matrices, partial products
@@ -619,14 +619,26 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
     }
 }
 
-// ---- small matrices: the whole iteration in one workgroup ----------------------------------------------------------------
+// ---- short sides of up to 64 ---------------------------------------------------------------------------------------------
+// A, Q and up to 448 columns of X fit into LDS as limbs (16 + 16 + 112 KB), so one workgroup can take a step's products one after the
+// other with a barrier between them; as launches they cost 5 us each at these sizes.  Short matrices run their whole iteration in one
+// workgroup (ortho_small_kernel).  Longer ones are cut into panels of columns, one workgroup each: a launch per step adds the panels'
+// shares of the Gram matrix up (every workgroup for itself, in a fixed order), forms Q, multiplies its panel by it and leaves the
+// panel's share of the next Gram matrix (ortho_panel_kernel).  Five steps, whole iteration / panels / the products as launches, us:
+//   64 x 128  34 / 58 / -     64 x 256  53 / 61 / -     64 x 448  85 / 64 / 112     8 of 33 x 1000  - / 71 / 128
+//   64 x 4096 - / 93 / 142    20 x 8192 - / 111 / 152   40 of 64 x 576 - / 85 / 126   80 of 64 x 576 - / 104 / 147
+// Past one workgroup per CU panels lose (400 of 64 x 576: 440, 308 as launches).  Panels of 1 or 2 chunks are as fast for one matrix and
+// slower for several (8 of 33 x 1000: 93, 79); 16 panels at most instead of 32 cost 20 x 8192 155 us, 64 cost 64 x 4096 116.
 #define ORTHO_SMALL_M 64
-#define ORTHO_SMALL_N 448      // 14 chunks of 8 KB next to A and Q, 16 KB each
+#define ORTHO_SMALL_N 448      // columns that fit into LDS
+#define ORTHO_ALONE_N 256      // up to here one workgroup per matrix
+#define ORTHO_WIDE 4           // narrowest panel, in chunks of 32 columns
+#define ORTHO_PANELS 32        // longest row of panels: every workgroup reads 16 KB of each
 struct OrthoSmallStep {
   float gram, s0, s1, diag, x;      // factors of A; of A A, A and I in Q = a I + b A + c A A; of Q X
 };
 struct OrthoSmall {
-  OrthoGroups gs;
+  OrthoGroups gs;                   // aux: partial sums of squares in front of the group's (panels)
   OrthoSmallStep step[ORTHO_STEPS];
   OrthoMomentum mo;
   int steps, mode;
@@ -635,10 +647,135 @@ struct OrthoSmall {
 
 // byte of 16-byte unit u of row r of a chunk of 64 rows x 32 columns in LDS
 __device__ __forceinline__ int og_unit(int r, int u) { return r * 128 + ((u ^ ((r >> 1) & 7)) << 4); }
+// 8 columns of a row, half chunk `half`, one limb: a lane's MFMA operand
+__device__ __forceinline__ og_h8 og_frag(const char *chunk, int row, int half, int limb) {
+  return *reinterpret_cast<const og_h8 *>(chunk + og_unit(row, (half * 2 + ((threadIdx.x >> 5) & 1)) * 2 + limb));
+}
+// 4 values of a row from column 8 q + 4 (lane / 32) on
+__device__ __forceinline__ void og_put(char *chunk, int row, int q, const float (&v)[4]) {
+  const int lh = (threadIdx.x >> 5) & 1;
+  og_h4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    _Float16 a, b;
+    og_split(v[e], a, b);
+    h[e] = a;
+    l[e] = b;
+  }
+  *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2) + lh * 8) = h;
+  *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2 + 1) + lh * 8) = l;
+}
 
-// One matrix per workgroup, M <= 64 <= and N <= 448 after padding: X, A and Q stay in LDS as limbs, the three products of a step
-// follow each other with a barrier between them (through launches they take ~5 us each at these sizes).  4 waves; A and Q: one
-// 32 x 32 tile each; X <- Q X: a wave owns whole chunks of 32 columns, so it can write where it has read.
+// this wave's 32 x 32 tile of Y Y^T, Y = `chunks` chunks at `in`; small cross products apart from hi hi, as in ortho_product_kernel
+__device__ __forceinline__ void og_square(const char *in, int chunks, int ti, int tj, float (&v)[16]) {
+  const int l31 = threadIdx.x & 31;
+  og_f16v acc, acx;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = acx[e] = 0.f;
+  for (int c = 0; c < chunks; ++c, in += 8192)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const og_h8 ih = og_frag(in, ti + l31, h, 0), il = og_frag(in, ti + l31, h, 1);
+      const og_h8 jh = og_frag(in, tj + l31, h, 0), jl = og_frag(in, tj + l31, h, 1);
+      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, il, acx, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, ih, acc, 0, 0, 0);
+      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jl, ih, acx, 0, 0, 0);
+    }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = acc[e] + acx[e];
+}
+
+// A from the wave's tile of it (v, unscaled), then Q; barriers in front of, between and behind them
+__device__ __forceinline__ void og_make_q(char *A, char *Q, int ti, int tj, const float (&v)[16], const OrthoSmallStep &st) {
+  const int l31 = threadIdx.x & 31, lh = (threadIdx.x >> 5) & 1;
+  char *a = A + (tj >> 5) * 8192;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float w[4] = {st.gram * v[q * 4], st.gram * v[q * 4 + 1], st.gram * v[q * 4 + 2], st.gram * v[q * 4 + 3]};
+    og_put(a, ti + l31, q, w);
+  }
+  __syncthreads();
+  float p[16];
+  og_square(A, 2, ti, tj, p);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const og_h4 eh = *reinterpret_cast<const og_h4 *>(a + og_unit(ti + l31, q * 2) + lh * 8);
+    const og_h4 el = *reinterpret_cast<const og_h4 *>(a + og_unit(ti + l31, q * 2 + 1) + lh * 8);
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = st.s0 * p[q * 4 + e] + st.s1 * ((float)eh[e] + (float)el[e]) + (ti + l31 == tj + q * 8 + lh * 4 + e ? st.diag : 0.f);
+    og_put(Q + (tj >> 5) * 8192, ti + l31, q, w);
+  }
+  __syncthreads();
+}
+
+// Q times one chunk of 32 columns of X (transposing reads), all 64 rows: store(row, q, 4 values) gets the result.  A wave takes
+// whole chunks, so the result may go where they were read.
+template <typename F>
+__device__ __forceinline__ void og_apply(const char *Q, const char *chunk, float factor, F store) {
+  const int lane = threadIdx.x & 63, l31 = lane & 31, lh = lane >> 5;
+  og_f16v acc[2], acx[2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[f][e] = acx[f][e] = 0.f;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2;
+    og_h8 x[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      x[q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)chunk + og_unit(r, u + q) + (lane & 1) * 8,
+                                                  (const unsigned char *)chunk + og_unit(r + 4, u + q) + (lane & 1) * 8));
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const og_h8 ih = og_frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 0), il = og_frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 1);
+      acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], il, acx[f], 0, 0, 0);
+      acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], ih, acc[f], 0, 0, 0);
+      acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[1], ih, acx[f], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = factor * (acc[f][q * 4 + e] + acx[f][q * 4 + e]);
+      store(f * 32 + l31, q, v);
+    }
+}
+
+// 8 columns of f32 in the place of their two units, and from there into limbs
+__device__ __forceinline__ void og_place(char *chunk, int row, int q, const float (&v)[8]) {
+  *reinterpret_cast<og_f4 *>(chunk + og_unit(row, q * 2)) = og_f4{v[0], v[1], v[2], v[3]};
+  *reinterpret_cast<og_f4 *>(chunk + og_unit(row, q * 2 + 1)) = og_f4{v[4], v[5], v[6], v[7]};
+}
+__device__ __forceinline__ void og_limbs(char *chunk, int row, int q, float norm, float scale) {
+  char *p0 = chunk + og_unit(row, q * 2), *p1 = chunk + og_unit(row, q * 2 + 1);
+  const og_f4 f0 = *reinterpret_cast<og_f4 *>(p0), f1 = *reinterpret_cast<og_f4 *>(p1);
+  og_h8 h, l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    _Float16 a, b;
+    og_split((e < 4 ? f0[e] : f1[e - 4]) / norm * scale, a, b);
+    h[e] = a;
+    l[e] = b;
+  }
+  *reinterpret_cast<og_h8 *>(p0) = h;
+  *reinterpret_cast<og_h8 *>(p1) = l;
+}
+
+// sum of a workgroup's 256 values, in 64 bits
+__device__ __forceinline__ double og_block_sum(double s, double *red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ortho_small_kernel(OrthoSmall c) {
   extern __shared__ __align__(1024) char smem[];
@@ -647,15 +784,13 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(OrthoSmall c) {
   const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
   const int mat = blockIdx.x - g.first;
   const OrthoPtr ptr = ortho_ptr(c.gs, g, mat, sizeof(T));
-  const int m = og_short(g), n = og_long(g), chunks = (n + 31) / 32;
+  const int m = og_short(g), n = og_long(g), chunks = (n + 31) / 32, groups = chunks * 4;
   const bool tall = g.rows > g.cols;
   char *A = smem, *Q = smem + 16384, *X = smem + 32768;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, lh = lane >> 5;
-  // G as f32, 8 columns in the place of their two units; lanes run along the rows of G
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lh = (threadIdx.x >> 5) & 1;
   const T *src = (const T *)ptr.g;
-  const int groups = chunks * 4;                                 // of 8 columns
   double sum = 0.;
-  for (int t = threadIdx.x; t < 64 * groups; t += 256) {
+  for (int t = threadIdx.x; t < 64 * groups; t += 256) {         // lanes run along the rows of G
     const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
     float v[8];
 #pragma unroll
@@ -674,126 +809,120 @@ __global__ __launch_bounds__(256) void ortho_small_kernel(OrthoSmall c) {
       }
       sum += (double)v[e] * (double)v[e];
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const og_f4 f = {v[h * 4], v[h * 4 + 1], v[h * 4 + 2], v[h * 4 + 3]};
-      *reinterpret_cast<og_f4 *>(X + (q >> 2) * 8192 + og_unit(i, (q & 3) * 2 + h)) = f;
-    }
+    og_place(X + (q >> 2) * 8192, i, q & 3, v);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  if (lane == 0) red[wave] = sum;
-  __syncthreads();
-  const float norm = (float)(sqrt(red[0] + red[1] + red[2] + red[3]) + (double)c.eps);
-  for (int t = threadIdx.x; t < 64 * groups; t += 256) {         // every thread turns what it stored into limbs
+  const float norm = (float)(sqrt(og_block_sum(sum, red)) + (double)c.eps);
+  for (int t = threadIdx.x; t < 64 * groups; t += 256) {         // every thread turns what it placed into limbs
     const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
-    char *p0 = X + (q >> 2) * 8192 + og_unit(i, (q & 3) * 2), *p1 = X + (q >> 2) * 8192 + og_unit(i, (q & 3) * 2 + 1);
-    const og_f4 f0 = *reinterpret_cast<og_f4 *>(p0), f1 = *reinterpret_cast<og_f4 *>(p1);
-    og_h8 h, l;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      _Float16 a, b;
-      og_split((e < 4 ? f0[e] : f1[e - 4]) / norm * c.x0, a, b);
-      h[e] = a;
-      l[e] = b;
-    }
-    *reinterpret_cast<og_h8 *>(p0) = h;
-    *reinterpret_cast<og_h8 *>(p1) = l;
+    og_limbs(X + (q >> 2) * 8192, i, q & 3, norm, c.x0);
   }
   const int ti = (wave >> 1) * 32, tj = (wave & 1) * 32;         // this wave's tile of A and Q
   for (int k = 0; k < c.steps; ++k) {
     const OrthoSmallStep st = c.step[k];
-    auto frag = [&](const char *chunk, int row, int half, int limb) {      // 8 columns of a row: half-chunk `half`
-      return *reinterpret_cast<const og_h8 *>(chunk + og_unit(row, (half * 2 + lh) * 2 + limb));
-    };
-    auto put = [&](char *chunk, int row, int q, const float (&v)[4]) {     // 4 values of a row from column 8 q + 4 lh on
-      og_h4 h, l;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        _Float16 a, b;
-        og_split(v[e], a, b);
-        h[e] = a;
-        l[e] = b;
-      }
-      *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2) + lh * 8) = h;
-      *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2 + 1) + lh * 8) = l;
-    };
-    // A = X X^T, then Q = a I + b A + c A A; small cross products apart from hi hi, as in ortho_product_kernel
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const char *in = which ? A : X;
-      og_f16v acc, acx;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[e] = acx[e] = 0.f;
-      __syncthreads();
-#pragma unroll 4
-      for (int h = 0; h < (which ? 4 : chunks * 2); ++h) {
-        const char *chunk = in + (h >> 1) * 8192;
-        const og_h8 ih = frag(chunk, ti + l31, h & 1, 0), il = frag(chunk, ti + l31, h & 1, 1);
-        const og_h8 jh = frag(chunk, tj + l31, h & 1, 0), jl = frag(chunk, tj + l31, h & 1, 1);
-        acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, il, acx, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, ih, acc, 0, 0, 0);
-        acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jl, ih, acx, 0, 0, 0);
-      }
-      char *chunk = (which ? Q : A) + (tj >> 5) * 8192;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
-        const char *e1 = A + (tj >> 5) * 8192;
-        const og_h4 eh = *reinterpret_cast<const og_h4 *>(e1 + og_unit(ti + l31, q * 2) + lh * 8);
-        const og_h4 el = *reinterpret_cast<const og_h4 *>(e1 + og_unit(ti + l31, q * 2 + 1) + lh * 8);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = acc[q * 4 + e] + acx[q * 4 + e];
-          if (which) v[e] = st.s0 * p + st.s1 * ((float)eh[e] + (float)el[e]) + (ti + l31 == tj + q * 8 + lh * 4 + e ? st.diag : 0.f);
-          else v[e] = st.gram * p;
-        }
-        put(chunk, ti + l31, q, v);
-      }
-    }
+    float v[16];
     __syncthreads();
-    // X = Q X: the reduction runs down the rows of X (transposing reads)
+    og_square(X, chunks, ti, tj, v);
+    og_make_q(A, Q, ti, tj, v, st);
     for (int ch = wave; ch < chunks; ch += 4) {
       char *chunk = X + ch * 8192;
-      og_f16v acc[2], acx[2];
+      og_apply(Q, chunk, st.x, [&](int i, int q, const float (&w)[4]) {
+        if (k + 1 < c.steps) {
+          og_put(chunk, i, q, w);
+        } else if (i < m) {
 #pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[f][e] = acx[f][e] = 0.f;
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2;
-        og_h8 x[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          x[q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)chunk + og_unit(r, u + q) + (lane & 1) * 8,
-                                                      (const unsigned char *)chunk + og_unit(r + 4, u + q) + (lane & 1) * 8));
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const og_h8 ih = frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 0), il = frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 1);
-          acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], il, acx[f], 0, 0, 0);
-          acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], ih, acc[f], 0, 0, 0);
-          acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[1], ih, acx[f], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int i = f * 32 + l31, j = ch * 32 + q * 8 + lh * 4;
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = st.x * (acc[f][q * 4 + e] + acx[f][q * 4 + e]);
-          if (k + 1 < c.steps) {
-            put(chunk, i, q, v);
-          } else if (i < m) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (j + e < n) og_result(ptr.out, tall ? (long)(j + e) * m + i : (long)i * n + j + e, v[e], c.mode, g.step, c.decay);
+          for (int e = 0; e < 4; ++e) {
+            const int j = ch * 32 + q * 8 + lh * 4 + e;
+            if (j < n) og_result(ptr.out, tall ? (long)j * m + i : (long)i * n + j, w[e], c.mode, g.step, c.decay);
           }
         }
+      });
     }
   }
+}
+
+__host__ __device__ static inline int og_panels(const OrthoGroup &g) { return ((og_long(g) + 31) / 32 + g.jobs - 1) / g.jobs; }
+
+// Launch k of a chain of panels: k = 0 forms X0's panel and its share of the first Gram matrix, launch k > 0 takes step k - 1.  X's
+// panels lie in the workspace as they lie in LDS; the shares (f32, as the MFMAs leave them) go to one of two sets in turn, since
+// other workgroups may still read the last launch's.
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256) void ortho_panel_kernel(OrthoSmall c, char *__restrict__ ws, const double *__restrict__ sums, int k) {
+  extern __shared__ __align__(1024) char smem[];
+  __shared__ double red[4];
+  int grp;
+  const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
+  const int panels = og_panels(g), wide = g.jobs, mat = og_div(blockIdx.x - g.first, panels), pan = blockIdx.x - g.first - mat * panels;
+  const int m = og_short(g), n = og_long(g), all = (n + 31) / 32, chunks = all - pan * wide < wide ? all - pan * wide : wide;
+  const bool tall = g.rows > g.cols;
+  char *A = smem, *Q = smem + 16384, *X = smem + 32768;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lh = (threadIdx.x >> 5) & 1;
+  const int ti = (wave >> 1) * 32, tj = (wave & 1) * 32;
+  const OrthoPtr ptr = ortho_ptr(c.gs, g, mat, sizeof(T));
+  char *mine = ws + (size_t)g.x_off * 256 + ((size_t)mat * all + pan * wide) * 8192;
+  og_f4 *share = reinterpret_cast<og_f4 *>(ws + (size_t)g.p_off * 256);                       // [set][mat][panel][q][thread]
+  const size_t set = (size_t)g.count * panels * 1024;
+  if (k == 0) {
+    const int nb = og_norm_blocks(g);
+    double s = 0.;
+    for (int i = threadIdx.x; i < nb; i += 256) s += sums[g.aux + (long)mat * nb + i];
+    const float norm = (float)(sqrt(og_block_sum(s, red)) + (double)c.eps);
+    const T *src = (const T *)ptr.g;
+    const int groups = chunks * 4;
+    for (int t = threadIdx.x; t < 64 * groups; t += 256) {       // lanes run along the rows of G
+      const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = pan * wide * 32 + q * 8 + e;
+        const bool in = i < m && j < n;
+        const long o = tall ? (long)j * m + i : (long)i * n + j;
+        v[e] = in ? (float)src[o] : 0.f;
+        if constexpr (MUON)
+          if (in) v[e] = c.mo.nesterov ? fmaf(c.mo.mu, ptr.m[o], v[e] * c.mo.gscale) : ptr.m[o];
+      }
+      og_place(X + (q >> 2) * 8192, i, q & 3, v);
+      og_limbs(X + (q >> 2) * 8192, i, q & 3, norm, c.x0);
+    }
+  } else {
+    for (int t = threadIdx.x; t < chunks * 512; t += 256)
+      reinterpret_cast<og_h8 *>(X)[t] = reinterpret_cast<const og_h8 *>(mine)[t];
+    const OrthoSmallStep st = c.step[k - 1];
+    const og_f4 *p = share + ((k - 1) & 1) * set + (size_t)mat * panels * 1024 + threadIdx.x;
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = 0.f;
+#pragma unroll 4
+    for (int z = 0; z < panels; ++z, p += 1024)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const og_f4 w = p[q * 256];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q * 4 + e] += w[e];
+      }
+    og_make_q(A, Q, ti, tj, v, st);
+    for (int ch = wave; ch < chunks; ch += 4) {
+      char *chunk = X + ch * 8192;
+      og_apply(Q, chunk, st.x, [&](int i, int q, const float (&w)[4]) {
+        if (k < c.steps) {
+          og_put(chunk, i, q, w);
+        } else if (i < m) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = (pan * wide + ch) * 32 + q * 8 + lh * 4 + e;
+            if (j < n) og_result(ptr.out, tall ? (long)j * m + i : (long)i * n + j, w[e], c.mode, g.step, c.decay);
+          }
+        }
+      });
+    }
+    if (k == c.steps) return;
+  }
+  __syncthreads();
+  float v[16];
+  og_square(X, chunks, ti, tj, v);
+  og_f4 *o = share + (k & 1) * set + ((size_t)mat * panels + pan) * 1024 + threadIdx.x;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) o[q * 256] = og_f4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
+  for (int t = threadIdx.x; t < chunks * 512; t += 256) reinterpret_cast<og_h8 *>(mine)[t] = reinterpret_cast<const og_h8 *>(X)[t];
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -952,12 +1081,27 @@ static int ortho_kz(int K, long own, long tiles) {
 
 struct OrthoLayout {
   size_t sums, bytes;
-  bool small;                       // every matrix fits ortho_small_kernel
+  bool small, panels;               // every matrix fits ortho_small_kernel, ortho_panel_kernel
   int chain[ORTHO_GROUPS];
   int kz[ORTHO_GROUPS];             // of the Gram matrices
   int norm_first[ORTHO_GROUPS], split_first[ORTHO_GROUPS];
   int norm_blocks, split_blocks;
 };
+
+// Widths of the panels (g[i].jobs): the smallest from ORTHO_WIDE chunks on that leaves no matrix more than ORTHO_PANELS
+// panels and the pass no more workgroups than CUs.  False if none does.
+static bool ortho_panel_chunks(OrthoGroup *g, int n) {
+  for (int w = ORTHO_WIDE; w <= ORTHO_SMALL_N / 32; ++w) {
+    long blocks = 0, most = 0;
+    for (int i = 0; i < n; ++i) {
+      g[i].jobs = w;
+      blocks += (long)g[i].count * og_panels(g[i]);
+      if (og_panels(g[i]) > most) most = og_panels(g[i]);
+    }
+    if (blocks <= 256 && most <= ORTHO_PANELS) return true;
+  }
+  return false;
+}
 
 // workspace: pointers | partial sums of squares | per group X (two when there is more than one chain), the M x M matrices, the
 // partial Gram matrices
@@ -965,24 +1109,44 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
   OrthoLayout lo;
   memset(&lo, 0, sizeof lo);
   lo.sums = align_up(sizeof(OrthoPtr) * ORTHO_MATRICES, 256);
-  lo.small = true;
-  for (int i = 0; i < n; ++i) lo.small = lo.small && og_short(g[i]) <= ORTHO_SMALL_M && og_long(g[i]) <= ORTHO_SMALL_N;
+  lo.panels = true;
+  int most = 0;
+  for (int i = 0; i < n; ++i) {
+    lo.chain[i] = 1;
+    lo.norm_first[i] = lo.norm_blocks;
+    lo.norm_blocks += g[i].count * og_norm_blocks(g[i]);
+    if (og_long(g[i]) > most) most = og_long(g[i]);
+    lo.panels = lo.panels && og_short(g[i]) <= ORTHO_SMALL_M;
+  }
+  size_t at = lo.sums + align_up(lo.norm_blocks * sizeof(double), 256);
+  lo.small = lo.panels && most <= ORTHO_ALONE_N;
+  if (lo.panels && !lo.small) {
+    lo.panels = ortho_panel_chunks(g, n);
+    lo.small = !lo.panels && most <= ORTHO_SMALL_N;
+  }
   if (lo.small) {
-    for (int i = 0; i < n; ++i) lo.chain[i] = 1;
+    lo.panels = false;
     lo.bytes = lo.sums;
+    return lo;
+  }
+  if (lo.panels) {                                                       // X | two sets of the panels' shares
+    for (int i = 0; i < n; ++i) {
+      g[i].x_off = (unsigned)(at / 256);
+      at += (size_t)g[i].count * ((og_long(g[i]) + 31) / 32) * 8192;
+      g[i].p_off = (unsigned)(at / 256);
+      at += (size_t)g[i].count * og_panels(g[i]) * 2 * 16384;
+    }
+    lo.bytes = at;
     return lo;
   }
   long tiles = 0, rect = 0;
   for (int i = 0; i < n; ++i) rect += (long)g[i].count * og_tiles(g[i], OL_RECT, 128);
   for (int i = 0; i < n; ++i) {
     lo.chain[i] = ortho_chain(g[i], rect);
-    lo.norm_first[i] = lo.norm_blocks;
     lo.split_first[i] = lo.split_blocks;
-    lo.norm_blocks += g[i].count * og_norm_blocks(g[i]);
     lo.split_blocks += g[i].count * og_split_blocks(g[i]);
     tiles += (long)g[i].count * og_tiles(g[i], OL_SYM, 64);
   }
-  size_t at = lo.sums + align_up(lo.norm_blocks * sizeof(double), 256);
   for (int i = 0; i < n; ++i) {
     const size_t M = og_pad(og_short(g[i])), N = og_pad(og_long(g[i]));
     g[i].x_off = (unsigned)(at / 256);
@@ -1031,7 +1195,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     lv.gs.g[i].first = i < n ? lo.norm_first[i] : INT_MAX;
     lv.gs.g[i].aux = lo.norm_first[i];
   }
-  if (lo.small) {
+  if (lo.small || lo.panels) {
     OrthoSmall sm;
     memset(&sm, 0, sizeof sm);
     sm.gs = lv.gs;
@@ -1041,20 +1205,34 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     sm.decay = c.decay;
     sm.eps = c.eps;
     sm.x0 = x0;
-    int blocks = 0, most = 0;
+    int blocks = 0, most = 0;                                            // most: chunks that a workgroup keeps in LDS
     for (int i = 0; i < n; ++i) {
+      const int chunks = (og_long(g[i]) + 31) / 32, kept = lo.panels && g[i].jobs < chunks ? g[i].jobs : chunks;
       sm.gs.g[i].first = blocks;
-      blocks += g[i].count;
-      if (og_long(g[i]) > most) most = og_long(g[i]);
+      blocks += lo.panels ? g[i].count * og_panels(g[i]) : g[i].count;
+      if (kept > most) most = kept;
     }
     for (int k = 0; k < c.steps; ++k) {
       const OrthoJob *a = plan[0].level[3 * k].job, *q = plan[0].level[3 * k + 1].job, *x = plan[0].level[3 * k + 2].job;
       sm.step[k] = OrthoSmallStep{a->k0, q->k0, q->k1, q->diag, x->k0};
     }
-    const int lds = 32768 + (most + 31) / 32 * 8192;
-    auto kernel = c.mode == OM_MUON ? ortho_small_kernel<float, true> : c.bf16 ? ortho_small_kernel<__bf16, false> : ortho_small_kernel<float, false>;
-    if (const int rc = lds_optin(reinterpret_cast<const void *>(kernel), 32768 + ORTHO_SMALL_N / 32 * 8192, "ortho_small_kernel")) return rc;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), lds, st, sm);
+    const int lds = 32768 + most * 8192;
+#define ORTHO_SMALL(T, MUON)                                                                                                            \
+  do {                                                                                                                                  \
+    const void *fn = lo.small ? reinterpret_cast<const void *>(&ortho_small_kernel<T, MUON>) : reinterpret_cast<const void *>(&ortho_panel_kernel<T, MUON>); \
+    if (const int rc = lds_optin(fn, 32768 + ORTHO_SMALL_N / 32 * 8192, "ortho_small_kernel")) return rc;                               \
+    if (lo.small) {                                                                                                                     \
+      hipLaunchKernelGGL((ortho_small_kernel<T, MUON>), dim3(blocks), dim3(256), lds, st, sm);                                          \
+    } else {                                                                                                                            \
+      hipLaunchKernelGGL((ortho_norm_kernel<T, MUON>), dim3(lo.norm_blocks), dim3(256), 0, st, lv.gs, sums, c.mo);                      \
+      for (int k = 0; k <= c.steps; ++k)                                                                                                \
+        hipLaunchKernelGGL((ortho_panel_kernel<T, MUON>), dim3(blocks), dim3(256), lds, st, sm, ws, sums, k);                           \
+    }                                                                                                                                   \
+  } while (0)
+    if (c.mode == OM_MUON) ORTHO_SMALL(float, true);
+    else if (!c.bf16) ORTHO_SMALL(float, false);
+    else ORTHO_SMALL(__bf16, false);
+#undef ORTHO_SMALL
     LSPS_CHECK_LAUNCH("newton_schulz");
     return 0;
   }

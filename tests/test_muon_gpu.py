@@ -46,7 +46,11 @@ def grads(count, rows, cols, seed=0, size=1e-3):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 9), (2, 9, 1), (1, 2, 3), (3, 20, 50), (1, 50, 108), (2, 64, 64), (2, 64, 49), (1, 65, 63), (1, 128, 129),
-          (2, 130, 65), (5, 100, 333), (1, 333, 1021), (2, 256, 256), (1, 257, 700), (1, 20, 8192), (3, 8192, 20), (70, 33, 40), (1, 512, 513), (3, 64, 448), (2, 449, 64), (2, 448, 30), (300, 5, 31),
+          (2, 130, 65), (5, 100, 333), (1, 333, 1021), (2, 256, 256), (1, 257, 700), (1, 20, 8192), (3, 8192, 20), (70, 33, 40), (1, 512, 513),
+          (3, 64, 448), (2, 449, 64), (2, 448, 30), (300, 5, 31),
+          # short sides of up to 64: panels of several widths, the last one narrow, and too many of them for panels
+          (2, 64, 257), (2, 64, 449), (3, 50, 1000), (2, 9000, 33), (1, 1, 14336), (2, 3, 14337), (40, 64, 576), (70, 64, 448),
+          (300, 40, 300), (90, 20, 700),
           (40, 192, 200), (1, 1024, 1100), (20, 448, 1000),
           # 128 x 128 tiles with odd 64-row halves, symmetric and not; chains of two and three
           (40, 520, 600), (40, 200, 930), (16, 260, 1100)]
@@ -135,7 +139,8 @@ def muon_reference(p, g, m, lr, momentum, nesterov, wd, rms, gscale, steps=5):
 
 SETS = [[(50, 108)], [(50, 108), (20, 50), (50, 20), (108, 50)], [(64, 1, 7, 7), (128, 64, 3, 3), (20, 48, 2, 2), (1, 9), (9, 1), (256, 300)],
         [(33 + i % 7, 20 + i) for i in range(70)],
-        [(30, 40), (40, 30), (30, 40), (200, 900), (70, 30), (200, 900), (520, 2100), (400, 420), (40, 30), (192, 500)]]
+        [(30, 40), (40, 30), (30, 40), (200, 900), (70, 30), (200, 900), (520, 2100), (400, 420), (40, 30), (192, 500)],
+        [(64, 600), (20, 8192), (900, 40), (30, 40)]]
 
 
 @pytest.mark.parametrize('nesterov', [True, False])
