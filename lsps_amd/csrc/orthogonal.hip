@@ -37,6 +37,8 @@ namespace lsps {
 typedef _Float16 og_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 og_h4 __attribute__((ext_vector_type(4)));
 typedef float og_f16v __attribute__((ext_vector_type(16)));
+typedef float og_f2 __attribute__((ext_vector_type(2)));
+typedef _Float16 og_h2 __attribute__((ext_vector_type(2)));
 typedef float og_f4 __attribute__((ext_vector_type(4)));
 typedef float og_f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short og_u4u __attribute__((ext_vector_type(4), aligned(2)));
@@ -199,10 +201,22 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroups gs, double 
   if (threadIdx.x == 0) sums[g.aux + rel] = red[0] + red[1] + red[2] + red[3];
 }
 
-__device__ __forceinline__ void og_split(float v, _Float16 &hi, _Float16 &lo) {
-  hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
+// 4 values as two limbs each.  Kept in pairs, with -1 out of the compiler's sight: so a pair takes one conversion and two mixed
+// fused multiply-adds (6 instructions otherwise).
+__device__ __forceinline__ void og_split(const float (&v)[4], og_h4 &hi, og_h4 &lo) {
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    og_h2 h = __builtin_convertvector((og_f2{v[e], v[e + 1]}), og_h2);
+    float minus = -1.f;
+    asm("" : "+s"(minus), "+v"(h));
+    hi[e] = h[0];
+    hi[e + 1] = h[1];
+    lo[e] = (_Float16)fmaf((float)h[0], minus, v[e]);
+    lo[e + 1] = (_Float16)fmaf((float)h[1], minus, v[e + 1]);
+  }
 }
+
+__device__ __forceinline__ og_h8 og_join(const og_h4 (&v)[2]) { return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // X0 as limbs, the short side in rows.  One 64 x 64 tile of G per block, through LDS (turned round there for a tall G).
 template <typename T, bool MUON>
@@ -252,17 +266,17 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroups gs, char *
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int u = threadIdx.x + k * 256, i = u >> 3, j = (u & 7) * 8;
-    og_h8 h, l;
+    og_h4 h[2], l[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      _Float16 x, y;
-      og_split(tall ? tile[j + e][i] : tile[i][j + e], x, y);
-      h[e] = x;
-      l[e] = y;
+    for (int e = 0; e < 8; e += 4) {
+      float x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = tall ? tile[j + e + c][i] : tile[i][j + e + c];
+      og_split(x, h[e / 4], l[e / 4]);
     }
     og_h8 *o = reinterpret_cast<og_h8 *>(dst + og_at(M, i0 + i, j0 + j));
-    o[0] = h;
-    o[1] = l;
+    o[0] = og_join(h);
+    o[1] = og_join(l);
   }
 }
 
@@ -556,13 +570,9 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
         if (!last) {
           og_h4 h, l;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 4; ++k)
             if (i == j + k) v[k] += job.diag;
-            _Float16 a, b;
-            og_split(v[k], a, b);
-            h[k] = a;
-            l[k] = b;
-          }
+          og_split(v, h, l);
           *reinterpret_cast<og_h4 *>(tp + l31 * TP + q * 32 + lh * 8) = h;
           *reinterpret_cast<og_h4 *>(tp + l31 * TP + q * 32 + 16 + lh * 8) = l;
           hq[q] = h;
@@ -631,14 +641,13 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
 // slower for several (8 of 33 x 1000: 93, 79); 16 panels at most instead of 32 cost 20 x 8192 155 us, 64 cost 64 x 4096 116.
 #define ORTHO_SMALL_M 64
 #define ORTHO_SMALL_N 448      // columns that fit into LDS
-#define ORTHO_ALONE_N 256      // up to here one workgroup per matrix
 #define ORTHO_WIDE 4           // narrowest panel, in chunks of 32 columns
 #define ORTHO_PANELS 32        // longest row of panels: every workgroup reads 16 KB of each
 struct OrthoSmallStep {
   float gram, s0, s1, diag, x;      // factors of A; of A A, A and I in Q = a I + b A + c A A; of Q X
 };
 struct OrthoSmall {
-  OrthoGroups gs;                   // aux: partial sums of squares in front of the group's (panels)
+  OrthoGroups gs;
   OrthoSmallStep step[ORTHO_STEPS];
   OrthoMomentum mo;
   int steps, mode;
@@ -655,274 +664,393 @@ __device__ __forceinline__ og_h8 og_frag(const char *chunk, int row, int half, i
 __device__ __forceinline__ void og_put(char *chunk, int row, int q, const float (&v)[4]) {
   const int lh = (threadIdx.x >> 5) & 1;
   og_h4 h, l;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    _Float16 a, b;
-    og_split(v[e], a, b);
-    h[e] = a;
-    l[e] = b;
-  }
+  og_split(v, h, l);
   *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2) + lh * 8) = h;
   *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2 + 1) + lh * 8) = l;
 }
 
-// this wave's 32 x 32 tile of Y Y^T, Y = `chunks` chunks at `in`; small cross products apart from hi hi, as in ortho_product_kernel
-__device__ __forceinline__ void og_square(const char *in, int chunks, int ti, int tj, float (&v)[16]) {
+// A panel's elements, 256 threads, 64 columns x 16 per thread at a time; lanes run along the rows of G (TALL: along the short side).
+// Loads and stores go through buffer descriptors, whose bounds check does the padding's zeros: no branch stands between 16 loads.
+template <bool TALL>
+struct OgWalk {
+  int so, valid, row;             // elements between two of a thread's; how many it has there; bytes of its row and column in LDS
+  int o, step, left;              // first element; to the next 64 columns; columns left
+  int lane, wave, m;
+  __device__ __forceinline__ OgWalk(const OrthoGroup &g, int j0, int chunks) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    m = og_short(g);
+    const int n = og_long(g);
+    left = n - j0 < chunks * 32 ? n - j0 : chunks * 32;
+    so = TALL ? 4 * m : 4 * n;
+    step = TALL ? 64 * m : 64;
+    o = TALL ? (j0 + wave) * m + lane : wave * n + j0 + lane;
+    row = TALL ? lane * 128 + wave * 4 : (lane >> 5) * 8192 + wave * 128 + (lane & 3) * 4;
+    count();
+  }
+  __device__ __forceinline__ void count() { valid = TALL ? (lane < m ? (left - wave + 3) >> 2 : 0) : lane < left ? (m - wave + 3) >> 2 : 0; }
+  __device__ __forceinline__ void next() {
+    left -= 64;
+    o += step;
+    row += 2 * 8192;
+    count();
+  }
+  __device__ __forceinline__ int at(int e) const { return e < valid ? o + e * so : -1; }      // -1: behind every buffer
+  __device__ __forceinline__ int lds(int e) const {
+    if constexpr (TALL) return row + (e >> 3) * 8192 + (((e & 7) ^ ((lane >> 1) & 7)) << 4);
+    else return row + e * 512 + ((((lane & 31) >> 2) ^ ((wave >> 1) + 2 * (e & 3))) << 4);
+  }
+};
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t og_buffer(void *p, int bytes) { return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00027000); }
+template <typename T>
+__device__ __forceinline__ float og_get(__amdgpu_buffer_rsrc_t b, int o) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, o < 0 ? -1 : o * 4, 0, 0));
+  else return __uint_as_float((unsigned)__builtin_amdgcn_raw_buffer_load_b16(b, o < 0 ? -1 : o * 2, 0, 0) << 16);
+}
+__device__ __forceinline__ void og_set(__amdgpu_buffer_rsrc_t b, int o, float v) {
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), b, o < 0 ? -1 : o * 4, 0, 0);
+}
+
+// G (Muon: the momentum, updated on the way) as f32 into the place of its limbs; returns the thread's sum of squares
+template <typename T, bool MUON, bool TALL>
+__device__ __forceinline__ double og_fetch(const OrthoGroup &g, int j0, int chunks, const OrthoPtr &ptr, const OrthoMomentum &mo, char *X) {
+  const int size = g.rows * g.cols;
+  const __amdgpu_buffer_rsrc_t src = og_buffer(const_cast<void *>((const void *)ptr.g), size * (int)sizeof(T));
+  const __amdgpu_buffer_rsrc_t mom = og_buffer(ptr.m, MUON ? size * 4 : 0);
+  OgWalk<TALL> w(g, j0, chunks);
+  double sum = 0.;
+  for (int c = 0; c < chunks; c += 2, w.next()) {
+    float v[16], mm[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = og_get<T>(src, w.at(e));
+    if constexpr (MUON)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mm[e] = og_get<float>(mom, w.at(e));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if constexpr (MUON) {
+        v[e] *= mo.gscale;
+        mm[e] = fmaf(mo.mu, mm[e], v[e]);
+        og_set(mom, w.at(e), mm[e]);
+        v[e] = mo.nesterov ? fmaf(mo.mu, mm[e], v[e]) : mm[e];
+      }
+      sum += (double)v[e] * (double)v[e];
+      *reinterpret_cast<float *>(X + w.lds(e)) = v[e];
+    }
+  }
+  return sum;
+}
+
+// f32 into limbs in place: X0 = G / norm * scale.  The quotient is a power of two times a factor near the scale: no division per
+// element, and nothing overflows on the way for any norm.
+template <int MT>
+__device__ __forceinline__ void og_limbs(char *X, int chunks, double norm, float scale) {
+  int ex;
+  const float f = (float)((double)scale / frexp(norm, &ex));
+  for (int t = threadIdx.x; t < chunks * 128 * MT; t += 256) {
+    const int row = t & (32 * MT - 1), q = t / (32 * MT);
+    char *chunk = X + (q >> 2) * 8192, *p0 = chunk + og_unit(row, (q & 3) * 2), *p1 = chunk + og_unit(row, (q & 3) * 2 + 1);
+    const og_f4 x[2] = {*reinterpret_cast<og_f4 *>(p0), *reinterpret_cast<og_f4 *>(p1)};
+    og_h4 h[2], l[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float v[4] = {ldexpf(x[e][0], -ex) * f, ldexpf(x[e][1], -ex) * f, ldexpf(x[e][2], -ex) * f, ldexpf(x[e][3], -ex) * f};
+      og_split(v, h[e], l[e]);
+    }
+    *reinterpret_cast<og_h8 *>(p0) = og_join(h);
+    *reinterpret_cast<og_h8 *>(p1) = og_join(l);
+  }
+}
+
+// the results, f32 in X, to where they belong
+template <typename T, bool MUON, bool TALL>
+__device__ __forceinline__ void og_deliver(const OrthoGroup &g, int j0, int chunks, const OrthoPtr &ptr, const char *X, float decay) {
+  const __amdgpu_buffer_rsrc_t out = og_buffer(ptr.out, g.rows * g.cols * (int)sizeof(T));
+  OgWalk<TALL> w(g, j0, chunks);
+  for (int c = 0; c < chunks; c += 2, w.next()) {
+    float old[16];
+    if constexpr (MUON)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) old[e] = og_get<float>(out, w.at(e));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float v = *reinterpret_cast<const float *>(X + w.lds(e));
+      const int o = w.at(e);
+      if constexpr (MUON) og_set(out, o, fmaf(-g.step, v, old[e] * decay));
+      else if constexpr (sizeof(T) == 4) og_set(out, o, v);
+      else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), out, o < 0 ? -1 : o * 2, 0, 0);  // the one rounding
+    }
+  }
+}
+
+// this wave's 32 x 32 tile of Y Y^T, Y = `chunks` chunks at `in`, each chunk's operands requested a chunk ahead; small cross products
+// apart from hi hi, as in ortho_product_kernel
+template <bool DIAG>
+__device__ __forceinline__ void og_square_tile(const char *in, int chunks, int ti, int tj, float (&v)[16]) {
   const int l31 = threadIdx.x & 31;
   og_f16v acc, acx;
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = acx[e] = 0.f;
-  for (int c = 0; c < chunks; ++c, in += 8192)
+  og_h8 f[2][4], g[2][4];
+  auto load = [&](int c, int b) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const og_h8 ih = og_frag(in, ti + l31, h, 0), il = og_frag(in, ti + l31, h, 1);
-      const og_h8 jh = og_frag(in, tj + l31, h, 0), jl = og_frag(in, tj + l31, h, 1);
-      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, il, acx, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, ih, acc, 0, 0, 0);
-      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jl, ih, acx, 0, 0, 0);
+    for (int h = 0; h < 4; ++h) {
+      f[b][h] = og_frag(in + c * 8192, ti + l31, h >> 1, h & 1);
+      if constexpr (!DIAG) g[b][h] = og_frag(in + c * 8192, tj + l31, h >> 1, h & 1);
     }
+  };
+  auto multiply = [&](int b) {
+#pragma unroll
+    for (int h = 0; h < 4; h += 2) {
+      const og_h8 jh = DIAG ? f[b][h] : g[b][h], jl = DIAG ? f[b][h + 1] : g[b][h + 1];
+      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, f[b][h + 1], acx, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, f[b][h], acc, 0, 0, 0);
+      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jl, f[b][h], acx, 0, 0, 0);
+    }
+  };
+  load(0, 0);
+  for (int c = 0;;) {
+    load(c + 1 < chunks ? c + 1 : c, 1);
+    multiply(0);
+    if (++c == chunks) break;
+    load(c + 1 < chunks ? c + 1 : c, 0);
+    multiply(1);
+    if (++c == chunks) break;
+  }
 #pragma unroll
   for (int e = 0; e < 16; ++e) v[e] = acc[e] + acx[e];
 }
-
-// A from the wave's tile of it (v, unscaled), then Q; barriers in front of, between and behind them
-__device__ __forceinline__ void og_make_q(char *A, char *Q, int ti, int tj, const float (&v)[16], const OrthoSmallStep &st) {
-  const int l31 = threadIdx.x & 31, lh = (threadIdx.x >> 5) & 1;
-  char *a = A + (tj >> 5) * 8192;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float w[4] = {st.gram * v[q * 4], st.gram * v[q * 4 + 1], st.gram * v[q * 4 + 2], st.gram * v[q * 4 + 3]};
-    og_put(a, ti + l31, q, w);
-  }
-  __syncthreads();
-  float p[16];
-  og_square(A, 2, ti, tj, p);
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const og_h4 eh = *reinterpret_cast<const og_h4 *>(a + og_unit(ti + l31, q * 2) + lh * 8);
-    const og_h4 el = *reinterpret_cast<const og_h4 *>(a + og_unit(ti + l31, q * 2 + 1) + lh * 8);
-    float w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w[e] = st.s0 * p[q * 4 + e] + st.s1 * ((float)eh[e] + (float)el[e]) + (ti + l31 == tj + q * 8 + lh * 4 + e ? st.diag : 0.f);
-    og_put(Q + (tj >> 5) * 8192, ti + l31, q, w);
-  }
-  __syncthreads();
+__device__ __forceinline__ void og_square(const char *in, int chunks, int ti, int tj, float (&v)[16]) {
+  if (ti == tj) og_square_tile<true>(in, chunks, ti, tj, v);
+  else og_square_tile<false>(in, chunks, ti, tj, v);
 }
 
-// Q times one chunk of 32 columns of X (transposing reads), all 64 rows: store(row, q, 4 values) gets the result.  A wave takes
-// whole chunks, so the result may go where they were read.
-template <typename F>
-__device__ __forceinline__ void og_apply(const char *Q, const char *chunk, float factor, F store) {
-  const int lane = threadIdx.x & 63, l31 = lane & 31, lh = lane >> 5;
-  og_f16v acc[2], acx[2];
-#pragma unroll
-  for (int f = 0; f < 2; ++f)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[f][e] = acx[f][e] = 0.f;
-#pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2;
-    og_h8 x[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      x[q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)chunk + og_unit(r, u + q) + (lane & 1) * 8,
-                                                  (const unsigned char *)chunk + og_unit(r + 4, u + q) + (lane & 1) * 8));
-#pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      const og_h8 ih = og_frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 0), il = og_frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, 1);
-      acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], il, acx[f], 0, 0, 0);
-      acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], ih, acc[f], 0, 0, 0);
-      acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[1], ih, acx[f], 0, 0, 0);
-    }
-  }
-#pragma unroll
-  for (int f = 0; f < 2; ++f)
+// A from the wave's tile of it (v, unscaled), then Q; a barrier in between, none behind
+__device__ __forceinline__ void og_make_q(char *A, char *Q, int tiles, int ti, int tj, float (&v)[16], const OrthoSmallStep &st) {
+  const int l31 = threadIdx.x & 31, lh = (threadIdx.x >> 5) & 1;
+  const bool mine = tiles > 1 || threadIdx.x < 64;
+  if (mine) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = factor * (acc[f][q * 4 + e] + acx[f][q * 4 + e]);
-      store(f * 32 + l31, q, v);
+      const float w[4] = {v[q * 4] *= st.gram, v[q * 4 + 1] *= st.gram, v[q * 4 + 2] *= st.gram, v[q * 4 + 3] *= st.gram};
+      og_put(A + (tj >> 5) * 8192, ti + l31, q, w);
     }
-}
-
-// 8 columns of f32 in the place of their two units, and from there into limbs
-__device__ __forceinline__ void og_place(char *chunk, int row, int q, const float (&v)[8]) {
-  *reinterpret_cast<og_f4 *>(chunk + og_unit(row, q * 2)) = og_f4{v[0], v[1], v[2], v[3]};
-  *reinterpret_cast<og_f4 *>(chunk + og_unit(row, q * 2 + 1)) = og_f4{v[4], v[5], v[6], v[7]};
-}
-__device__ __forceinline__ void og_limbs(char *chunk, int row, int q, float norm, float scale) {
-  char *p0 = chunk + og_unit(row, q * 2), *p1 = chunk + og_unit(row, q * 2 + 1);
-  const og_f4 f0 = *reinterpret_cast<og_f4 *>(p0), f1 = *reinterpret_cast<og_f4 *>(p1);
-  og_h8 h, l;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    _Float16 a, b;
-    og_split((e < 4 ? f0[e] : f1[e - 4]) / norm * scale, a, b);
-    h[e] = a;
-    l[e] = b;
   }
-  *reinterpret_cast<og_h8 *>(p0) = h;
-  *reinterpret_cast<og_h8 *>(p1) = l;
-}
-
-// sum of a workgroup's 256 values, in 64 bits
-__device__ __forceinline__ double og_block_sum(double s, double *red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
+  if (mine) {
+    float p[16];
+    og_square(A, tiles, ti, tj, p);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = fmaf(st.s0, p[q * 4 + e], fmaf(st.s1, v[q * 4 + e], ti + l31 == tj + q * 8 + lh * 4 + e ? st.diag : 0.f));
+      og_put(Q + (tj >> 5) * 8192, ti + l31, q, w);
+    }
+  }
 }
 
-template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_small_kernel(OrthoSmall c) {
-  extern __shared__ __align__(1024) char smem[];
-  __shared__ double red[4];
-  int grp;
-  const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
-  const int mat = blockIdx.x - g.first;
-  const OrthoPtr ptr = ortho_ptr(c.gs, g, mat, sizeof(T));
-  const int m = og_short(g), n = og_long(g), chunks = (n + 31) / 32, groups = chunks * 4;
-  const bool tall = g.rows > g.cols;
-  char *A = smem, *Q = smem + 16384, *X = smem + 32768;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lh = (threadIdx.x >> 5) & 1;
-  const T *src = (const T *)ptr.g;
-  double sum = 0.;
-  for (int t = threadIdx.x; t < 64 * groups; t += 256) {         // lanes run along the rows of G
-    const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
-    float v[8];
+// X <- Q X, a wave's chunks one after the other (so a result may go where the chunk was read).  Begins with a barrier, in front of
+// which the first chunk is requested (transposing reads).  `last`: f32 instead of limbs.
+template <int MT>
+__device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, float factor, bool last) {
+  const int lane = threadIdx.x & 63, l31 = lane & 31, lh = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  og_h8 x[2 * MT][2], qf[2 * MT][MT][2];
+  auto load = [&](const char *chunk) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = q * 8 + e;
-      const bool in = i < m && j < n;
-      const long o = tall ? (long)j * m + i : (long)i * n + j;
-      v[e] = in ? (float)src[o] : 0.f;
-      if constexpr (MUON) {
-        if (in) {
-          v[e] *= c.mo.gscale;
-          const float mm = fmaf(c.mo.mu, ptr.m[o], v[e]);
-          ptr.m[o] = mm;
-          v[e] = c.mo.nesterov ? fmaf(c.mo.mu, mm, v[e]) : mm;
-        }
-      }
-      sum += (double)v[e] * (double)v[e];
+    for (int h = 0; h < 2 * MT; ++h) {
+      const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        x[h][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)chunk + og_unit(r, u + q) + (lane & 1) * 8,
+                                                       (const unsigned char *)chunk + og_unit(r + 4, u + q) + (lane & 1) * 8));
     }
-    og_place(X + (q >> 2) * 8192, i, q & 3, v);
+  };
+  if (wave < chunks) load(X + wave * 8192);
+  __syncthreads();
+  if (wave >= chunks) return;
+#pragma unroll
+  for (int h = 0; h < 2 * MT; ++h)
+#pragma unroll
+    for (int f = 0; f < MT; ++f)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) qf[h][f][q] = og_frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, q);
+  for (int ch = wave; ch < chunks; ch += 4) {
+    char *chunk = X + ch * 8192;
+    og_f16v acc[MT], acx[MT];
+#pragma unroll
+    for (int f = 0; f < MT; ++f)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[f][e] = acx[f][e] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2 * MT; ++h)
+#pragma unroll
+      for (int f = 0; f < MT; ++f) {
+        acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][0], qf[h][f][1], acx[f], 0, 0, 0);
+        acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][0], qf[h][f][0], acc[f], 0, 0, 0);
+        acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][1], qf[h][f][0], acx[f], 0, 0, 0);
+      }
+    if (ch + 4 < chunks) load(chunk + 4 * 8192);
+#pragma unroll
+    for (int f = 0; f < MT; ++f)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[f][e] = factor * (acc[f][e] + acx[f][e]);
+    auto each = [&](auto store) {
+#pragma unroll
+      for (int f = 0; f < MT; ++f)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float v[4] = {acc[f][q * 4], acc[f][q * 4 + 1], acc[f][q * 4 + 2], acc[f][q * 4 + 3]};
+          store(f * 32 + l31, q, v);
+        }
+    };
+    if (last)
+      each([&](int i, int q, const float(&v)[4]) { *reinterpret_cast<og_f4 *>(chunk + og_unit(i, q * 2 + lh)) = og_f4{v[0], v[1], v[2], v[3]}; });
+    else
+      each([&](int i, int q, const float(&v)[4]) { og_put(chunk, i, q, v); });
   }
-  const float norm = (float)(sqrt(og_block_sum(sum, red)) + (double)c.eps);
-  for (int t = threadIdx.x; t < 64 * groups; t += 256) {         // every thread turns what it placed into limbs
-    const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
-    og_limbs(X + (q >> 2) * 8192, i, q & 3, norm, c.x0);
-  }
-  const int ti = (wave >> 1) * 32, tj = (wave & 1) * 32;         // this wave's tile of A and Q
+}
+
+// sum over 256 threads, the same in all of them; a barrier inside
+template <int CTRL>
+__device__ __forceinline__ double og_dpp(double v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, 0xf, 0xf, true);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xf, 0xf, true);
+  return v + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double og_block_sum(double s, double *red) {
+  s = og_dpp<0xB1>(s);           // lane ^ 1, lane ^ 2, mirrored in 8, in 16
+  s = og_dpp<0x4E>(s);
+  s = og_dpp<0x141>(s);
+  s = og_dpp<0x140>(s);
+  if ((threadIdx.x & 15) == 0) red[threadIdx.x >> 4] = s;
+  __syncthreads();
+  double t = 0.;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t += red[i];
+  return t;
+}
+
+template <typename T, bool MUON, int MT>
+__device__ __forceinline__ void ortho_alone(const OrthoSmall &c, const OrthoGroup &g, const OrthoPtr &ptr, char *smem, double *red) {
+  const int chunks = (og_long(g) + 31) / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char *A = smem, *Q = smem + 16384, *X = smem + 32768;
+  const bool tall = g.rows > g.cols;
+  const double sum = tall ? og_fetch<T, MUON, true>(g, 0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false>(g, 0, chunks, ptr, c.mo, X);
+  og_limbs<MT>(X, chunks, sqrt(og_block_sum(sum, red)) + (double)c.eps, c.x0);
+  const int ti = MT > 1 ? (wave >> 1) * 32 : 0, tj = MT > 1 ? (wave & 1) * 32 : 0;          // this wave's tile of A and Q
   for (int k = 0; k < c.steps; ++k) {
     const OrthoSmallStep st = c.step[k];
     float v[16];
     __syncthreads();
-    og_square(X, chunks, ti, tj, v);
-    og_make_q(A, Q, ti, tj, v, st);
-    for (int ch = wave; ch < chunks; ch += 4) {
-      char *chunk = X + ch * 8192;
-      og_apply(Q, chunk, st.x, [&](int i, int q, const float (&w)[4]) {
-        if (k + 1 < c.steps) {
-          og_put(chunk, i, q, w);
-        } else if (i < m) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = ch * 32 + q * 8 + lh * 4 + e;
-            if (j < n) og_result(ptr.out, tall ? (long)j * m + i : (long)i * n + j, w[e], c.mode, g.step, c.decay);
-          }
-        }
-      });
-    }
+    if (MT > 1 || wave == 0) og_square(X, chunks, ti, tj, v);
+    og_make_q(A, Q, MT, ti, tj, v, st);
+    og_apply<MT>(Q, X, chunks, st.x, k + 1 == c.steps);
   }
+  __syncthreads();
+  if (tall) og_deliver<T, MUON, true>(g, 0, chunks, ptr, X, c.decay);
+  else og_deliver<T, MUON, false>(g, 0, chunks, ptr, X, c.decay);
+}
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256, 2) void ortho_small_kernel(OrthoSmall c) {
+  extern __shared__ __align__(1024) char smem[];
+  __shared__ double red[16];
+  int grp;
+  const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
+  const OrthoPtr ptr = ortho_ptr(c.gs, g, blockIdx.x - g.first, sizeof(T));
+  if (og_short(g) <= 32) ortho_alone<T, MUON, 1>(c, g, ptr, smem, red);
+  else ortho_alone<T, MUON, 2>(c, g, ptr, smem, red);
 }
 
 __host__ __device__ static inline int og_panels(const OrthoGroup &g) { return ((og_long(g) + 31) / 32 + g.jobs - 1) / g.jobs; }
 
 // Launch k of a chain of panels: k = 0 forms X0's panel and its share of the first Gram matrix, launch k > 0 takes step k - 1.  X's
 // panels lie in the workspace as they lie in LDS; the shares (f32, as the MFMAs leave them) go to one of two sets in turn, since
-// other workgroups may still read the last launch's.
-template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ortho_panel_kernel(OrthoSmall c, char *__restrict__ ws, const double *__restrict__ sums, int k) {
-  extern __shared__ __align__(1024) char smem[];
-  __shared__ double red[4];
-  int grp;
-  const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
+// other workgroups may still read the last launch's.  Launch 0 knows only its own panel's norm and divides by that; launch 1 knows
+// all of them and puts it right: a panel's share counts (its norm / the matrix' norm)^2 times, its result their quotient times.
+template <typename T, bool MUON, int MT>
+__device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGroup &g, char *ws, double *sums, int k, char *smem, double *red) {
   const int panels = og_panels(g), wide = g.jobs, mat = og_div(blockIdx.x - g.first, panels), pan = blockIdx.x - g.first - mat * panels;
-  const int m = og_short(g), n = og_long(g), all = (n + 31) / 32, chunks = all - pan * wide < wide ? all - pan * wide : wide;
-  const bool tall = g.rows > g.cols;
+  const int all = (og_long(g) + 31) / 32, chunks = all - pan * wide < wide ? all - pan * wide : wide;
   char *A = smem, *Q = smem + 16384, *X = smem + 32768;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lh = (threadIdx.x >> 5) & 1;
-  const int ti = (wave >> 1) * 32, tj = (wave & 1) * 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ti = MT > 1 ? (wave >> 1) * 32 : 0, tj = MT > 1 ? (wave & 1) * 32 : 0;
+  const bool square = MT > 1 || wave == 0;
   const OrthoPtr ptr = ortho_ptr(c.gs, g, mat, sizeof(T));
+  const bool tall = g.rows > g.cols;
+  const int j0 = pan * wide * 32;
   char *mine = ws + (size_t)g.x_off * 256 + ((size_t)mat * all + pan * wide) * 8192;
   og_f4 *share = reinterpret_cast<og_f4 *>(ws + (size_t)g.p_off * 256);                       // [set][mat][panel][q][thread]
   const size_t set = (size_t)g.count * panels * 1024;
-  if (k == 0) {
-    const int nb = og_norm_blocks(g);
-    double s = 0.;
-    for (int i = threadIdx.x; i < nb; i += 256) s += sums[g.aux + (long)mat * nb + i];
-    const float norm = (float)(sqrt(og_block_sum(s, red)) + (double)c.eps);
-    const T *src = (const T *)ptr.g;
-    const int groups = chunks * 4;
-    for (int t = threadIdx.x; t < 64 * groups; t += 256) {       // lanes run along the rows of G
-      const int i = tall ? t & 63 : t / groups, q = tall ? t >> 6 : t - i * groups;
-      float v[8];
+  float v[16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = pan * wide * 32 + q * 8 + e;
-        const bool in = i < m && j < n;
-        const long o = tall ? (long)j * m + i : (long)i * n + j;
-        v[e] = in ? (float)src[o] : 0.f;
-        if constexpr (MUON)
-          if (in) v[e] = c.mo.nesterov ? fmaf(c.mo.mu, ptr.m[o], v[e] * c.mo.gscale) : ptr.m[o];
-      }
-      og_place(X + (q >> 2) * 8192, i, q & 3, v);
-      og_limbs(X + (q >> 2) * 8192, i, q & 3, norm, c.x0);
-    }
+  for (int e = 0; e < 16; ++e) v[e] = 0.f;
+  if (k == 0) {
+    const double part = tall ? og_fetch<T, MUON, true>(g, j0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false>(g, j0, chunks, ptr, c.mo, X);
+    const double sum = og_block_sum(part, red);
+    if (threadIdx.x == 0) sums[blockIdx.x] = sum;
+    og_limbs<MT>(X, chunks, sum == 0. ? 1. : sqrt(sum), c.x0);
   } else {
     for (int t = threadIdx.x; t < chunks * 512; t += 256)
       reinterpret_cast<og_h8 *>(X)[t] = reinterpret_cast<const og_h8 *>(mine)[t];
     const OrthoSmallStep st = c.step[k - 1];
     const og_f4 *p = share + ((k - 1) & 1) * set + (size_t)mat * panels * 1024 + threadIdx.x;
-    float v[16];
+    float own = 1.f;
+    float *weight = reinterpret_cast<float *>(red + 16);
+    if (k == 1) {
+      const int lane = threadIdx.x & 63;
+      const double part = lane < panels ? sums[blockIdx.x - pan + lane] : 0.;
+      double norm = part;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = 0.f;
-#pragma unroll 4
-    for (int z = 0; z < panels; ++z, p += 1024)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const og_f4 w = p[q * 256];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[q * 4 + e] += w[e];
-      }
-    og_make_q(A, Q, ti, tj, v, st);
-    for (int ch = wave; ch < chunks; ch += 4) {
-      char *chunk = X + ch * 8192;
-      og_apply(Q, chunk, st.x, [&](int i, int q, const float (&w)[4]) {
-        if (k < c.steps) {
-          og_put(chunk, i, q, w);
-        } else if (i < m) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = (pan * wide + ch) * 32 + q * 8 + lh * 4 + e;
-            if (j < n) og_result(ptr.out, tall ? (long)j * m + i : (long)i * n + j, w[e], c.mode, g.step, c.decay);
-          }
-        }
-      });
+      for (int o = 32; o > 0; o >>= 1) norm += __shfl_xor(norm, o, 64);
+      norm = sqrt(norm) + (double)c.eps;
+      const float quotient = (float)(sqrt(part) / norm);
+      own = __shfl(quotient, pan, 64);
+      if (lane < panels) weight[lane] = quotient * quotient;     // (every wave the same)
     }
-    if (k == c.steps) return;
+    auto gather = [&](auto part) {
+#pragma unroll 4
+      for (int z = 0; z < panels; ++z, p += 1024) {
+        const float share = part(z);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const og_f4 s = p[q * 256];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[q * 4 + e] = fmaf(s[e], share, v[q * 4 + e]);
+        }
+      }
+    };
+    if (square && k == 1) gather([&](int z) { return weight[z]; });
+    else if (square) gather([](int) { return 1.f; });
+    og_make_q(A, Q, MT, ti, tj, v, st);
+    og_apply<MT>(Q, X, chunks, st.x * own, k == c.steps);
   }
   __syncthreads();
-  float v[16];
-  og_square(X, chunks, ti, tj, v);
-  og_f4 *o = share + (k & 1) * set + ((size_t)mat * panels + pan) * 1024 + threadIdx.x;
+  if (k == c.steps) {
+    if (tall) og_deliver<T, MUON, true>(g, j0, chunks, ptr, X, c.decay);
+    else og_deliver<T, MUON, false>(g, j0, chunks, ptr, X, c.decay);
+    return;
+  }
+  if (square) {
+    og_square(X, chunks, ti, tj, v);
+    og_f4 *o = share + (k & 1) * set + ((size_t)mat * panels + pan) * 1024 + threadIdx.x;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) o[q * 256] = og_f4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
+    for (int q = 0; q < 4; ++q) o[q * 256] = og_f4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
+  }
   for (int t = threadIdx.x; t < chunks * 512; t += 256) reinterpret_cast<og_h8 *>(mine)[t] = reinterpret_cast<const og_h8 *>(X)[t];
+}
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256, 2) void ortho_panel_kernel(OrthoSmall c, char *__restrict__ ws, double *__restrict__ sums, int k) {
+  extern __shared__ __align__(1024) char smem[];
+  __shared__ double red[16 + ORTHO_PANELS / 2];
+  int grp;
+  const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
+  if (og_short(g) <= 32) ortho_panel<T, MUON, 1>(c, g, ws, sums, k, smem, red);
+  else ortho_panel<T, MUON, 2>(c, g, ws, sums, k, smem, red);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -1119,17 +1247,14 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
     lo.panels = lo.panels && og_short(g[i]) <= ORTHO_SMALL_M;
   }
   size_t at = lo.sums + align_up(lo.norm_blocks * sizeof(double), 256);
-  lo.small = lo.panels && most <= ORTHO_ALONE_N;
-  if (lo.panels && !lo.small) {
-    lo.panels = ortho_panel_chunks(g, n);
-    lo.small = !lo.panels && most <= ORTHO_SMALL_N;
-  }
+  lo.small = lo.panels && most <= ORTHO_SMALL_N;
+  lo.panels = lo.panels && !lo.small && ortho_panel_chunks(g, n);
   if (lo.small) {
-    lo.panels = false;
     lo.bytes = lo.sums;
     return lo;
   }
-  if (lo.panels) {                                                       // X | two sets of the panels' shares
+  if (lo.panels) {                                                       // the panels' sums of squares | X | two sets of their shares
+    at = lo.sums + 256 * sizeof(double);
     for (int i = 0; i < n; ++i) {
       g[i].x_off = (unsigned)(at / 256);
       at += (size_t)g[i].count * ((og_long(g[i]) + 31) / 32) * 8192;
@@ -1216,7 +1341,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
       const OrthoJob *a = plan[0].level[3 * k].job, *q = plan[0].level[3 * k + 1].job, *x = plan[0].level[3 * k + 2].job;
       sm.step[k] = OrthoSmallStep{a->k0, q->k0, q->k1, q->diag, x->k0};
     }
-    const int lds = 32768 + most * 8192;
+    const int lds = 32768 + (most + 1) / 2 * 16384;                      // (og_fetch's padding: an even number of chunks)
 #define ORTHO_SMALL(T, MUON)                                                                                                            \
   do {                                                                                                                                  \
     const void *fn = lo.small ? reinterpret_cast<const void *>(&ortho_small_kernel<T, MUON>) : reinterpret_cast<const void *>(&ortho_panel_kernel<T, MUON>); \
@@ -1224,7 +1349,6 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     if (lo.small) {                                                                                                                     \
       hipLaunchKernelGGL((ortho_small_kernel<T, MUON>), dim3(blocks), dim3(256), lds, st, sm);                                          \
     } else {                                                                                                                            \
-      hipLaunchKernelGGL((ortho_norm_kernel<T, MUON>), dim3(lo.norm_blocks), dim3(256), 0, st, lv.gs, sums, c.mo);                      \
       for (int k = 0; k <= c.steps; ++k)                                                                                                \
         hipLaunchKernelGGL((ortho_panel_kernel<T, MUON>), dim3(blocks), dim3(256), lds, st, sm, ws, sums, k);                           \
     }                                                                                                                                   \
