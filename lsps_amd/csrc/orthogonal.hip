@@ -631,14 +631,18 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
 
 // ---- short sides of up to 64 ---------------------------------------------------------------------------------------------
 // A, Q and up to 448 columns of X fit into LDS as limbs (16 + 16 + 112 KB), so one workgroup can take a step's products one after the
-// other with a barrier between them; as launches they cost 5 us each at these sizes.  Short matrices run their whole iteration in one
-// workgroup (ortho_small_kernel).  Longer ones are cut into panels of columns, one workgroup each: a launch per step adds the panels'
-// shares of the Gram matrix up (every workgroup for itself, in a fixed order), forms Q, multiplies its panel by it and leaves the
-// panel's share of the next Gram matrix (ortho_panel_kernel).  Five steps, whole iteration / panels / the products as launches, us:
-//   64 x 128  34 / 58 / -     64 x 256  53 / 61 / -     64 x 448  85 / 64 / 112     8 of 33 x 1000  - / 71 / 128
-//   64 x 4096 - / 93 / 142    20 x 8192 - / 111 / 152   40 of 64 x 576 - / 85 / 126   80 of 64 x 576 - / 104 / 147
-// Past one workgroup per CU panels lose (400 of 64 x 576: 440, 308 as launches).  Panels of 1 or 2 chunks are as fast for one matrix and
-// slower for several (8 of 33 x 1000: 93, 79); 16 panels at most instead of 32 cost 20 x 8192 155 us, 64 cost 64 x 4096 116.
+// other with a barrier between them; as launches they cost 5 us each at these sizes.  Matrices of up to 448 columns run their whole
+// iteration in one workgroup (ortho_small_kernel).  Longer ones are cut into panels of columns, one workgroup each: a launch per step
+// adds the panels' shares of the Gram matrix up (every workgroup for itself, in a fixed order), forms Q, multiplies its panel by it and
+// leaves the panel's share of the next Gram matrix (ortho_panel_kernel).  A step of 108 x 50 takes 2.8 us: 0.7 for the Gram matrix, 0.8
+// for A A and Q, 1.2 for Q X; of them 24 + 12 + 24 MFMAs of 33 cycles 0.8, the LDS reads at 128 bytes a cycle 0.5, the conversions 0.6,
+// one after the other with a single wave per SIMD.
+// Five steps, panels / the products as launches, us (one workgroup: 50 x 108 20, 64 x 256 31, 64 x 448 47):
+//   64 x 449  51 / 113     8 of 33 x 1000  59 / 127     100 of 64 x 576  93 / 150     64 x 4096   79 / 142    16 of 64 x 8192 221 / 246
+//   20 x 8192 86 / 152    40 of 64 x 576  69 / 126      256 of 64 x 576 183 / 229     64 x 14336 121 / 171    30 of 64 x 4096 204 / 224
+// Past two workgroups per CU their shares of the Gram matrices cost more than they save (1000 of 20 x 1500: 2140, 1700 as launches).
+// Panels of 1 or 2 chunks are as fast for one matrix and slower for several; 16 panels at most instead of 32 cost 20 x 8192 a third, 64
+// cost 64 x 4096 a quarter.
 #define ORTHO_SMALL_M 64
 #define ORTHO_SMALL_N 448      // columns that fit into LDS
 #define ORTHO_WIDE 4           // narrowest panel, in chunks of 32 columns
@@ -1216,18 +1220,19 @@ struct OrthoLayout {
   int norm_blocks, split_blocks;
 };
 
-// Widths of the panels (g[i].jobs): the smallest from ORTHO_WIDE chunks on that leaves no matrix more than ORTHO_PANELS
-// panels and the pass no more workgroups than CUs.  False if none does.
+// Widths of the panels (g[i].jobs): the smallest from ORTHO_WIDE chunks on that leaves the pass no more workgroups than CUs, or else
+// than twice as many (two fit on a CU), and no matrix more than ORTHO_PANELS panels.  False if there is none.
 static bool ortho_panel_chunks(OrthoGroup *g, int n) {
-  for (int w = ORTHO_WIDE; w <= ORTHO_SMALL_N / 32; ++w) {
-    long blocks = 0, most = 0;
-    for (int i = 0; i < n; ++i) {
-      g[i].jobs = w;
-      blocks += (long)g[i].count * og_panels(g[i]);
-      if (og_panels(g[i]) > most) most = og_panels(g[i]);
+  for (long limit : {256L, 512L})
+    for (int w = ORTHO_WIDE; w <= ORTHO_SMALL_N / 32; ++w) {
+      long blocks = 0, most = 0;
+      for (int i = 0; i < n; ++i) {
+        g[i].jobs = w;
+        blocks += (long)g[i].count * og_panels(g[i]);
+        if (og_panels(g[i]) > most) most = og_panels(g[i]);
+      }
+      if (blocks <= limit && most <= ORTHO_PANELS) return true;
     }
-    if (blocks <= 256 && most <= ORTHO_PANELS) return true;
-  }
   return false;
 }
 
@@ -1254,7 +1259,9 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
     return lo;
   }
   if (lo.panels) {                                                       // the panels' sums of squares | X | two sets of their shares
-    at = lo.sums + 256 * sizeof(double);
+    long blocks = 0;
+    for (int i = 0; i < n; ++i) blocks += (long)g[i].count * og_panels(g[i]);
+    at = lo.sums + align_up(blocks * sizeof(double), 256);
     for (int i = 0; i < n; ++i) {
       g[i].x_off = (unsigned)(at / 256);
       at += (size_t)g[i].count * ((og_long(g[i]) + 31) / 32) * 8192;

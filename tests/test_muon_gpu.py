@@ -49,7 +49,7 @@ SHAPES = [(1, 1, 1), (2, 1, 9), (2, 9, 1), (1, 2, 3), (3, 20, 50), (1, 50, 108),
           (2, 130, 65), (5, 100, 333), (1, 333, 1021), (2, 256, 256), (1, 257, 700), (1, 20, 8192), (3, 8192, 20), (70, 33, 40), (1, 512, 513),
           (3, 64, 448), (2, 449, 64), (2, 448, 30), (300, 5, 31),
           # short sides of up to 64: panels of several widths, the last one narrow, and too many of them for panels
-          (2, 64, 257), (2, 64, 449), (3, 50, 1000), (2, 9000, 33), (1, 1, 14336), (2, 3, 14337), (40, 64, 576), (70, 64, 448),
+          (2, 64, 257), (2, 64, 449), (3, 50, 1000), (2, 9000, 33), (1, 1, 14336), (2, 3, 14337), (40, 64, 576), (150, 40, 600), (70, 64, 448),
           (300, 40, 300), (90, 20, 700),
           (40, 192, 200), (1, 1024, 1100), (20, 448, 1000),
           # 128 x 128 tiles with odd 64-row halves, symmetric and not; chains of two and three
