@@ -1792,26 +1792,33 @@ class _LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, stats = ctx.saved_tensors
-        cols, rows = ctx.cols, stats.shape[1]
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = dy.new_empty(dy.shape) if need_x else None
-        alloc = stats.new_empty if rows else stats.new_zeros
-        dw = alloc(w.shape) if need_w else None
-        db = alloc(ctx.bshape) if need_b else None
-        if rows:
-            L = _lib.lib()
-            dt = _DTYPES[x.dtype]
-            xr, ldx = _rows(x, rows, cols)
-            gr, ldg = _rows(dy, rows, cols)
-            buf, ws, n = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x)
-            sp = stats.data_ptr()
-            _launch('layernorm_bwd', x.get_device(), L.lsps_layernorm_bwd, gr.data_ptr(), xr.data_ptr(), sp, sp + 4 * rows,
-                    None if w is None else w.data_ptr(), dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
-                    db.data_ptr() if need_b else None, rows, cols, ldx, ldg, dt, ws, n)
-        return dx, dw, db, None, None, None
+        # once_differentiable's wrapper costs 2 - 4 us: only for a backward pass that is itself recorded
+        return (_layer_norm_backward_once if torch.is_grad_enabled() else _layer_norm_backward)(ctx, dy)
+
+
+def _layer_norm_backward(ctx, dy):
+    x, w, stats = ctx.saved_tensors
+    cols, rows = ctx.cols, stats.shape[1]
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dx = dy.new_empty(dy.shape) if need_x else None
+    alloc = stats.new_empty if rows else stats.new_zeros
+    dw = alloc(w.shape) if need_w else None
+    db = alloc(ctx.bshape) if need_b else None
+    if rows:
+        L = _lib.lib()
+        dt = _DTYPES[x.dtype]
+        xr, ldx = _rows(x, rows, cols)
+        gr, ldg = _rows(dy, rows, cols)
+        buf, ws, n = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x)
+        sp = stats.data_ptr()
+        _launch('layernorm_bwd', x.get_device(), L.lsps_layernorm_bwd, gr.data_ptr(), xr.data_ptr(), sp, sp + 4 * rows,
+                None if w is None else w.data_ptr(), dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                db.data_ptr() if need_b else None, rows, cols, ldx, ldg, dt, ws, n)
+    return dx, dw, db, None, None, None
+
+
+_layer_norm_backward_once = torch.autograd.function.once_differentiable(_layer_norm_backward)
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
