@@ -1848,6 +1848,14 @@ def _coeffs(coeffs):
     return a, b, c
 
 
+def _ints(what, *values):
+    """The values as C ints (ctypes would wrap them round without a word)."""
+    values = tuple(int(v) for v in values)
+    if any(v != _ctypes.c_int(v).value for v in values):
+        raise _lib.LspsHipError("%s: %s do not fit 32 bits" % (what, values))
+    return values
+
+
 def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """Newton-Schulz iterate of the matrices [..., rows, cols] of `g` (float32 or bfloat16; the same type comes back): singular vectors
     kept, singular values driven towards 1 (csrc/orthogonal.hip).  X = G / (|G|_F + eps), then `steps` times
@@ -1866,9 +1874,9 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         L = _lib.lib()
         g = _c(g)
         rows, cols = g.shape[-2:]
-        count = g.numel() // (rows * cols)
-        buf, ws, n = _scratch(L.lsps_newton_schulz_workspace_bytes(count, rows, cols, int(steps)), g)
-        _launch('newton_schulz', index, L.lsps_newton_schulz, g.data_ptr(), out.data_ptr(), count, rows, cols, _DTYPES[g.dtype], int(steps),
+        count, rows, cols, steps = _ints('newton_schulz', g.numel() // (rows * cols), rows, cols, steps)
+        buf, ws, n = _scratch(L.lsps_newton_schulz_workspace_bytes(count, rows, cols, steps), g)
+        _launch('newton_schulz', index, L.lsps_newton_schulz, g.data_ptr(), out.data_ptr(), count, rows, cols, _DTYPES[g.dtype], steps,
                 *_coeffs(coeffs), float(eps), ws, n)
     return out
 
@@ -1906,11 +1914,12 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     index = _same_device('muon_step_', params[0], *(params + grads + momenta))
     mats = (_lib.LspsMuonMatrix * len(params))()
     for k, (p, g, m) in enumerate(zip(params, grads, momenta)):
-        mats[k] = _lib.LspsMuonMatrix(_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), p.shape[0], p.numel() // p.shape[0])
+        mats[k] = _lib.LspsMuonMatrix(_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), *_ints('muon_step_', p.shape[0], p.numel() // p.shape[0]))
     _disjoint('muon_step_', params + momenta, grads)
-    buf, ws, n = _scratch(L.lsps_muon_workspace_bytes(mats, len(params), int(steps)), params[0])
+    steps, = _ints('muon_step_', steps)
+    buf, ws, n = _scratch(L.lsps_muon_workspace_bytes(mats, len(params), steps), params[0])
     _launch('muon_step', index, L.lsps_muon_step, mats, len(params), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
-            float(rms), float(grad_scale), int(steps), *_coeffs(coeffs), float(eps), ws, n)
+            float(rms), float(grad_scale), steps, *_coeffs(coeffs), float(eps), ws, n)
     torch.autograd.graph.increment_version(params + momenta)       # written behind torch's back
 
 

@@ -89,7 +89,7 @@ def test_converges_to_the_orthogonal_factor():
     assert float((out - u @ v.T).norm()) <= 16 * 2.0 ** -22 * 40 ** 0.5 * 4
 
 
-@pytest.mark.parametrize('rows,cols', [(48, 100), (300, 170)])
+@pytest.mark.parametrize('rows,cols', [(48, 100), (300, 170), (20, 30), (48, 700), (900, 20)])
 def test_zero_tiny_huge_low_rank_and_bad_matrices(rows, cols):
     """One bad matrix of a stack leaves the others alone; sizes at the ends of f32 neither overflow nor vanish."""
     from lsps_amd import ops
@@ -192,7 +192,8 @@ def test_streams_and_graphs():
             ops.muon_step_(p, gs, m, lr=0.1)
         return p + m
     want = [run(n) for n in (1, 2, 3)]
-    ns = ops.newton_schulz(gs[1])
+    wide = grads(3, 40, 1000)
+    ns, nw = ops.newton_schulz(gs[1]), ops.newton_schulz(wide)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
@@ -205,13 +206,46 @@ def test_streams_and_graphs():
         ops.muon_step_(p, gs, m, lr=0.1)
     with torch.cuda.graph(g2):
         out = ops.newton_schulz(gs[1])
+        out_wide = ops.newton_schulz(wide)
     for k in range(3):
         out.zero_()
+        out_wide.zero_()
         g1.replay()
         g2.replay()
         run(1)
         torch.cuda.synchronize()
-        assert all(torch.equal(a, b) for a, b in zip(p + m, want[k])) and torch.equal(out, ns)
+        assert all(torch.equal(a, b) for a, b in zip(p + m, want[k])) and torch.equal(out, ns) and torch.equal(out_wide, nw)
+
+
+def test_two_threads_at_once():
+    """Two host threads, each with a stream and matrices of its own: the same bits as one after the other."""
+    import threading
+
+    from lsps_amd import ops
+    work = [[grads(1, *s, seed=k)[0] for s in ((60, 90), (130, 200), (40, 1000))[k:] + ((300, 320),)] for k in range(2)]
+
+    def run(gs):
+        p, m = [torch.full_like(g, 0.5) for g in gs], [torch.zeros_like(g) for g in gs]
+        for _ in range(8):
+            ops.muon_step_(p, gs, m, lr=0.1)
+            x = ops.layer_norm(p[0], p[0].shape[-1])
+        return p + m + [x, ops.newton_schulz(gs[-1])]
+    want = [run(gs) for gs in work]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def thread(k):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got[k] = run(work[k])
+        s.synchronize()
+    threads = [threading.Thread(target=thread, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert all(g is not None and all(torch.equal(a, b) for a, b in zip(g, w)) for g, w in zip(got, want))
+
 
 
 def test_beyond_32_bits():

@@ -26,6 +26,10 @@ def test_refusals_of_the_python_entry_points():
         with pytest.raises(_lib.LspsHipError):
             bad()
     assert ops.muon_step_([], [], [], lr=0.1) is None
+    assert ops._ints('t', 5, (1 << 31) - 1, -3) == (5, (1 << 31) - 1, -3)
+    for n in (1 << 31, (1 << 32) + 5, -(1 << 31) - 1):                        # a C int would be another size
+        with pytest.raises(_lib.LspsHipError):
+            ops._ints('t', 2, n)
 
 
 def test_overlapping_tensors_are_refused():
