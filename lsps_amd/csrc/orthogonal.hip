@@ -43,6 +43,7 @@ typedef float og_f4 __attribute__((ext_vector_type(4)));
 typedef float og_f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short og_u4u __attribute__((ext_vector_type(4), aligned(2)));
 
+#define OG_BAND 512            // columns of a band of tiles of a symmetric product
 #define ORTHO_GROUPS 16        // shapes per pass (they travel in the kernels' arguments)
 #define ORTHO_MATRICES 1024    // matrices with pointers of their own per pass
 #define ORTHO_CHAINS 3         // longest chain: steps between two Gram matrices of the long side
@@ -295,6 +296,14 @@ __device__ __forceinline__ int og_div(int a, int b) {
   return __builtin_amdgcn_readfirstlane(q);
 }
 
+// the largest j with j (j + 1) / 2 <= t
+__device__ __forceinline__ int og_triangle(int t) {
+  int j = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+  while ((j + 1) * (j + 2) / 2 <= t) ++j;
+  while (j * (j + 1) / 2 > t) --j;
+  return j;
+}
+
 struct OgTrue {
   static constexpr bool value = true;
 };
@@ -324,7 +333,7 @@ struct OrthoLevel {
 // A product with few tiles and a long reduction is split into kz ranges of it: f32 partial tiles in the workspace, added in a
 // fixed order by a second launch of this kernel.
 template <int T, int KC, int S, int WI, int WJ>
-__global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
+__global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
   constexpr int WAVES = WI * WJ, SUB = KC / 32, STAGE = T * KC * 4, PIECES = T * SUB / 8 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = 144;
   static_assert(S * 2 * STAGE >= WAVES * 32 * TP, "the exchange buffers of the epilogue lie in the stages");
   static_assert((S - 1) * 2 * PIECES < 64, "the range of s_waitcnt vmcnt");
@@ -344,10 +353,20 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
   const int u1 = unit0 - second * per * g.count, mat = og_div(u1, per), u2 = u1 - mat * per, tile = og_div(u2, kz), z = u2 - tile * kz;
   int bi, bj;
   if (type == OL_SYM) {
-    bj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-    while ((bj + 1) * (bj + 2) / 2 <= tile) ++bj;
-    while (bj * (bj + 1) / 2 > tile) --bj;
-    bi = tile - bj * (bj + 1) / 2;
+    // bands of W column tiles, in each row by row down to its triangle on the diagonal: an XCD's tiles make a block of about W x W
+    constexpr int W = OG_BAND / T;
+    const int m = (M + T - 1) / T;
+    int b = og_triangle(tile) & -W, t = tile - b * (b + 1) / 2;  // the band's first column (the tiles in front of it make a triangle too)
+    const int w = m - b < W ? m - b : W;
+    if (t < b * w) {
+      bi = og_div(t, w);
+      bj = b + t - bi * w;
+    } else {
+      t -= b * w;
+      bj = og_triangle(t);
+      bi = b + t - bj * (bj + 1) / 2;
+      bj += b;
+    }
   } else {
     const int tm = (M + T - 1) / T;                              // the row tiles of one column panel one after the other
     bj = og_div(tile, tm);
@@ -416,32 +435,40 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
       }
     };
     // Fragments are read from LDS one half chunk ahead of their MFMAs, across the barrier too: the barrier of chunk c comes when its
-    // last fragments are in registers, so its stage is free for chunk c + S, and chunk c + 1 has landed
+    // last fragments are in registers, so its stage is free for chunk c + S, and chunk c + 1 has landed.  The chunks go round the
+    // stages in a loop unrolled S times, so that a lane's LDS addresses are eight registers and constants, and the last chunk has code
+    // of its own: where paths meet, the compiler would wait for every LDS read in flight.
     static_assert(KC == 32, "two halves per chunk");
     og_h8 lf[2][FI][2], rf[2][FJ][2];
     auto product = [&](auto turn) {
-      auto load = [&](int h, const char *sl) {
-        const char *sr = sl + STAGE;
-        const int kg = h * 2 + lh;
+      // lines of 32 columns: halves and limbs differ in bits of the unit; chunks of X: lane i of 16 points at 4 columns of row i / 4 and
+      // receives 4 rows of column i, the other 4 rows lie 512 bytes on
+      const char *la[2][2], *ra[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int unit = h * 4 + lh * 2 + q, li = wi * FI * 32 + l31, rj = wj * FJ * 32 + l31;
+          la[h][q] = smem + li * 128 + ((unit ^ ((li >> 1) & 7)) * 16);
+          if constexpr (!turn.value) {
+            ra[h][q] = smem + STAGE + rj * 128 + ((unit ^ ((rj >> 1) & 7)) * 16);
+          } else {                                               // [4 rows further][limb]
+            const int r = lh * 8 + ((lane & 15) >> 2) + h * 4, u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2 + q;
+            ra[h][q] = smem + STAGE + (wj * FJ * KC + r) * 128 + (lane & 1) * 8 + ((u ^ ((r >> 1) & 7)) * 16);
+          }
+        }
+      auto load = [&](int h, int at) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
           for (int f = 0; f < FJ; ++f)
-            if constexpr (!turn.value) {
-              const int rj = (wj * FJ + f) * 32 + l31;
-              rf[h][f][q] = *reinterpret_cast<const og_h8 *>(sr + rj * 128 + (((kg * 2 + q) ^ ((rj >> 1) & 7)) * 16));
-            } else {
-              // lane i of 16 points at 4 columns of row i / 4 and receives 4 rows of column i
-              const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2 + q;
-              const char *at = sr + ((wj * FJ + f) * KC + r) * 128 + (lane & 1) * 8;
-              rf[h][f][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)at + ((u ^ ((r >> 1) & 7)) * 16),
-                                                                 (const unsigned char *)at + 512 + ((u ^ (((r + 4) >> 1) & 7)) * 16)));
-            }
+            if constexpr (!turn.value)
+              rf[h][f][q] = *reinterpret_cast<const og_h8 *>(ra[h][q] + at * 2 * STAGE + f * 4096);
+            else
+              rf[h][f][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)ra[0][q] + at * 2 * STAGE + f * KC * 128 + h * 2048,
+                                                                 (const unsigned char *)ra[1][q] + at * 2 * STAGE + f * KC * 128 + h * 2048));
 #pragma unroll
-          for (int f = 0; f < FI; ++f) {
-            const int li = (wi * FI + f) * 32 + l31;
-            lf[h][f][q] = *reinterpret_cast<const og_h8 *>(sl + li * 128 + (((kg * 2 + q) ^ ((li >> 1) & 7)) * 16));
-          }
+          for (int f = 0; f < FI; ++f) lf[h][f][q] = *reinterpret_cast<const og_h8 *>(la[h][q] + at * 2 * STAGE + f * 4096);
         }
       };
       auto multiply = [&](int h) {
@@ -468,26 +495,34 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 ? 3 : WI * WJ == 8 ? 4 : 2) v
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      load(0, smem);
-      int at = 0;
-      for (int c = 0; c < n; ++c) {
-        load(1, smem + at * 2 * STAGE);
+      load(0, 0);
+      int c = 0, left = n - 1;                                   // chunks with one behind them
+      auto step = [&](int at) {                                  // chunk c, in stage `at`
+        load(1, at);
         __builtin_amdgcn_sched_barrier(0);
         multiply(0);
         __builtin_amdgcn_sched_barrier(0);
-        if (c + 1 < n) {
-          // chunks c + 1 ... c + S - 1 are requested
-          if (n - 2 - c >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * 2 * PIECES) : "memory");
-          else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-          __builtin_amdgcn_s_barrier();
-          asm volatile("" ::: "memory");
-          if (c + S < n) stage(at, c0 + c + S);
-          at = at + 1 == S ? 0 : at + 1;
-          load(0, smem + at * 2 * STAGE);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        // chunks c + 1 ... c + S - 1 are requested
+        if (S == 2 || left < S - 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * 2 * PIECES) : "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);                      // lgkmcnt(0), in the compiler's sight
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (left >= S) stage(at, c0 + c + S);
+        load(0, at + 1 == S ? 0 : at + 1);
+        __builtin_amdgcn_sched_barrier(0);
         multiply(1);
-      }
+        ++c;
+        --left;
+      };
+      while (left >= S)
+#pragma unroll
+        for (int at = 0; at < S; ++at) step(at);
+      int at = 0;
+      while (left > 0) step(at++);
+      load(1, at);
+      multiply(0);
+      multiply(1);
     };
     if (c0 < c1) {
       if (turned) product(OgTrue());
@@ -1409,7 +1444,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
       if (!blocks) break;
       // 64 x 64 tiles: up to two blocks per CU a third stage hides more latency than more resident blocks would (1024 x 4608: 415 us,
       // 492 with two stages), from then on they do (2048 x 9216: 1574, 1475 with two)
-      const int rc = T == 128       ? ortho_launch<128, 32, 2, 2, 4>(ws, lv, blocks, st)
+      const int rc = T == 128       ? ortho_launch<128, 32, 2, 2, 2>(ws, lv, blocks, st)
                      : blocks > 512 ? ortho_launch<64, 32, 2, 2, 2>(ws, lv, blocks, st)
                                     : ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st);
       if (rc) return rc;
