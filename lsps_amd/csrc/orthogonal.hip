@@ -1442,11 +1442,13 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
         blocks += (int)((units + 7) / 8 * 8);
       }
       if (!blocks) break;
-      // 64 x 64 tiles: up to two blocks per CU a third stage hides more latency than more resident blocks would (1024 x 4608: 415 us,
-      // 492 with two stages), from then on they do (2048 x 9216: 1574, 1475 with two)
+      // 64 x 64 tiles: more stages hide more latency as long as the blocks that a CU gets fit beside each other: 4 for one block per CU
+      // (1024 x 4608: 326 us, 347 with 3, 475 with 2), 3 for two (28 x 256 x 2304: 310; 316 with 4, 329 with 2), else 2 (2048 x 9216:
+      // 1282; 1398 with 3).  128 x 128 tiles: 2 stages, two blocks per CU (2048 x 9216: 1281; 1468 with 3)
       const int rc = T == 128       ? ortho_launch<128, 32, 2, 2, 2>(ws, lv, blocks, st)
                      : blocks > 512 ? ortho_launch<64, 32, 2, 2, 2>(ws, lv, blocks, st)
-                                    : ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st);
+                     : blocks > 256 ? ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st)
+                                    : ortho_launch<64, 32, 4, 2, 2>(ws, lv, blocks, st);
       if (rc) return rc;
       if (!split_any) break;
     }
