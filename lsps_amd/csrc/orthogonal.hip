@@ -1106,10 +1106,10 @@ struct OrthoCall {
 // on, and only where the long side's products fill the chip (`tiles`: 128 x 128 tiles of Q X of the whole pass; below, the number of
 // launches counts, and chains of one have the fewest).  They carry rounding further, the more the smaller M.  Five steps with chains
 // of 1 / 2 / 3, time and relative error against 64 bits, and the error of the plain iteration in f32:
-//   28 x 256 x 2304  438 / 369 / 332 us    1.5 / 1.7 / 3.0e-6  (3.4e-6)      4 x 256 x 1152   161 / 163 / 159 us    1.2 / 1.8 / 3.0e-6  (2.7e-6)
-//   2048 x 9216     2250 / 1708 / 1444     1.8 / 1.8 / 2.6e-6  (5.4e-6)      3 x 333 x 1021   171 / 181 / 180       1.2 / 1.6 / 2.7e-6  (2.7e-6)
-//   20 x 200 x 1000  226 / 212 / 208       1.3 / 2.1 / 3.7e-6  (2.5e-6)      1500 x 2000      476 / 500 / 492       1.3 / 1.3 / 4.1e-6  (3.6e-6)
-//   20 x 160 x 600   165 / 165 / 166       1.0 / 2.5 / 4.4e-6  (2.1e-6)      4 x 128 x 576    134 / 139 / 138       0.6 / 2.8 / 3.5e-6  (1.8e-6)
+//   28 x 256 x 2304  423 / 356 / 331 us    1.5 / 1.7 / 3.0e-6  (3.4e-6)      4 x 256 x 1152   156 / 150 / 162 us    1.2 / 1.8 / 3.0e-6  (2.7e-6)
+//   2048 x 9216     2060 / 1586 / 1348     1.8 / 1.8 / 2.6e-6  (5.4e-6)      3 x 333 x 1021   163 / 164 / 176       1.2 / 1.6 / 2.7e-6  (2.7e-6)
+//   20 x 200 x 1000  205 / 194 / 196       1.3 / 2.1 / 3.7e-6  (2.5e-6)      1500 x 2000      447 / 460 / 455       1.3 / 1.3 / 4.1e-6  (3.6e-6)
+//   1024 x 4608      435 / 363 / 329       1.3 / 1.3 / 3.1e-6  (3.8e-6)      4 x 128 x 576    122 / 121 / 135       0.7 / 2.8 / 3.5e-6  (1.8e-6)
 static int ortho_chain(const OrthoGroup &g, long tiles) {
   const int M = og_short(g), N = og_long(g);
   if (tiles < 256 || M < 192 || N < 2 * M) return 1;
@@ -1233,14 +1233,14 @@ static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
   return true;
 }
 
-// Ranges of a Gram matrix' reduction.  A product whose tiles leave CUs idle splits a long reduction into ranges of 256 columns (512
-// of the longest), at the price of the launch that adds them up.  Five steps: 3 x 333 x 1021 171 us with ranges of 256, 180 of 512, 189 of
-// 1024; 20 x 8192 149 us with 16 ranges, 166 with 32, 209 with 4; 4 x 128 x 576 122 us unsplit, 139 in two.
+// Ranges of a Gram matrix' reduction.  A product whose tiles leave CUs idle splits a long reduction into ranges of 512 columns, at the
+// price of the launch that adds them up.  Five steps: 512 x 2304 177 us, 187 with ranges of 1024; 200 x 4000 157, 168 with 256, 170 with
+// 1024; 4 x 128 x 576 110, 118 in two ranges; 3 x 333 x 1021 160 to 164 whatever the ranges.
 #define ORTHO_KZ 16
 static int ortho_kz(int K, long own, long tiles) {
   long z = 256 / (tiles > 0 ? tiles : 1);
   if (own <= 16 && z < K / 1024) z = K / 1024;             // few tiles in the company of many: not the launch's last ones
-  const long most = K < 768 ? 1 : K <= 1536 ? K / 256 : K / 512;
+  const long most = K / 512;
   if (z > most) z = most;
   if (z > ORTHO_KZ) z = ORTHO_KZ;
   return z < 2 ? 1 : (int)z;
