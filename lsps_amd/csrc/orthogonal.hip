@@ -18,12 +18,13 @@
 // Layout of a matrix with R rows: [column / 32][R][(column % 32) / 8][hi 8 | lo 8], rows and columns padded with zeros to multiples
 // of 64: a 32-deep chunk of a row is one 128-byte line and the rows of a chunk follow each other, so that a tile's chunk is one
 // contiguous run.  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.  X is kept one way round only:
-// Q X reads it transposed from LDS (28 x 256 x 2304: 407 us; with X^T beside X, 451).
+// Q X reads it transposed from LDS (28 x 256 x 2304 with an earlier loop: 407 us, 451 with X^T beside X).
 //
-// Times (MI355X): 28 x 256 x 2304 333 us (prologue 41, two Gram matrices 2 x 31, twelve 256 x 256 products 9 to 15 each, Q X 47 and
-// 40), 2048 x 9216 1443 us.  The 256 x 256 products are latency: 2 us from launch to launch, 1.6 to the first request, 1 to its
-// arrival, 2.5 for the product, 1.7 for the result.  The large ones run at 0.5 (symmetric) to 0.9 PFLOP/s of f16 MFMAs (a large
-// library product: 1.17): their blocks leave CUs idle (528 tiles, 256 CUs), and L2 to LDS carries 10 to 13 TB/s beside the MFMAs.
+// Times (MI355X): 28 x 256 x 2304 331 us (prologue 41, two Gram matrices 30 each, twelve 256 x 256 products 10.5 to 14, Q X 42 each),
+// 2048 x 9216 1281 to 1350 us from one card to the next.  The 256 x 256 products are latency: 2 us from launch to launch, 1.6 to the
+// first request, 1 to its arrival, 2.5 for the product, 1.7 for the result.  The large ones run at 0.5 to 0.7 (symmetric; Q X: 1.0 to
+// 1.1) PFLOP/s of f16 MFMAs, a large library product at 1.17.  Parts of them alone, 2048 x 9216: Gram matrix on 64-wide tiles 165 us
+// (MFMAs 105, LDS-DMA 130, LDS reads 61), Q X on 128-wide ones 214 (173, 136, 53).
 // All matrices of a call go through one launch per product (a block finds its group of equal matrices in the kernel's arguments).
 #include <limits.h>
 #include <math.h>

@@ -1760,6 +1760,11 @@ def _rows(t, rows, cols):
     return v, (v.stride(0) if rows > 1 else cols)
 
 
+def _like(t):
+    """A contiguous buffer of the shape and type of `t` (new_empty(t.shape) takes twice as long)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 LN_FWD_COLS = 16384       # rows up to here need no workspace in the forward (csrc/layernorm.hip)
 
 
@@ -1769,8 +1774,8 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, index, cols, eps):
         rows = x.numel() // cols
-        y = x.new_empty(x.shape)
-        stats = x.new_empty((2, rows), dtype=torch.float32)
+        y = _like(x)
+        stats = x.new_empty((2, rows)) if x.dtype is torch.float32 else x.new_empty((2, rows), dtype=torch.float32)
         ctx.cols = cols
         if b is not None:
             ctx.bshape = b.shape
@@ -1801,11 +1806,14 @@ def _layer_norm_backward(ctx, dy):
     x, w, stats = ctx.saved_tensors
     cols, rows = ctx.cols, stats.shape[1]
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    dx = dy.new_empty(dy.shape) if need_x else None
-    alloc = stats.new_empty if rows else stats.new_zeros
-    dw = alloc(w.shape) if need_w else None
-    db = alloc(ctx.bshape) if need_b else None
-    if rows:
+    dx = _like(dy) if need_x else None
+    dw = torch.empty_like(w) if need_w else None
+    db = (stats.new_empty(ctx.bshape) if w is None else torch.empty_like(w)) if need_b else None
+    if not rows:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    else:
         L = _lib.lib()
         dt = _DTYPES[x.dtype]
         xr, ldx = _rows(x, rows, cols)
