@@ -420,7 +420,8 @@ int lsps_adam_step(float *p, const float *g, float *m, float *v,
  * lsps_muon_step: for every matrix  m <- momentum m + grad_scale g,  G = nesterov ? grad_scale g + momentum m : m,
  *   p <- p (1 - lr weight_decay) - lr rms sqrt(max(rows, cols)) NS(G).  (A matrix with orthonormal rows or columns has entries
  *   of root mean square 1 / sqrt(max(rows, cols)): `rms` is the size of a weight's step in units of lr; 0.2 is about Adam's.)
- *   All matrices go through the same launches; `mats` is host memory and is not read after the call returns.
+ *   All matrices go through the same launches; `mats` is host memory and is not read after the call returns.  Memory that is
+ *   written may not overlap other memory of the call.
  * Neither call allocates, synchronises or keeps anything: both can be captured. */
 typedef struct LspsMuonMatrix {
   float *p;            /* weights   [rows][cols], updated */

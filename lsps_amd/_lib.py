@@ -77,8 +77,8 @@ _SIGNATURES = {
     'lsps_adam_step': (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int] + [c_float] * 6 + [_P]),
     'lsps_newton_schulz_workspace_bytes': (c_size_t, [c_int] * 4),
     'lsps_newton_schulz': (c_int, [_P, _P] + [c_int] * 5 + [c_float] * 4 + [_P, c_size_t, _P]),
-    'lsps_muon_workspace_bytes': (c_size_t, [ctypes.POINTER(LspsMuonMatrix), c_int, c_int]),
-    'lsps_muon_step': (c_int, [ctypes.POINTER(LspsMuonMatrix), c_int, c_float, c_float, c_int, c_float, c_float, c_float, c_int] +
+    'lsps_muon_workspace_bytes': (c_size_t, [_P, c_int, c_int]),
+    'lsps_muon_step': (c_int, [_P, c_int, c_float, c_float, c_int, c_float, c_float, c_float, c_int] +
                        [c_float] * 4 + [_P, c_size_t, _P]),
     'lsps_layernorm_workspace_bytes': (c_size_t, [c_long, c_long, c_int]),
     'lsps_layernorm_fwd': (c_int, [_P] * 6 + [c_long] * 3 + [c_int, c_float, _P, c_size_t, _P]),

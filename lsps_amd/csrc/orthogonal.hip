@@ -28,6 +28,7 @@
 // All matrices of a call go through one launch per product (a block finds its group of equal matrices in the kernel's arguments).
 #include <limits.h>
 #include <math.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include "c8util.h"
@@ -1586,6 +1587,35 @@ size_t lsps_muon_workspace_bytes(const LspsMuonMatrix *mats, int n, int steps) {
   return most;
 }
 
+// Does memory that the step writes overlap other memory of it?  (-1: no memory to look.)
+struct MuonSpan {
+  uintptr_t lo, hi;
+  int written;
+};
+static int muon_before(const void *a, const void *b) {
+  const MuonSpan *x = (const MuonSpan *)a, *y = (const MuonSpan *)b;
+  return x->lo < y->lo ? -1 : x->lo > y->lo;
+}
+static int muon_overlap(const LspsMuonMatrix *mats, int n) {
+  MuonSpan few[96], *v = n <= 32 ? few : (MuonSpan *)malloc(sizeof(MuonSpan) * 3 * n);
+  if (!v) return -1;
+  for (int i = 0; i < n; ++i) {
+    const uintptr_t size = (uintptr_t)mats[i].rows * mats[i].cols * sizeof(float);
+    const uintptr_t at[3] = {(uintptr_t)mats[i].p, (uintptr_t)mats[i].m, (uintptr_t)mats[i].g};
+    for (int k = 0; k < 3; ++k) v[3 * i + k] = MuonSpan{at[k], at[k] + size, k < 2};
+  }
+  qsort(v, 3 * (size_t)n, sizeof *v, muon_before);
+  uintptr_t end = 0, end_written = 0;
+  int found = 0;
+  for (int i = 0; i < 3 * n && !found; ++i) {
+    found = v[i].lo < end_written || (v[i].written && v[i].lo < end);
+    if (v[i].hi > end) end = v[i].hi;
+    if (v[i].written && v[i].hi > end_written) end_written = v[i].hi;
+  }
+  if (v != few) free(v);
+  return found;
+}
+
 int lsps_muon_step(const LspsMuonMatrix *mats, int n, float lr, float momentum, int nesterov, float weight_decay, float rms, float grad_scale,
                    int steps, float a, float b, float c, float eps, void *ws, size_t ws_bytes, void *stream) {
   static thread_local MuonPass p;
@@ -1598,6 +1628,8 @@ int lsps_muon_step(const LspsMuonMatrix *mats, int n, float lr, float momentum, 
     LSPS_CHECK_ARG(mats[i].p && mats[i].g && mats[i].m, "muon_step: null pointer in matrix %d", i);
     LSPS_CHECK_ARG(ortho_sane(ortho_group(1, mats[i].rows, mats[i].cols)), "muon_step: matrix %d of %d x %d", i, mats[i].rows, mats[i].cols);
   }
+  const int overlap = muon_overlap(mats, n);
+  LSPS_CHECK_ARG(overlap == 0, "muon_step: %s", overlap < 0 ? "out of host memory" : "weights, momenta or gradients overlap");
   const OrthoCall call = {steps, a, b, c, eps, OM_MUON, false, 1.f - lr * weight_decay, {momentum, grad_scale, nesterov != 0}};
   OrthoPlan *plan = ortho_plans();
   for (int at = 0; at < n; at += p.taken) {

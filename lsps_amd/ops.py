@@ -5,6 +5,7 @@ op below runs in liblsps_hip.so.  Each Function names the torch built-in of the 
 replaces.  Inputs must be HIP float32 tensors — there is no CPU fallback (``_lib.ptr`` raises).
 """
 import ctypes as _ctypes
+import struct as _struct
 
 import torch
 
@@ -1889,17 +1890,7 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     return out
 
 
-def _disjoint(what, written, read):
-    """Refuses memory that one call would both write and use twice."""
-    spans = sorted([(t.data_ptr(), t.data_ptr() + 4 * t.numel(), True) for t in written] +
-                   [(t.data_ptr(), t.data_ptr() + 4 * t.numel(), False) for t in read])
-    end, end_written = 0, 0
-    for lo, hi, w in spans:
-        if lo < end_written or (w and lo < end):
-            raise _lib.LspsHipError("%s: tensors overlap" % what)
-        end = max(end, hi)
-        if w:
-            end_written = max(end_written, hi)
+_MUON_MATRIX = _struct.Struct('@PPPii')        # struct LspsMuonMatrix
 
 
 def muon_step_(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, rms=0.2, grad_scale=1.0, steps=5,
@@ -1911,19 +1902,25 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not (len(params) == len(grads) == len(momenta)):
         raise _lib.LspsHipError("muon_step_: %d weights, %d gradients, %d momenta" % (len(params), len(grads), len(momenta)))
-    for p, g, m in zip(params, grads, momenta):
-        if not all(isinstance(t, torch.Tensor) for t in (p, g, m)):
-            raise _lib.LspsHipError("muon_step_: a weight, gradient or momentum is no tensor")
-        if p.dim() < 2 or p.shape != g.shape or p.shape != m.shape or p.numel() == 0:
-            raise _lib.LspsHipError("muon_step_: weight %s, gradient %s, momentum %s" % (tuple(p.shape), tuple(g.shape), tuple(m.shape)))
     if not params:
         return
+    mats, index = [], None
+    for matrix in zip(params, grads, momenta):          # (the host's part of a small step: no more calls here than it takes)
+        p, g, m = matrix
+        if not (isinstance(p, torch.Tensor) and isinstance(g, torch.Tensor) and isinstance(m, torch.Tensor)):
+            raise _lib.LspsHipError("muon_step_: a weight, gradient or momentum is no tensor")
+        shape, n = p.shape, p.numel()
+        if len(shape) < 2 or g.shape != shape or m.shape != shape or not 0 < n < 1 << 31:
+            raise _lib.LspsHipError("muon_step_: weight %s, gradient %s, momentum %s" % (tuple(shape), tuple(g.shape), tuple(m.shape)))
+        if index is None:
+            index = _same_device('muon_step_', p)
+        for t in matrix:
+            if t.get_device() != index or t.dtype is not torch.float32 or not t.is_contiguous():
+                _lib.ptr(t)                             # raises, unless it is the device
+                _same_device('muon_step_', p, t)
+        mats.append(_MUON_MATRIX.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), shape[0], n // shape[0]))
+    mats = b''.join(mats)
     L = _lib.lib()
-    index = _same_device('muon_step_', params[0], *(params + grads + momenta))
-    mats = (_lib.LspsMuonMatrix * len(params))()
-    for k, (p, g, m) in enumerate(zip(params, grads, momenta)):
-        mats[k] = _lib.LspsMuonMatrix(_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), *_ints('muon_step_', p.shape[0], p.numel() // p.shape[0]))
-    _disjoint('muon_step_', params + momenta, grads)
     steps, = _ints('muon_step_', steps)
     buf, ws, n = _scratch(L.lsps_muon_workspace_bytes(mats, len(params), steps), params[0])
     _launch('muon_step', index, L.lsps_muon_step, mats, len(params), float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),

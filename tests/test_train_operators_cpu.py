@@ -32,18 +32,31 @@ def test_refusals_of_the_python_entry_points():
             ops._ints('t', 2, n)
 
 
-def test_overlapping_tensors_are_refused():
-    a, b = torch.zeros(40), torch.zeros(40)
-    ops._disjoint('t', [a[:10], a[10:20], b], [a[20:], a[20:30]])           # reads may overlap reads
-    for written, read in (([a, a], []), ([a[:10], a[9:12]], []), ([a[:10]], [a[5:6]]), ([a[5:6]], [a]), ([b, a[30:]], [a[:31]])):
-        with pytest.raises(_lib.LspsHipError):
-            ops._disjoint('t', written, read)
+@pytest.mark.parametrize('more', [0, 40])
+def test_overlapping_matrices_are_refused(more):
+    """What a Muon step writes (weights, momenta) may not overlap anything else of it; gradients may be shared.  The addresses are
+    never followed: a call that passes ends at the missing workspace."""
+    h = _lib.lib()
+    far = [(1 << 30) + k * 4096 for k in range(3 * more)]                   # (more matrices than the check keeps on its stack)
+
+    def step(*mats):
+        mats = [_lib.LspsMuonMatrix(*m) for m in mats] + [_lib.LspsMuonMatrix(*far[3 * k:3 * k + 3], 4, 8) for k in range(more)]
+        return h.lsps_muon_step((_lib.LspsMuonMatrix * len(mats))(*mats), len(mats), 0.1, 0.9, 1, 0.0, 0.2, 1.0, 5, 3.4445, -4.775, 2.0315, 1e-7,
+                                None, 0, None)
+    a, size = 4096, 4 * 4 * 8
+    assert step((a, a + size, a + 2 * size, 4, 8)) == -2
+    assert step((a, a + size, a + 2 * size, 4, 8), (a + 4 * size, a + 3 * size, a + 6 * size, 4, 8)) == -2
+    assert step((a, a + size, a + 2 * size, 4, 8), (a + 4 * size, a + size, a + 5 * size, 4, 8)) == -2      # one gradient for two weights
+    for p, g, m in ((a, a, a + size), (a, a + size, a), (a, a + size, a + 4), (a, a + size - 4, a + 4 * size), (a + size - 4, a, a + 4 * size)):
+        assert step((p, g, m, 4, 8)) == -1 and 'overlap' in err(), (p, g, m)
+    assert step((a, a + size, a + 2 * size, 4, 8), (a + 4 * size, a + 5 * size, a, 4, 8)) == -1             # one weight is another's momentum
+    assert step((a, a + 9 * size, a + 3 * size, 4, 8), (a + size // 2, a + 5 * size, a + 6 * size, 2, 2)) == -1
 
 
 def test_refusals_of_the_c_entry_points():
     """Arguments are checked before anything touches the device (there is none here)."""
     h = _lib.lib()
-    buf = (ctypes.c_char * 64)()
+    buf = (ctypes.c_char * 256)()
     p = ctypes.cast(buf, ctypes.c_void_p)
 
     def ln(rows=2, cols=8, ldx=8, dtype=0, eps=1e-5, x=p, y=p, mean=p, ws=None, n=0):
@@ -77,7 +90,7 @@ def test_refusals_of_the_c_entry_points():
     def muon(mats, lr=0.1, mu=0.9, wd=0.0, rms=0.2, gs=1.0, n=0):
         arr = (_lib.LspsMuonMatrix * max(1, len(mats)))(*mats)
         return h.lsps_muon_step(arr, len(mats), lr, mu, 1, wd, rms, gs, 5, 3.4445, -4.775, 2.0315, 1e-7, p, n, None)
-    one = _lib.LspsMuonMatrix(p.value, p.value, p.value, 4, 4)
+    one = _lib.LspsMuonMatrix(p.value, p.value + 64, p.value + 128, 4, 4)
     assert muon([]) == -1 and muon([_lib.LspsMuonMatrix(None, p.value, p.value, 4, 4)]) == -1
     assert muon([_lib.LspsMuonMatrix(p.value, p.value, p.value, 0, 4)]) == -1
     for kw in (dict(lr=float('nan')), dict(mu=1.0), dict(mu=-0.1), dict(mu=float('nan')), dict(wd=float('inf')), dict(gs=float('nan'))):
