@@ -438,8 +438,8 @@ int lsps_muon_step(const LspsMuonMatrix *mats, int n, float lr, float momentum, 
 
 /* ---- LayerNorm over the last dimension (nn.LayerNorm; no reference counterpart: its nets use Instance- and BatchNorm) ----
  * x: `rows` rows of `cols` elements (dtype LSPS_F32 or LSPS_BF16) with a pitch of `ldx` elements between rows; y and dx have the
- * same type, contiguous; gamma / beta (nullable), the statistics mean[rows] / rstd[rows] saved for the backward and the gradients
- * dgamma / dbeta (nullable, overwritten) are float32.  dx nullable.  The same inputs give the same bits (no atomics). */
+ * same type, contiguous; gamma / beta (nullable), the statistics mean[rows] / rstd[rows] saved for the backward (the forward's: both
+ * or neither) and the gradients dgamma / dbeta (nullable, overwritten) are float32.  dx nullable.  The same inputs give the same bits (no atomics). */
 size_t lsps_layernorm_workspace_bytes(long rows, long cols, int dtype);
 int lsps_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, long rows, long cols,
                        long ldx, int dtype, float eps, void *ws, size_t ws_bytes, void *stream);

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(WG) void ln_fwd_kernel(const typename U::type *__re
       for (int e = 0; e < V; ++e) o[e] = fmaf(v[u][e] * rs, wv[u][e], bv[u][e]);
       if (skip[u] < V) ln_put<U>(y + r * cols + at[u], o);                             // (columns of two units get the same bits twice)
     }
-    if (t == 0) {
+    if (t == 0 && mean) {
       mean[r] = mu;
       rstd[r] = rs;
     }
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(256) void ln_split_fwd_kernel(const T *__restrict__
         ln_store<T>(y + r * cols + c0 + c, n - c, o);
       }
     }
-    if (threadIdx.x == 0 && c0 == 0) {
+    if (threadIdx.x == 0 && c0 == 0 && mean) {
       mean[r] = mu;
       rstd[r] = rs;
     }
@@ -696,9 +696,9 @@ size_t lsps_layernorm_workspace_bytes(long rows, long cols, int dtype) {
   return align_up(ln_ws_bytes(rows, cols, dtype == LSPS_F32 ? 4 : 8), 256);
 }
 
-static int ln_check(const char *what, const void *x, const float *mean, const float *rstd, long rows, long cols, long ldx, int dtype,
-                    void *ws, size_t ws_bytes, bool needs_ws) {
-  LSPS_CHECK_ARG(x && mean && rstd, "%s: null pointer", what);
+static int ln_check(const char *what, const void *x, bool stats, long rows, long cols, long ldx, int dtype, void *ws, size_t ws_bytes,
+                    bool needs_ws) {
+  LSPS_CHECK_ARG(x && stats, "%s: null pointer", what);
   LSPS_CHECK_ARG(dtype == LSPS_F32 || dtype == LSPS_BF16, "%s: dtype %d (LSPS_F32 or LSPS_BF16)", what, dtype);
   LSPS_CHECK_ARG(rows > 0 && cols > 0 && rows <= (1L << 40) / cols, "%s: %ld rows of %ld columns", what, rows, cols);
   LSPS_CHECK_ARG(ldx >= cols || rows == 1, "%s: row pitch %ld below %ld columns", what, ldx, cols);
@@ -715,7 +715,7 @@ static int ln_check(const char *what, const void *x, const float *mean, const fl
 int lsps_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, long rows, long cols,
                        long ldx, int dtype, float eps, void *ws, size_t ws_bytes, void *stream) {
   (void)hipGetLastError();   // clear stale sticky errors left by other users of the runtime
-  if (const int rc = ln_check("layernorm_fwd", x, mean, rstd, rows, cols, ldx, dtype, ws, ws_bytes, cols > LN_FWD_COLS)) return rc;
+  if (const int rc = ln_check("layernorm_fwd", x, !mean == !rstd, rows, cols, ldx, dtype, ws, ws_bytes, cols > LN_FWD_COLS)) return rc;
   LSPS_CHECK_ARG(y, "layernorm_fwd: null output");
   LSPS_CHECK_ARG(eps >= 0.f, "layernorm_fwd: eps %g", (double)eps);
   return dtype == LSPS_F32 ? ln_fwd<float>(x, gamma, beta, y, mean, rstd, rows, cols, ldx, eps, ws, (hipStream_t)stream)
@@ -725,7 +725,7 @@ int lsps_layernorm_fwd(const void *x, const float *gamma, const float *beta, voi
 int lsps_layernorm_bwd(const void *dy, const void *x, const float *mean, const float *rstd, const float *gamma, void *dx, float *dgamma,
                        float *dbeta, long rows, long cols, long ldx, long lddy, int dtype, void *ws, size_t ws_bytes, void *stream) {
   (void)hipGetLastError();   // clear stale sticky errors left by other users of the runtime
-  if (const int rc = ln_check("layernorm_bwd", x, mean, rstd, rows, cols, ldx, dtype, ws, ws_bytes, true)) return rc;
+  if (const int rc = ln_check("layernorm_bwd", x, mean && rstd, rows, cols, ldx, dtype, ws, ws_bytes, true)) return rc;
   LSPS_CHECK_ARG(dy && (dx || dgamma || dbeta), "layernorm_bwd: null gradient");
   LSPS_CHECK_ARG(lddy >= cols || rows == 1, "layernorm_bwd: row pitch %ld below %ld columns", lddy, cols);
   return dtype == LSPS_F32 ? ln_bwd<float>(dy, x, mean, rstd, gamma, dx, dgamma, dbeta, rows, cols, ldx, lddy, ws, (hipStream_t)stream)

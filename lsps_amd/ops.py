@@ -1769,32 +1769,38 @@ def _like(t):
 LN_FWD_COLS = 16384       # rows up to here need no workspace in the forward (csrc/layernorm.hip)
 
 
+def _layer_norm_forward(x, w, b, stats, index, cols, eps):
+    """(y, the rows that were read, their weights).  `stats`: [2, rows] for the backward, or None."""
+    rows = x.numel() // cols
+    y = _like(x)
+    if not rows:
+        return y, x, w
+    L = _lib.lib()
+    dt = _DTYPES[x.dtype]
+    if w is not None:
+        w = _c(w)
+    if b is not None:
+        b = _c(b)
+    xr, ldx = _rows(x, rows, cols)
+    buf, ws, n = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x) if cols > LN_FWD_COLS else (None, None, 0)
+    mean, rstd = (None, None) if stats is None else (stats.data_ptr(), stats.data_ptr() + 4 * rows)
+    _launch('layernorm_fwd', index, L.lsps_layernorm_fwd, xr.data_ptr(), None if w is None else w.data_ptr(),
+            None if b is None else b.data_ptr(), y.data_ptr(), mean, rstd, rows, cols, ldx, dt, eps, ws, n)
+    return y, (x if xr.data_ptr() == x.data_ptr() else xr), w
+
+
 class _LayerNormFn(torch.autograd.Function):
     """nn.LayerNorm.  The statistics are saved, the normalised values are formed again in the backward."""
 
     @staticmethod
     def forward(ctx, x, w, b, index, cols, eps):
-        rows = x.numel() // cols
-        y = _like(x)
-        stats = x.new_empty((2, rows)) if x.dtype is torch.float32 else x.new_empty((2, rows), dtype=torch.float32)
+        shape = (2, x.numel() // cols)
+        stats = x.new_empty(shape) if x.dtype is torch.float32 else x.new_empty(shape, dtype=torch.float32)
+        y, xr, w = _layer_norm_forward(x, w, b, stats, index, cols, eps)
         ctx.cols = cols
         if b is not None:
             ctx.bshape = b.shape
-        if not rows:
-            ctx.save_for_backward(x, w, stats)
-            return y
-        L = _lib.lib()
-        dt = _DTYPES[x.dtype]
-        if w is not None:
-            w = _c(w)
-        if b is not None:
-            b = _c(b)
-        xr, ldx = _rows(x, rows, cols)
-        buf, ws, n = _scratch(L.lsps_layernorm_workspace_bytes(rows, cols, dt), x) if cols > LN_FWD_COLS else (None, None, 0)
-        sp = stats.data_ptr()
-        _launch('layernorm_fwd', index, L.lsps_layernorm_fwd, xr.data_ptr(), None if w is None else w.data_ptr(),
-                None if b is None else b.data_ptr(), y.data_ptr(), sp, sp + 4 * rows, rows, cols, ldx, dt, eps, ws, n)
-        ctx.save_for_backward(x if xr.data_ptr() == x.data_ptr() else xr, w, stats)
+        ctx.save_for_backward(xr, w, stats)
         return y
 
     @staticmethod
@@ -1846,7 +1852,10 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
         if t is not None and (t.shape != shape or t.dtype != torch.float32):
             raise _lib.LspsHipError("layer_norm: weight or bias of shape %s, %s (expected %s, float32)" % (tuple(t.shape), t.dtype, shape))
     index = _same_device('layer_norm', x, weight, bias)
-    return _LayerNormFn.apply(x, weight, bias, index, cols, float(eps))
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _LayerNormFn.apply(x, weight, bias, index, cols, float(eps))
+    return _layer_norm_forward(x, weight, bias, None, index, cols, float(eps))[0]
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)     # quintic whose iterates send (0, 1] near 1 within five steps (the usual choice with Muon)

@@ -186,6 +186,21 @@ def test_gradient_against_differences():
         assert abs(num - ana) <= tol and abs(ana) > tol, (k, num, ana, tol)
 
 
+@pytest.mark.parametrize('rows,cols', [(9, 3), (33, 50), (7, 1023), (5, 9000), (3, 20000)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_without_gradients_the_same_bits(rows, cols, dtype):
+    """No statistics are kept when nothing needs a gradient."""
+    from lsps_amd import ops
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, cols, generator=gen).to(dtype).cuda()
+    w, b = torch.randn(cols, generator=gen).cuda(), torch.randn(cols, generator=gen).cuda()
+    want = ops.layer_norm(x, cols, w.clone().requires_grad_(True), b)
+    assert want.requires_grad and not ops.layer_norm(x, cols, w, b).requires_grad
+    assert torch.equal(ops.layer_norm(x, cols, w, b), want)
+    with torch.no_grad():
+        assert torch.equal(ops.layer_norm(x.requires_grad_(True), cols, w, b), want)
+
+
 def test_empty():
     from lsps_amd import ops
     for dtype in (torch.float32, torch.bfloat16):
