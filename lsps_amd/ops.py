@@ -1885,17 +1885,16 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     if g.requires_grad and torch.is_grad_enabled():
         raise _lib.LspsHipError("newton_schulz has no backward pass: call it under torch.no_grad() or on a detached tensor")
     index = _same_device('newton_schulz', g)
-    with torch.no_grad():
-        out = torch.empty_like(g, memory_format=torch.contiguous_format)
-        if g.numel() == 0:
-            return out
-        L = _lib.lib()
-        g = _c(g)
-        rows, cols = g.shape[-2:]
-        count, rows, cols, steps = _ints('newton_schulz', g.numel() // (rows * cols), rows, cols, steps)
-        buf, ws, n = _scratch(L.lsps_newton_schulz_workspace_bytes(count, rows, cols, steps), g)
-        _launch('newton_schulz', index, L.lsps_newton_schulz, g.data_ptr(), out.data_ptr(), count, rows, cols, _DTYPES[g.dtype], steps,
-                *_coeffs(coeffs), float(eps), ws, n)
+    out = _like(g)
+    if g.numel() == 0:
+        return out
+    L = _lib.lib()
+    g = _c(g)
+    rows, cols = g.shape[-2:]
+    count, rows, cols, steps = _ints('newton_schulz', g.numel() // (rows * cols), rows, cols, steps)
+    buf, ws, n = _scratch(L.lsps_newton_schulz_workspace_bytes(count, rows, cols, steps), g)
+    _launch('newton_schulz', index, L.lsps_newton_schulz, g.data_ptr(), out.data_ptr(), count, rows, cols, _DTYPES[g.dtype], steps,
+            *_coeffs(coeffs), float(eps), ws, n)
     return out
 
 
