@@ -1416,7 +1416,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
   else ORTHO_PRE(__bf16, false);
 #undef ORTHO_PRE
   for (int l = 0; l < levels; ++l) {
-    long b128 = 0, long128 = 0;                                         // 128 x 128 tiles, those of short sides from 1024 on
+    long b128 = 0, mid128 = 0, long128 = 0;                             // 128 x 128 tiles, those of short sides from 256, 1024 on
     bool square = true;
     for (int i = 0; i < n; ++i) {
       const OrthoPlan &p = plan[lo.chain[i] - 1];
@@ -1426,6 +1426,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
       square = square && lv.gs.g[i].type == OL_SYM;
       const long units = (long)g[i].count * lv.gs.g[i].jobs * og_tiles(g[i], lv.gs.g[i].type, 128);
       b128 += units;
+      if (og_short(g[i]) >= 256) mid128 += units;
       if (og_short(g[i]) >= 1024) long128 += units;
     }
     // 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs, symmetric products of short sides
@@ -1433,7 +1434,9 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     // 2048 x 9216 (136 of 128) 1281 / 1465 us, 6 x 1024 x 1024 (216) 590 / 553, 2500 x 2500 (210) 1272 / 1119, 3700 x 3700 (435) 3330 /
     // 3030; 100 x 200 x 300 (300) 325 / 369, 64 x 256 x 2304 (192) 599 / 674, 40 x 512 x 512 (400) 561 / 564.  A split reduction on 128
     // does not help: 2048 x 2048, 3 ranges 34 us and 17 to join them, 46 on 64
-    const int T = b128 >= (square ? 500 : 256) || (square && long128 >= 200) ? 128 : 64;
+    // Q X: 2048 x 9216 (1152) 1545 / 1370, 64 x 256 x 2304 (2304) 660 / 642; 28 x 256 x 2304 (1008) 341 / 341, 1024 x 4608 (288) 346 / 343,
+    // 8 x 512 x 2304 (576) 340 / 347, 200 x 128 x 576 (1000) 327 / 342, the generator's 38 matrices (1080) 437 / 453
+    const int T = square ? (b128 >= 500 || long128 >= 200 ? 128 : 64) : mid128 >= 2000 || long128 >= 256 ? 128 : 64;
     bool split_any = false;
     for (int pass = 0; pass < 2; ++pass) {
       int blocks = 0;
