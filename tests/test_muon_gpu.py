@@ -53,7 +53,7 @@ SHAPES = [(1, 1, 1), (2, 1, 9), (2, 9, 1), (1, 2, 3), (3, 20, 50), (1, 50, 108),
           (300, 40, 300), (90, 20, 700),
           (40, 192, 200), (1, 1024, 1100), (20, 448, 1000),
           # 128 x 128 tiles with odd 64-row halves, symmetric and not; chains of two and three
-          (40, 520, 600), (40, 200, 930), (16, 260, 1100)]
+          (40, 520, 600), (40, 200, 930), (16, 260, 1100), (6, 1030, 1100), (2, 2100, 1030), (250, 260, 450)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
@@ -140,7 +140,8 @@ def muon_reference(p, g, m, lr, momentum, nesterov, wd, rms, gscale, steps=5):
 SETS = [[(50, 108)], [(50, 108), (20, 50), (50, 20), (108, 50)], [(64, 1, 7, 7), (128, 64, 3, 3), (20, 48, 2, 2), (1, 9), (9, 1), (256, 300)],
         [(33 + i % 7, 20 + i) for i in range(70)],
         [(30, 40), (40, 30), (30, 40), (200, 900), (70, 30), (200, 900), (520, 2100), (400, 420), (40, 30), (192, 500)],
-        [(64, 600), (20, 8192), (900, 40), (30, 40)]]
+        [(64, 600), (20, 8192), (900, 40), (30, 40)],
+        [(1100, 1030)] * 5 + [(40, 60), (1030, 1090)]]
 
 
 @pytest.mark.parametrize('nesterov', [True, False])
