@@ -687,8 +687,10 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
 struct OrthoSmallStep {
   float gram, s0, s1, diag, x;      // factors of A; of A A, A and I in Q = a I + b A + c A A; of Q X
 };
+#define ORTHO_FEW 16           // pointers that travel in the kernels' arguments, without a launch that fills the table
 struct OrthoSmall {
   OrthoGroups gs;
+  OrthoPtr few[ORTHO_FEW];          // read one per lane, as the groups are
   OrthoSmallStep step[ORTHO_STEPS];
   OrthoMomentum mo;
   int steps, mode;
@@ -974,6 +976,12 @@ __device__ __forceinline__ double og_block_sum(double s, double *red) {
   return t;
 }
 
+__device__ __forceinline__ OrthoPtr og_small_ptr(const OrthoSmall &c, const OrthoGroup &g, int mat, int bytes) {
+  if (g.ptr < 0 || c.gs.table) return ortho_ptr(c.gs, g, mat, bytes);
+  const OrthoPtr mine = c.few[threadIdx.x & (ORTHO_FEW - 1)];
+  return og_readlane(mine, __builtin_amdgcn_readfirstlane(g.ptr + mat));
+}
+
 template <typename T, bool MUON, int MT>
 __device__ __forceinline__ void ortho_alone(const OrthoSmall &c, const OrthoGroup &g, const OrthoPtr &ptr, char *smem, double *red) {
   const int chunks = (og_long(g) + 31) / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1001,7 +1009,7 @@ __global__ __launch_bounds__(256, 2) void ortho_small_kernel(OrthoSmall c) {
   __shared__ double red[16];
   int grp;
   const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
-  const OrthoPtr ptr = ortho_ptr(c.gs, g, blockIdx.x - g.first, sizeof(T));
+  const OrthoPtr ptr = og_small_ptr(c, g, blockIdx.x - g.first, sizeof(T));
   if (og_short(g) <= 32) ortho_alone<T, MUON, 1>(c, g, ptr, smem, red);
   else ortho_alone<T, MUON, 2>(c, g, ptr, smem, red);
 }
@@ -1020,7 +1028,7 @@ __device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGrou
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ti = MT > 1 ? (wave >> 1) * 32 : 0, tj = MT > 1 ? (wave & 1) * 32 : 0;
   const bool square = MT > 1 || wave == 0;
-  const OrthoPtr ptr = ortho_ptr(c.gs, g, mat, sizeof(T));
+  const OrthoPtr ptr = og_small_ptr(c, g, mat, sizeof(T));
   const bool tall = g.rows > g.cols;
   const int j0 = pan * wide * 32;
   char *mine = ws + (size_t)g.x_off * 256 + ((size_t)mat * all + pan * wide) * 8192;
@@ -1347,7 +1355,8 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
   const float x0 = plan[lo.chain[0] - 1].x0;                             // (the same for every chain length)
   for (int i = 0; i < n; ++i)
     if (plan[lo.chain[i] - 1].levels > levels) levels = plan[lo.chain[i] - 1].levels;
-  for (int i = 0; i < nptr; i += ORTHO_PTR_PART) {
+  const bool few = (lo.small || lo.panels) && nptr <= ORTHO_FEW;
+  for (int i = 0; i < nptr && !few; i += ORTHO_PTR_PART) {
     OrthoPtrPart part;
     const int k = nptr - i < ORTHO_PTR_PART ? nptr - i : ORTHO_PTR_PART;
     memcpy(part.p, ptrs + i, k * sizeof(OrthoPtr));
@@ -1358,7 +1367,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
   lv.mode = c.mode;
   lv.decay = c.decay;
   lv.gs.base = base;
-  lv.gs.table = (const OrthoPtr *)ws;
+  lv.gs.table = few ? nullptr : (const OrthoPtr *)ws;
   for (int i = 0; i < ORTHO_GROUPS; ++i) {
     if (i < n) lv.gs.g[i] = g[i];
     lv.gs.g[i].first = i < n ? lo.norm_first[i] : INT_MAX;
@@ -1368,6 +1377,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     OrthoSmall sm;
     memset(&sm, 0, sizeof sm);
     sm.gs = lv.gs;
+    if (few && nptr) memcpy(sm.few, ptrs, nptr * sizeof(OrthoPtr));
     sm.mo = c.mo;
     sm.steps = c.steps;
     sm.mode = c.mode;
