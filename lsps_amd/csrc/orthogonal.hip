@@ -334,6 +334,8 @@ struct OrthoLevel {
 //   OL_LAST: the same, the result in the caller's layout and type, or the weight update
 // A product with few tiles and a long reduction is split into kz ranges of it: f32 partial tiles in the workspace, added in a
 // fixed order by a second launch of this kernel.
+// Registers: as many waves per SIMD as fit beside each other in LDS (the second argument of the launch bounds); the accumulators have to
+// stay in VGPRs, and nothing may spill: one reload in the loop waits for every request under way.
 template <int T, int KC, int S, int WI, int WJ>
 __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
   constexpr int WAVES = WI * WJ, SUB = KC / 32, STAGE = T * KC * 4, PIECES = T * SUB / 8 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = 144;
@@ -672,8 +674,8 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
 // iteration in one workgroup (ortho_small_kernel).  Longer ones are cut into panels of columns, one workgroup each: a launch per step
 // adds the panels' shares of the Gram matrix up (every workgroup for itself, in a fixed order), forms Q, multiplies its panel by it and
 // leaves the panel's share of the next Gram matrix (ortho_panel_kernel).  A step of 108 x 50 takes 2.8 us: 0.7 for the Gram matrix, 0.8
-// for A A and Q, 1.2 for Q X; of them 24 + 12 + 24 MFMAs of 33 cycles 0.8, the LDS reads at 128 bytes a cycle 0.5, the conversions 0.6,
-// one after the other with a single wave per SIMD.
+// for A A and Q, 1.2 for Q X; of them 24 + 12 + 24 MFMAs of 33 cycles 0.8, the LDS reads at 250 bytes a cycle 0.4, the conversions 0.6,
+// one after the other with a single wave per SIMD, and three barriers.
 // Five steps, panels / the products as launches, us (one workgroup: 50 x 108 20, 64 x 256 31, 64 x 448 47):
 //   64 x 449  51 / 113     8 of 33 x 1000  59 / 127     100 of 64 x 576  93 / 150     64 x 4096   79 / 142    16 of 64 x 8192 221 / 246
 //   20 x 8192 86 / 152    40 of 64 x 576  69 / 126      256 of 64 x 576 183 / 229     64 x 14336 121 / 171    30 of 64 x 4096 204 / 224
