@@ -151,6 +151,11 @@ class FlatAdam(torch.optim.Optimizer):
         """Does `step` pass this parameter to lsps_adam_step?  (FlatMuon: not the matrices.)"""
         return True
 
+    def _of_another_kind(self, st):
+        """Is this a matrix' state from a FlatMuon?  It has no moments: Adam starts over with it (at the step count it comes with, its
+        bias corrections would make the first steps far too long)."""
+        return 'momentum_buffer' in st
+
     @torch.no_grad()
     def step(self, closure=None):
         if self.arena is None:
@@ -205,6 +210,10 @@ class FlatAdam(torch.optim.Optimizer):
         """Accepts a torch.optim.Adam / FlatAdam state dict (reference: lsps_trainer.py:288-295, load_opt=True).
         With an arena attached, the loaded moments are copied INTO the flat buffers (the kernel only reads those)."""
         super(FlatAdam, self).load_state_dict(state_dict)
+        fresh = [st for st in self.state.values() if self._of_another_kind(st)]
+        for st in fresh:
+            st.clear()
+            st['step'] = 0
         if self.arena is None:
             return                                   # attach() picks the loaded state up later
         a = self.arena
@@ -217,6 +226,8 @@ class FlatAdam(torch.optim.Optimizer):
                 view = flat[o:o + n].view(p.shape)
                 if key in st and st[key].data_ptr() != view.data_ptr():
                     view.copy_(st[key])
+                elif any(st is f for f in fresh):
+                    view.zero_()
                 st[key] = view
             st['step'] = int(st['step'].item()) if torch.is_tensor(st.get('step')) else int(st.get('step', 0))
 
@@ -243,6 +254,9 @@ class FlatMuon(FlatAdam):
 
     def _by_adam(self, p):
         return not self.is_matrix(p)
+
+    def _of_another_kind(self, st):
+        return False
 
     def _keep_momentum(self, loaded):
         """Leaves {step, momentum_buffer} as the state of each matrix; `loaded`: the momenta of a state dict (others start at zero:

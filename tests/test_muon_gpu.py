@@ -317,6 +317,45 @@ def test_flat_muon_matches_its_parts():
     assert not opt.state[ps[0]]['momentum_buffer'].any() and torch.equal(opt.state[ps[1]]['exp_avg'], oa.state[pa[1]]['exp_avg'])
 
 
+@pytest.mark.parametrize('before', [True, False])
+def test_adam_starts_over_with_matrices_of_a_muon_state(before):
+    """A FlatMuon's matrices have no moments: their first Adam step is one of a new optimizer, vectors go on where they were."""
+    from lsps_amd import optim
+    gen = torch.Generator().manual_seed(4)
+    shapes = [(12, 20), (12,)]
+    init = [0.1 * torch.randn(s, generator=gen) for s in shapes]
+    grad = [1e-2 * torch.randn(s, generator=gen).cuda() for s in shapes]
+
+    def build(cls, sd=None, loaded_first=False):
+        ps = [torch.nn.Parameter(t.clone().cuda()) for t in init]
+        opt = cls(ps, lr=0.01)
+        if sd and loaded_first:
+            opt.load_state_dict(sd)
+        opt.attach()
+        if sd and not loaded_first:
+            step(ps, opt)                                          # (moments that the load has to replace)
+            with torch.no_grad():
+                for p, t in zip(ps, init):
+                    p.copy_(t.cuda())
+            opt.load_state_dict(sd)
+        return ps, opt
+
+    def step(ps, opt):
+        opt.zero_grad()
+        sum((p * g).sum() for p, g in zip(ps, grad)).backward()
+        opt.step()
+    pm, om = build(optim.FlatMuon)
+    for _ in range(5):
+        step(pm, om)
+    ps, opt = build(optim.FlatAdam, om.state_dict(), before)
+    assert set(opt.state[ps[0]]) == {'step', 'exp_avg', 'exp_avg_sq'} and opt.state[ps[0]]['step'] == 0 and opt.state[ps[1]]['step'] == 5
+    assert torch.equal(opt.state[ps[1]]['exp_avg'], om.state[pm[1]]['exp_avg'])
+    pn, new = build(optim.FlatAdam)
+    step(ps, opt)
+    step(pn, new)
+    assert torch.equal(ps[0], pn[0]) and not torch.equal(ps[1], pn[1])
+
+
 def test_training_steps_with_layer_norm_and_muon():
     """The pose VAE with layer-normed hidden layers, stepped by FlatMuon through the trainer: the gradients and the first step are
     those of the plain computation in 64 bits; pretraining steps of the nets run on the same optimizer."""
