@@ -557,12 +557,15 @@ static int ln_rows_per_pass(long cols) { return cols <= 256 ? 16 : cols <= 1024 
 // workgroups of the register backward: enough to fill 256 CUs, few enough that the partial sums (8 bytes per column and
 // workgroup) stay small next to the rows they stand for; a handful of rows is one workgroup and needs no second launch.
 // Measured: 131072 x 256 f32 72 us with at most 768, 72 with 1024, 79 with 512, in bf16 37 / 41 / 36; one row per pass: 4096 x 4096
-// f32 34.5 us with 16 rows a workgroup, 37 with 8.
-static int ln_bwd_groups(long rows, long cols) {
+// f32 34.5 us with 16 rows a workgroup, 37 with 8.  One row per pass, 2^25 elements, with at most 256 / 512 / 768 / 1024 workgroups: f32
+// of 1500 columns 98 / 78 / 82 / 88, 3000 79 / 85 / 96, 8000 (one workgroup per CU) 89 / 113; bf16 of 1100 118 / 69 / 58 / 51, 1500 90 / 55 /
+// 47 / 47, 3000 54 / 45 / 48, 8000 50 / 73.
+static int ln_bwd_groups(long rows, long cols, int V) {
   const int rpp = ln_rows_per_pass(cols);
   const long passes = (rows + rpp - 1) / rpp;
   if (passes <= 4) return 1;
-  const long g = rpp > 1 ? (passes + 7) / 8 : (passes + 15) / 16, most = rpp > 1 ? 768 : 512;
+  const long g = rpp > 1 ? (passes + 7) / 8 : (passes + 15) / 16;
+  const long most = rpp > 1 ? 768 : cols > 4096 ? 256 : V == 4 ? (cols > 2048 ? 256 : 512) : cols > 2048 ? 512 : 768;
   return (int)(g < most ? g : most);
 }
 
@@ -578,7 +581,7 @@ static int ln_split_rows_per_group(long rows, long cols, int V) {
 
 static size_t ln_ws_bytes(long rows, long cols, int V) {
   if (cols <= LN_BWD_COLS) {
-    const int g = ln_bwd_groups(rows, cols);
+    const int g = ln_bwd_groups(rows, cols, V);
     return g > 1 ? (size_t)g * 2 * cols * sizeof(float) : 0;
   }
   const int rpg = ln_split_rows_per_group(rows, cols, V);
@@ -663,7 +666,7 @@ static int ln_bwd(const void *dy_, const void *x_, const float *mean, const floa
   int parts;
   if (cols <= LN_BWD_COLS) {
     part = (float *)ws;
-    parts = ln_bwd_groups(rows, cols);
+    parts = ln_bwd_groups(rows, cols, LnVec<T>::V);
     ln_bwd_launch<T>(dy, lddy, x, ldx, mean, rstd, w, dx, part, dw, db, rows, (int)cols, parts, st);
   } else {
     const int chunks = ln_chunks(cols), rpg = ln_split_rows_per_group(rows, cols, LnVec<T>::V);
