@@ -554,7 +554,8 @@ static int ln_chunks(long cols) { return (int)((cols + LN_CHUNK - 1) / LN_CHUNK)
 // rows per workgroup pass of the register variants
 static int ln_rows_per_pass(long cols) { return cols <= 256 ? 16 : cols <= 1024 ? 4 : 1; }
 
-// workgroups of the register backward: enough to fill 256 CUs, few enough that the partial sums (8 bytes per column and
+// workgroups of the register backward: one per CU as soon as there are passes for them (300 x 1500 f32 18 us with one for 16 rows, 9 so;
+// 100 x 8000 30 / 16; 1000 x 700 13 / 9), then enough to fill 256 CUs, few enough that the partial sums (8 bytes per column and
 // workgroup) stay small next to the rows they stand for; a handful of rows is one workgroup and needs no second launch.
 // Measured: 131072 x 256 f32 72 us with at most 768, 72 with 1024, 79 with 512, in bf16 37 / 41 / 36; one row per pass: 4096 x 4096
 // f32 34.5 us with 16 rows a workgroup, 37 with 8.  One row per pass, 2^25 elements, with at most 256 / 512 / 768 / 1024 workgroups: f32
@@ -564,7 +565,7 @@ static int ln_bwd_groups(long rows, long cols, int V) {
   const int rpp = ln_rows_per_pass(cols);
   const long passes = (rows + rpp - 1) / rpp;
   if (passes <= 4) return 1;
-  const long g = rpp > 1 ? (passes + 7) / 8 : (passes + 15) / 16;
+  const long few = passes < 256 ? passes : 256, many = rpp > 1 ? (passes + 7) / 8 : (passes + 15) / 16, g = many > few ? many : few;
   const long most = rpp > 1 ? 768 : cols > 4096 ? 256 : V == 4 ? (cols > 2048 ? 256 : 512) : cols > 2048 ? 512 : 768;
   return (int)(g < most ? g : most);
 }
