@@ -415,8 +415,9 @@ int lsps_adam_step(float *p, const float *g, float *m, float *v,
  * (no reference counterpart: the reference steps every parameter with Adam, lsps_trainer.py:26-29)
  * lsps_newton_schulz: out = the Newton-Schulz iterate of each of `count` contiguous rows x cols matrices (dtype LSPS_F32 or
  *   LSPS_BF16, out of the same type; may run in place):  X = G / (|G|_F + eps), then `steps` times
- *   X <- a X + (b A + c A^2) X with A = X X^T on the short side.  Arithmetic is f32-class for either type.  (a, b, c) is
- *   refused if it takes a value of [0, 1] out of bounds on the way (fixed-point limbs inside).
+ *   X <- a X + (b A + c A^2) X with A = X X^T on the short side.  Values are f32 (three bf16 limbs: 24 bits, f32's exponents) and
+ *   sums are f32 for either type, rows and columns far below the others included.  (a, b, c) is refused if it takes a value of
+ *   [0, 1] past 1e4 on the way.  Sides of at most 2^20, at most 2^29 elements a matrix with its sides rounded up to multiples of 64.
  * lsps_muon_step: for every matrix  m <- momentum m + grad_scale g,  G = nesterov ? grad_scale g + momentum m : m,
  *   p <- p (1 - lr weight_decay) - lr rms sqrt(max(rows, cols)) NS(G).  (A matrix with orthonormal rows or columns has entries
  *   of root mean square 1 / sqrt(max(rows, cols)): `rms` is the size of a weight's step in units of lr; 0.2 is about Adam's.)

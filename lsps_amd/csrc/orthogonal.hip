@@ -11,20 +11,18 @@
 // one of |b| / a (a^2)^k d, relatively, in the directions of small singular values after k more steps, so that chains of three
 // cost about what the plain iteration in f32 costs and longer ones more (ortho_chain has the measurements).
 //
-// Operands.  Every matrix lives in the workspace as two f16 limbs, v s = hi + lo with a power of two s chosen from a bound of
-// the matrix' entries (22 significand bits; the entries are bounded by the spectral norm, which is a polynomial of values in
-// [0, 1], see ortho_bounds), and a product is three v_mfma_f32_32x32x16_f16 (hi hi + hi lo + lo hi, f32 accumulation; the
-// dropped lo lo is below 2^-22 of the product): f32-class results at a third of the f16 rate, 5 x the f32 MFMA rate.
-// Layout of a matrix with R rows: [column / 32][R][(column % 32) / 8][hi 8 | lo 8], rows and columns padded with zeros to multiples
-// of 64: a 32-deep chunk of a row is one 128-byte line and the rows of a chunk follow each other, so that a tile's chunk is one
+// Operands.  Every matrix lives in the workspace as three bf16 limbs, which hold an f32 value exactly: 24 bits with an exponent of
+// their own, so that rows and columns far below the others (1e-9 and less) keep the relative accuracy they have in f32 arithmetic;
+// they grow by `a` a step and are as large as the others in the end.  (Two f16 limbs under one scale per matrix need half the
+// MFMAs, but are good for 22 bits down to 1e-5 of the norm only: rows of 1e-8 were off by 4 %.)  A product is six
+// v_mfma_f32_32x32x16_bf16 with f32 accumulation (limbs 0 0, 0 1, 1 0, 1 1, 0 2, 2 0; the dropped ones are below 2^-26 of it): 1.3 x
+// the rate of the f32 MFMAs.
+// Layout of a matrix with R rows: [column / 32][R][limb][(column % 32) / 8][8], rows and columns padded with zeros to multiples of 64:
+// a 32-deep chunk of a row is one line of 192 bytes and the rows of a chunk follow each other, so that a tile's chunk is one
 // contiguous run.  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.  X is kept one way round only:
-// Q X reads it transposed from LDS (28 x 256 x 2304 with an earlier loop: 407 us, 451 with X^T beside X).
+// Q X reads it transposed from LDS (28 x 256 x 2304 with an earlier loop on two limbs: 407 us, 451 with X^T beside X).
 //
-// Times (MI355X): 28 x 256 x 2304 331 us (prologue 41, two Gram matrices 30 each, twelve 256 x 256 products 10.5 to 14, Q X 42 each),
-// 2048 x 9216 1281 to 1350 us from one card to the next.  The 256 x 256 products are latency: 2 us from launch to launch, 1.6 to the
-// first request, 1 to its arrival, 2.5 for the product, 1.7 for the result.  The large ones run at 0.5 to 0.7 (symmetric; Q X: 1.0 to
-// 1.1) PFLOP/s of f16 MFMAs, a large library product at 1.17.  Parts of them alone, 2048 x 9216: Gram matrix on 64-wide tiles 165 us
-// (MFMAs 105, LDS-DMA 130, LDS reads 61), Q X on 128-wide ones 214 (173, 136, 53).
+// Times (MI355X): 28 x 256 x 2304 450 us, the generator's 38 matrices 570, 2048 x 9216 and the discriminator's other eight 3300.
 // All matrices of a call go through one launch per product (a block finds its group of equal matrices in the kernel's arguments).
 #include <limits.h>
 #include <math.h>
@@ -36,15 +34,17 @@
 
 namespace lsps {
 
-typedef _Float16 og_h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 og_h4 __attribute__((ext_vector_type(4)));
+typedef __bf16 og_b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 og_b4 __attribute__((ext_vector_type(4)));
 typedef float og_f16v __attribute__((ext_vector_type(16)));
 typedef float og_f2 __attribute__((ext_vector_type(2)));
-typedef _Float16 og_h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 og_b2 __attribute__((ext_vector_type(2)));
 typedef float og_f4 __attribute__((ext_vector_type(4)));
 typedef float og_f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short og_u4u __attribute__((ext_vector_type(4), aligned(2)));
 
+#define OG_BYTES 6             // of an element: three limbs
+#define OG_LINE (32 * OG_BYTES) // 32 columns of a row
 #define OG_BAND 512            // columns of a band of tiles of a symmetric product
 #define ORTHO_GROUPS 16        // shapes per pass (they travel in the kernels' arguments)
 #define ORTHO_MATRICES 1024    // matrices with pointers of their own per pass
@@ -128,12 +128,12 @@ __device__ __forceinline__ OrthoPtr ortho_ptr(const OrthoGroups &gs, const Ortho
 
 __device__ __forceinline__ char *ortho_buffer(char *ws, const OrthoGroup &g, int id, int mat) {
   const long M = og_pad(og_short(g)), N = og_pad(og_long(g));
-  if (id < OB_SMALL) return ws + (size_t)g.s_off * 256 + ((long)id * g.count + mat) * M * M * 4;
-  return ws + (size_t)g.x_off * 256 + ((long)(id - OB_X0) * g.count + mat) * M * N * 4;
+  if (id < OB_SMALL) return ws + (size_t)g.s_off * 256 + ((long)id * g.count + mat) * M * M * OG_BYTES;
+  return ws + (size_t)g.x_off * 256 + ((long)(id - OB_X0) * g.count + mat) * M * N * OG_BYTES;
 }
-// byte of element (row, col) of a matrix of R rows: its hi limb (the lo limb is 16 bytes on)
+// byte of element (row, col) of a matrix of R rows: its first limb (the others lie 64 and 128 bytes on)
 __device__ __forceinline__ long og_at(long R, int row, int col) {
-  return ((col >> 5) * R + row) * 128 + ((col >> 3) & 3) * 32 + (col & 7) * 2;
+  return ((col >> 5) * R + row) * OG_LINE + ((col >> 3) & 3) * 16 + (col & 7) * 2;
 }
 
 template <typename T>
@@ -204,27 +204,40 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoGroups gs, double 
   if (threadIdx.x == 0) sums[g.aux + rel] = red[0] + red[1] + red[2] + red[3];
 }
 
-// 4 values as two limbs each.  Kept in pairs, with -1 out of the compiler's sight: so a pair takes one conversion and two mixed
-// fused multiply-adds (6 instructions otherwise).
-__device__ __forceinline__ void og_split(const float (&v)[4], og_h4 &hi, og_h4 &lo) {
+// 4 values as three limbs each: what is left of one rounding to bf16 is exact, and so is the third limb of an f32 value
+__device__ __forceinline__ void og_split(const float (&v)[4], og_b4 (&l)[3]) {
 #pragma unroll
   for (int e = 0; e < 4; e += 2) {
-    og_h2 h = __builtin_convertvector((og_f2{v[e], v[e + 1]}), og_h2);
-    float minus = -1.f;
-    asm("" : "+s"(minus), "+v"(h));
-    hi[e] = h[0];
-    hi[e + 1] = h[1];
-    lo[e] = (_Float16)fmaf((float)h[0], minus, v[e]);
-    lo[e + 1] = (_Float16)fmaf((float)h[1], minus, v[e + 1]);
+    og_f2 r = {v[e], v[e + 1]};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const og_b2 b = __builtin_convertvector(r, og_b2);
+      l[k][e] = b[0];
+      l[k][e + 1] = b[1];
+      r = og_f2{r[0] - (float)b[0], r[1] - (float)b[1]};
+    }
   }
 }
+// the 4 values: sums of limbs, smallest first, are exact
+__device__ __forceinline__ void og_value(const og_b4 (&l)[3], float (&v)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = (float)l[0][k] + ((float)l[1][k] + (float)l[2][k]);
+}
 
-__device__ __forceinline__ og_h8 og_join(const og_h4 (&v)[2]) { return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ og_b8 og_join(const og_b4 &a, const og_b4 &b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// v / norm as f32: norm = mantissa * 2^ex, v 2^-ex rounded by one factor, so that nothing overflows on the way for any norm
+struct OgUnit {
+  float f;
+  int ex;
+  __device__ __forceinline__ explicit OgUnit(double norm) { f = (float)(1. / frexp(norm, &ex)); }
+  __device__ __forceinline__ float operator()(float v) const { return ldexpf(v, -ex) * f; }
+};
 
 // X0 as limbs, the short side in rows.  One 64 x 64 tile of G per block, through LDS (turned round there for a tall G).
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroups gs, char *__restrict__ ws, const double *__restrict__ sums,
-                                                          OrthoMomentum mo, float eps, float scale) {
+                                                          OrthoMomentum mo, float eps) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
   int grp;
@@ -256,12 +269,11 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroups gs, char *
     }
   }
   __syncthreads();
-  // one division of the 64-bit norm; the f32 quotient below is the rounding X / (|G| + eps) has in f32 arithmetic
-  const float norm = (float)(sqrt(red[0] + red[1] + red[2] + red[3]) + (double)eps);
+  const OgUnit unit(sqrt(red[0] + red[1] + red[2] + red[3]) + (double)eps);
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) tile[(threadIdx.x >> 4) + k * 16][(threadIdx.x & 15) * 4 + e] = v[k][e] / norm * scale;
+    for (int e = 0; e < 4; ++e) tile[(threadIdx.x >> 4) + k * 16][(threadIdx.x & 15) * 4 + e] = unit(v[k][e]);
   __syncthreads();
   const bool tall = g.rows > g.cols;
   char *dst = ortho_buffer(ws, g, OB_X0, mat);
@@ -269,21 +281,20 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoGroups gs, char *
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int u = threadIdx.x + k * 256, i = u >> 3, j = (u & 7) * 8;
-    og_h4 h[2], l[2];
+    og_b4 l[2][3];
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
       float x[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) x[c] = tall ? tile[j + e + c][i] : tile[i][j + e + c];
-      og_split(x, h[e / 4], l[e / 4]);
+      og_split(x, l[e / 4]);
     }
-    og_h8 *o = reinterpret_cast<og_h8 *>(dst + og_at(M, i0 + i, j0 + j));
-    o[0] = og_join(h);
-    o[1] = og_join(l);
+    char *o = dst + og_at(M, i0 + i, j0 + j);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<og_b8 *>(o + q * 64) = og_join(l[0][q], l[1][q]);
   }
 }
 
-// out = k0 (product) + k1 E1 + k2 E2 + diag I on stored (scaled) values: the scales are folded into the factors
 __device__ __forceinline__ void og_result(void *out, long o, float v, int mode, float step, float decay) {
   if (mode == OM_F32) ((float *)out)[o] = v;
   else if (mode == OM_BF16) ((__bf16 *)out)[o] = (__bf16)v;               // the one rounding of the result
@@ -312,7 +323,7 @@ struct OgTrue {
 struct OgFalse {
   static constexpr bool value = false;
 };
-struct OrthoJob {
+struct OrthoJob {                   // out = k0 (product) + k1 E1 + k2 E2 + diag I
   int l, r, e1, e2, out;
   float k0, k1, k2, diag;
 };
@@ -325,9 +336,9 @@ struct OrthoLevel {
 };
 
 // One product per block: a T x T tile.  WI x WJ waves, each (T / WI) x (T / WJ) in 32x32 MFMA tiles; the MFMA's row index is the tile's
-// COLUMN, so a lane holds one row of the result and runs of 4 columns (8-byte stores per limb).  hi hi has an accumulator of its
-// own: the small cross products, added to it, would cost it a rounding each (measured: that halves the error of the whole
-// iteration).  LDS: S stages of a KC-deep chunk of both operands, S - 1 of them requested ahead by LDS-DMA (from inline asm:
+// COLUMN, so a lane holds one row of the result and runs of 4 columns (8-byte stores per limb).  The product of the first limbs has an
+// accumulator of its own: the small cross products, added to it, would cost it a rounding each (measured: that halves the error of
+// the whole iteration).  LDS: S stages of a KC-deep chunk of both operands, S - 1 of them requested ahead by LDS-DMA (from inline asm:
 // in front of a transposing read the compiler would wait for all requests); one barrier per chunk.
 //   OL_SYM : L R^T, symmetric: tiles on and above the diagonal, the mirrored tile is stored from an LDS transpose
 //   OL_RECT: L X, X of the next chain: the reduction runs down the rows of X, whose chunks are read transposed from LDS
@@ -338,7 +349,8 @@ struct OrthoLevel {
 // stay in VGPRs, and nothing may spill: one reload in the loop waits for every request under way.
 template <int T, int KC, int S, int WI, int WJ>
 __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho_product_kernel(char *__restrict__ ws, OrthoLevel lv) {
-  constexpr int WAVES = WI * WJ, SUB = KC / 32, STAGE = T * KC * 4, PIECES = T * SUB / 8 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = 144;
+  constexpr int WAVES = WI * WJ, STAGE = T * KC * OG_BYTES, PIECES = STAGE / 1024 / WAVES, FI = T / WI / 32, FJ = T / WJ / 32, TP = OG_LINE + 16;
+  static_assert(PIECES * WAVES * 1024 == STAGE, "whole requests of a wave");
   static_assert(S * 2 * STAGE >= WAVES * 32 * TP, "the exchange buffers of the epilogue lie in the stages");
   static_assert((S - 1) * 2 * PIECES < 64, "the range of s_waitcnt vmcnt");
   extern __shared__ __align__(1024) char smem[];
@@ -393,7 +405,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
   const char *e2 = job.e2 == OB_NONE ? nullptr : ortho_buffer(ws, g, job.e2, mat);
   // one fragment per wave: E1 and E2 are fetched behind the product's first requests
   constexpr bool EARLY = FI * FJ == 1;
-  og_h4 eh[EARLY ? 8 : 1], el[EARLY ? 8 : 1];
+  og_b4 el[EARLY ? 8 : 1][3];
   auto early = [&]() {
     if constexpr (EARLY) {
       const long at = og_at(M, (bi * WI + wi) * 32 + l31, (bj * WJ + wj) * 32 + lh * 4);
@@ -401,36 +413,35 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
       for (int q = 0; q < 8; ++q) {
         const char *e = q < 4 ? e1 : e2;
         if (e) {
-          const og_h4 *p = reinterpret_cast<const og_h4 *>(e + at + (q & 3) * 32);
-          eh[q] = p[0];
-          el[q] = p[2];
+#pragma unroll
+          for (int k = 0; k < 3; ++k) el[q][k] = *reinterpret_cast<const og_b4 *>(e + at + (q & 3) * 16 + k * 64);
         }
       }
     }
   };
   if (!lv.joining) {
-    // a piece = 8 lines of 128 bytes = one DMA request of a wave: [sub-chunk of 32][line], line = row of the tile; for X in
-    // OL_RECT / OL_LAST: [32 columns][row of the chunk].  Unit u of line r lies at u ^ (r / 2): 16 lanes reading 16 consecutive
-    // lines, or four lines of the 64-bit transposing reads, touch all 64 banks once
+    // a piece = 64 units of 16 bytes = one DMA request of a wave; a line = 12 units, [limb][8 columns] of a row of the tile; for X in
+    // OL_RECT / OL_LAST: [32 columns][row of the chunk].  The unit of columns q of line r lies at q ^ (r / 4): 16 lanes reading 16
+    // consecutive lines, or four lines of the 64-bit transposing reads, touch all 64 banks once
     const bool turned = type != OL_SYM;
-    const c8_i32x4 lrs = c8_rsrc_words(ortho_buffer(ws, g, job.l, mat), (unsigned)((long)M * K * 4));
-    const c8_i32x4 rrs = c8_rsrc_words(ortho_buffer(ws, g, job.r, mat), (unsigned)((long)M * (turned ? N : K) * 4));
+    const c8_i32x4 lrs = c8_rsrc_words(ortho_buffer(ws, g, job.l, mat), (unsigned)((long)M * K * OG_BYTES));
+    const c8_i32x4 rrs = c8_rsrc_words(ortho_buffer(ws, g, job.r, mat), (unsigned)((long)M * (turned ? N : K) * OG_BYTES));
     unsigned lo[PIECES], ro[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int line = (wave + WAVES * p) * 8 + (lane >> 3), sub = line / T, row = line % T, unit = ((lane & 7) ^ ((line >> 1) & 7)) * 16;
-      const int li = bi * T + row < M ? bi * T + row : M - 1;
-      lo[p] = (unsigned)((sub * M + li) * 128 + unit);
+      const int u = (wave + WAVES * p) * 64 + lane, line = u / 12, unit = ((u - line * 12) ^ ((line >> 2) & 3)) * 16;
+      const int li = bi * T + line < M ? bi * T + line : M - 1;
+      lo[p] = (unsigned)(li * OG_LINE + unit);
       if (!turned) {
-        const int rj = bj * T + row < M ? bj * T + row : M - 1;
-        ro[p] = (unsigned)((sub * M + rj) * 128 + unit);
+        const int rj = bj * T + line < M ? bj * T + line : M - 1;
+        ro[p] = (unsigned)(rj * OG_LINE + unit);
       } else {                                                            // T / 32 column chunks of KC rows each
         const int cc = line / KC, r = line % KC;
         const int c = bj * (T / 32) + cc < N / 32 ? bj * (T / 32) + cc : N / 32 - 1;
-        ro[p] = (unsigned)((c * (long)M + r) * 128 + unit);
+        ro[p] = (unsigned)((c * (long)M + r) * OG_LINE + unit);
       }
     }
-    const unsigned lstep = (unsigned)M * SUB * 128, rstep = turned ? KC * 128 : lstep, lds0 = c8_lds_addr(smem);
+    const unsigned lstep = (unsigned)M * OG_LINE, rstep = turned ? KC * OG_LINE : lstep, lds0 = c8_lds_addr(smem);
     auto stage = [&](int buf, int c) {
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
@@ -442,52 +453,51 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
     // last fragments are in registers, so its stage is free for chunk c + S, and chunk c + 1 has landed.  The chunks go round the
     // stages in a loop unrolled S times, so that a lane's LDS addresses are eight registers and constants, and the last chunk has code
     // of its own: where paths meet, the compiler would wait for every LDS read in flight.
-    static_assert(KC == 32, "two halves per chunk");
-    og_h8 lf[2][FI][2], rf[2][FJ][2];
+    static_assert(KC == 32, "two halves per chunk, lines of one chunk");
+    og_b8 lf[2][FI][3], rf[2][FJ][3];
     auto product = [&](auto turn) {
-      // lines of 32 columns: halves and limbs differ in bits of the unit; chunks of X: lane i of 16 points at 4 columns of row i / 4 and
-      // receives 4 rows of column i, the other 4 rows lie 512 bytes on
-      const char *la[2][2], *ra[2][2];
+      // lines of 32 columns: halves differ in bits of the unit, limbs by 64 bytes; chunks of X: lane i of 16 points at 4 columns of row
+      // i / 4 and receives 4 rows of column i
+      const char *la[2], *ra[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int unit = h * 4 + lh * 2 + q, li = wi * FI * 32 + l31, rj = wj * FJ * 32 + l31;
-          la[h][q] = smem + li * 128 + ((unit ^ ((li >> 1) & 7)) * 16);
-          if constexpr (!turn.value) {
-            ra[h][q] = smem + STAGE + rj * 128 + ((unit ^ ((rj >> 1) & 7)) * 16);
-          } else {                                               // [4 rows further][limb]
-            const int r = lh * 8 + ((lane & 15) >> 2) + h * 4, u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2 + q;
-            ra[h][q] = smem + STAGE + (wj * FJ * KC + r) * 128 + (lane & 1) * 8 + ((u ^ ((r >> 1) & 7)) * 16);
-          }
+      for (int h = 0; h < 2; ++h) {
+        const int unit = h * 2 + lh, li = wi * FI * 32 + l31, rj = wj * FJ * 32 + l31;
+        la[h] = smem + li * OG_LINE + ((unit ^ ((li >> 2) & 3)) * 16);
+        if constexpr (!turn.value) {
+          ra[h] = smem + STAGE + rj * OG_LINE + ((unit ^ ((rj >> 2) & 3)) * 16);
+        } else {                                                 // [4 rows further]
+          const int r = lh * 8 + ((lane & 15) >> 2) + h * 4, u = ((lane >> 4) & 1) * 2 + ((lane & 2) >> 1);
+          ra[h] = smem + STAGE + (wj * FJ * KC + r) * OG_LINE + (lane & 1) * 8 + ((u ^ ((r >> 2) & 3)) * 16);
         }
+      }
       auto load = [&](int h, int at) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < 3; ++q) {
 #pragma unroll
           for (int f = 0; f < FJ; ++f)
             if constexpr (!turn.value)
-              rf[h][f][q] = *reinterpret_cast<const og_h8 *>(ra[h][q] + at * 2 * STAGE + f * 4096);
+              rf[h][f][q] = *reinterpret_cast<const og_b8 *>(ra[h] + at * 2 * STAGE + f * 32 * OG_LINE + q * 64);
             else
-              rf[h][f][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)ra[0][q] + at * 2 * STAGE + f * KC * 128 + h * 2048,
-                                                                 (const unsigned char *)ra[1][q] + at * 2 * STAGE + f * KC * 128 + h * 2048));
+              rf[h][f][q] = c8_tr_frag((const unsigned char *)ra[0] + at * 2 * STAGE + (f * KC + h * 16) * OG_LINE + q * 64,
+                                       (const unsigned char *)ra[1] + at * 2 * STAGE + (f * KC + h * 16) * OG_LINE + q * 64);
 #pragma unroll
-          for (int f = 0; f < FI; ++f) lf[h][f][q] = *reinterpret_cast<const og_h8 *>(la[h][q] + at * 2 * STAGE + f * 4096);
+          for (int f = 0; f < FI; ++f) lf[h][f][q] = *reinterpret_cast<const og_b8 *>(la[h] + at * 2 * STAGE + f * 32 * OG_LINE + q * 64);
         }
       };
+      // limbs (r, l) of the products, the smallest first; 1 2, 2 1 and 2 2 are below 2^-26 of 0 0
       auto multiply = [&](int h) {
+        auto add = [&](int r, int l, og_f16v (&to)[FI][FJ]) {
 #pragma unroll
-        for (int i = 0; i < FI; ++i)
+          for (int i = 0; i < FI; ++i)
 #pragma unroll
-          for (int j = 0; j < FJ; ++j) acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[h][j][0], lf[h][i][1], acx[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < FI; ++i)
-#pragma unroll
-          for (int j = 0; j < FJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[h][j][0], lf[h][i][0], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < FI; ++i)
-#pragma unroll
-          for (int j = 0; j < FJ; ++j) acx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rf[h][j][1], lf[h][i][0], acx[i][j], 0, 0, 0);
+            for (int j = 0; j < FJ; ++j) to[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[h][j][r], lf[h][i][l], to[i][j], 0, 0, 0);
+        };
+        add(0, 2, acx);
+        add(2, 0, acx);
+        add(1, 1, acx);
+        add(0, 0, acc);
+        add(0, 1, acx);
+        add(1, 0, acx);
       };
       const int n = c1 - c0;
 #pragma unroll
@@ -564,17 +574,15 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
           }
   }
   auto stored = [&](int which, int q, int i, int j, float (&v)[4]) {     // 4 stored values of row i from column j on
-    og_h4 h, l;
     if constexpr (EARLY) {
-      h = eh[which * 4 + q];
-      l = el[which * 4 + q];
+      og_value(el[which * 4 + q], v);
     } else {
-      const og_h4 *p = reinterpret_cast<const og_h4 *>((which ? e2 : e1) + og_at(M, i, j));
-      h = p[0];
-      l = p[2];
-    }
+      const char *p = (which ? e2 : e1) + og_at(M, i, j);
+      og_b4 l[3];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (float)h[k] + (float)l[k];
+      for (int k = 0; k < 3; ++k) l[k] = *reinterpret_cast<const og_b4 *>(p + k * 64);
+      og_value(l, v);
+    }
   };
   const bool last = type == OL_LAST, mirrored = type == OL_SYM && bi != bj;
   const OrthoPtr ptr = ortho_ptr(lv.gs, g, mat, lv.mode == OM_BF16 ? 2 : 4);
@@ -589,7 +597,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
     for (int fj = 0; fj < FJ; ++fj) {
       const int i0 = bi * T + (wi * FI + fi) * 32, j0 = bj * T + (wj * FJ + fj) * 32, i = i0 + l31;
       if (i0 >= M || j0 >= cols) continue;                               // (T = 128 on an odd number of 64-row halves)
-      og_h4 hq[4], lq[4];
+      og_b4 lq[4][3];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int j = j0 + q * 8 + lh * 4;
@@ -607,15 +615,12 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
           for (int k = 0; k < 4; ++k) v[k] = fmaf(job.k2, x[k], v[k]);
         }
         if (!last) {
-          og_h4 h, l;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             if (i == j + k) v[k] += job.diag;
-          og_split(v, h, l);
-          *reinterpret_cast<og_h4 *>(tp + l31 * TP + q * 32 + lh * 8) = h;
-          *reinterpret_cast<og_h4 *>(tp + l31 * TP + q * 32 + 16 + lh * 8) = l;
-          hq[q] = h;
-          lq[q] = l;
+          og_split(v, lq[q]);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<og_b4 *>(tp + l31 * TP + k * 64 + q * 16 + lh * 8) = lq[q][k];
         } else if (i < m) {
           if (!tall && j + 4 <= nn && lv.mode != OM_BF16) {
             og_f4u *o = reinterpret_cast<og_f4u *>((float *)ptr.out + (long)i * nn + j);
@@ -637,32 +642,27 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
         }
       }
       if (!last) {
-        // 32 rows x 128 bytes of the result lie one behind the other: 16 bytes per lane, four full stores
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        char *o = out + og_at(M, i0, j0);
+        // 32 lines of the result lie one behind the other: 16 bytes per lane, six full stores
+        auto leave = [&](char *o) {
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int u = lane + s * 64;
-          *reinterpret_cast<og_h8 *>(o + u * 16) = *reinterpret_cast<const og_h8 *>(tp + (u >> 3) * TP + (u & 7) * 16);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          for (int s = 0; s < 6; ++s) {
+            const int u = lane + s * 64;
+            *reinterpret_cast<og_b8 *>(o + u * 16) = *reinterpret_cast<const og_b8 *>(tp + u / 12 * TP + u % 12 * 16);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        };
+        leave(out + og_at(M, i0, j0));
         if (mirrored) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              char *d = tp + (q * 8 + lh * 4 + k) * TP + (l31 >> 3) * 32 + (l31 & 7) * 2;
-              *reinterpret_cast<_Float16 *>(d) = hq[q][k];
-              *reinterpret_cast<_Float16 *>(d + 16) = lq[q][k];
-            }
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          char *m = out + og_at(M, j0, i0);
+              char *d = tp + (q * 8 + lh * 4 + k) * TP + (l31 >> 3) * 16 + (l31 & 7) * 2;
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const int u = lane + s * 64;
-            *reinterpret_cast<og_h8 *>(m + u * 16) = *reinterpret_cast<const og_h8 *>(tp + (u >> 3) * TP + (u & 7) * 16);
-          }
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+              for (int n = 0; n < 3; ++n) *reinterpret_cast<__bf16 *>(d + n * 64) = lq[q][n][k];
+            }
+          leave(out + og_at(M, j0, i0));
         }
       }
     }
@@ -683,35 +683,41 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
 // Panels of 1 or 2 chunks are as fast for one matrix and slower for several; 16 panels at most instead of 32 cost 20 x 8192 a third, 64
 // cost 64 x 4096 a quarter.
 #define ORTHO_SMALL_M 64
-#define ORTHO_SMALL_N 448      // columns that fit into LDS
+#define ORTHO_SMALL_N 320      // columns that fit into LDS (chunks are handled in pairs)
 #define ORTHO_WIDE 4           // narrowest panel, in chunks of 32 columns
 #define ORTHO_PANELS 32        // longest row of panels: every workgroup reads 16 KB of each
-struct OrthoSmallStep {
-  float gram, s0, s1, diag, x;      // factors of A; of A A, A and I in Q = a I + b A + c A A; of Q X
-};
 #define ORTHO_FEW 16           // pointers that travel in the kernels' arguments, without a launch that fills the table
 struct OrthoSmall {
   OrthoGroups gs;
   OrthoPtr few[ORTHO_FEW];          // read one per lane, as the groups are
-  OrthoSmallStep step[ORTHO_STEPS];
   OrthoMomentum mo;
-  int steps, mode;
-  float decay, eps, x0;
+  int steps;
+  float a, b, c;
+  float decay, eps;
 };
 
-// byte of 16-byte unit u of row r of a chunk of 64 rows x 32 columns in LDS
-__device__ __forceinline__ int og_unit(int r, int u) { return r * 128 + ((u ^ ((r >> 1) & 7)) << 4); }
+#define OG_CHUNK (64 * OG_LINE) // bytes of 64 rows x 32 columns in LDS
+// byte of columns 8 q ... 8 q + 7 of row r, one limb, in a chunk in LDS
+__device__ __forceinline__ int og_unit(int r, int q, int limb) { return r * OG_LINE + limb * 64 + ((q ^ ((r >> 2) & 3)) << 4); }
 // 8 columns of a row, half chunk `half`, one limb: a lane's MFMA operand
-__device__ __forceinline__ og_h8 og_frag(const char *chunk, int row, int half, int limb) {
-  return *reinterpret_cast<const og_h8 *>(chunk + og_unit(row, (half * 2 + ((threadIdx.x >> 5) & 1)) * 2 + limb));
+__device__ __forceinline__ og_b8 og_frag(const char *chunk, int row, int half, int limb) {
+  return *reinterpret_cast<const og_b8 *>(chunk + og_unit(row, half * 2 + ((threadIdx.x >> 5) & 1), limb));
 }
 // 4 values of a row from column 8 q + 4 (lane / 32) on
 __device__ __forceinline__ void og_put(char *chunk, int row, int q, const float (&v)[4]) {
-  const int lh = (threadIdx.x >> 5) & 1;
-  og_h4 h, l;
-  og_split(v, h, l);
-  *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2) + lh * 8) = h;
-  *reinterpret_cast<og_h4 *>(chunk + og_unit(row, q * 2 + 1) + lh * 8) = l;
+  og_b4 l[3];
+  og_split(v, l);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) *reinterpret_cast<og_b4 *>(chunk + og_unit(row, q, k) + ((threadIdx.x >> 5) & 1) * 8) = l[k];
+}
+// acc, acx += (limbs of y)(limbs of x)^T; the smallest first, 0 0 apart from the others as in ortho_product_kernel
+__device__ __forceinline__ void og_multiply(const og_b8 (&y)[3], const og_b8 (&x)[3], og_f16v &acc, og_f16v &acx) {
+  acx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], x[2], acx, 0, 0, 0);
+  acx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[2], x[0], acx, 0, 0, 0);
+  acx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[1], x[1], acx, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], x[0], acc, 0, 0, 0);
+  acx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[0], x[1], acx, 0, 0, 0);
+  acx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[1], x[0], acx, 0, 0, 0);
 }
 
 // A panel's elements, 256 threads, 64 columns x 16 per thread at a time; lanes run along the rows of G (TALL: along the short side).
@@ -730,20 +736,20 @@ struct OgWalk {
     so = TALL ? 4 * m : 4 * n;
     step = TALL ? 64 * m : 64;
     o = TALL ? (j0 + wave) * m + lane : wave * n + j0 + lane;
-    row = TALL ? lane * 128 + wave * 4 : (lane >> 5) * 8192 + wave * 128 + (lane & 3) * 4;
+    row = TALL ? lane * OG_LINE + wave * 4 : (lane >> 5) * OG_CHUNK + wave * OG_LINE + ((lane >> 2) & 1) * 64 + (lane & 3) * 4;
     count();
   }
   __device__ __forceinline__ void count() { valid = TALL ? (lane < m ? (left - wave + 3) >> 2 : 0) : lane < left ? (m - wave + 3) >> 2 : 0; }
   __device__ __forceinline__ void next() {
     left -= 64;
     o += step;
-    row += 2 * 8192;
+    row += 2 * OG_CHUNK;
     count();
   }
   __device__ __forceinline__ int at(int e) const { return e < valid ? o + e * so : -1; }      // -1: behind every buffer
   __device__ __forceinline__ int lds(int e) const {
-    if constexpr (TALL) return row + (e >> 3) * 8192 + (((e & 7) ^ ((lane >> 1) & 7)) << 4);
-    else return row + e * 512 + ((((lane & 31) >> 2) ^ ((wave >> 1) + 2 * (e & 3))) << 4);
+    if constexpr (TALL) return row + (e >> 3) * OG_CHUNK + (e & 1) * 64 + ((((e & 7) >> 1) ^ ((lane >> 2) & 3)) << 4);
+    else return row + e * 4 * OG_LINE + ((((lane & 31) >> 3) ^ (e & 3)) << 4);
   }
 };
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t og_buffer(void *p, int bytes) { return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00027000); }
@@ -756,7 +762,8 @@ __device__ __forceinline__ void og_set(__amdgpu_buffer_rsrc_t b, int o, float v)
   __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), b, o < 0 ? -1 : o * 4, 0, 0);
 }
 
-// G (Muon: the momentum, updated on the way) as f32 into the place of its limbs; returns the thread's sum of squares
+// G (Muon: the momentum, updated on the way) as f32 into the place of its first two limbs (columns 8 q ... 8 q + 3 | 8 q + 4 ... 8 q + 7);
+// returns the thread's sum of squares
 template <typename T, bool MUON, bool TALL>
 __device__ __forceinline__ double og_fetch(const OrthoGroup &g, int j0, int chunks, const OrthoPtr &ptr, const OrthoMomentum &mo, char *X) {
   const int size = g.rows * g.cols;
@@ -786,24 +793,22 @@ __device__ __forceinline__ double og_fetch(const OrthoGroup &g, int j0, int chun
   return sum;
 }
 
-// f32 into limbs in place: X0 = G / norm * scale.  The quotient is a power of two times a factor near the scale: no division per
-// element, and nothing overflows on the way for any norm.
+// f32 into limbs in place: X0 = G / norm
 template <int MT>
-__device__ __forceinline__ void og_limbs(char *X, int chunks, double norm, float scale) {
-  int ex;
-  const float f = (float)((double)scale / frexp(norm, &ex));
+__device__ __forceinline__ void og_limbs(char *X, int chunks, double norm) {
+  const OgUnit unit(norm);
   for (int t = threadIdx.x; t < chunks * 128 * MT; t += 256) {
     const int row = t & (32 * MT - 1), q = t / (32 * MT);
-    char *chunk = X + (q >> 2) * 8192, *p0 = chunk + og_unit(row, (q & 3) * 2), *p1 = chunk + og_unit(row, (q & 3) * 2 + 1);
-    const og_f4 x[2] = {*reinterpret_cast<og_f4 *>(p0), *reinterpret_cast<og_f4 *>(p1)};
-    og_h4 h[2], l[2];
+    char *p = X + (q >> 2) * OG_CHUNK + og_unit(row, q & 3, 0);
+    const og_f4 x[2] = {*reinterpret_cast<og_f4 *>(p), *reinterpret_cast<og_f4 *>(p + 64)};
+    og_b4 l[2][3];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float v[4] = {ldexpf(x[e][0], -ex) * f, ldexpf(x[e][1], -ex) * f, ldexpf(x[e][2], -ex) * f, ldexpf(x[e][3], -ex) * f};
-      og_split(v, h[e], l[e]);
+      const float v[4] = {unit(x[e][0]), unit(x[e][1]), unit(x[e][2]), unit(x[e][3])};
+      og_split(v, l[e]);
     }
-    *reinterpret_cast<og_h8 *>(p0) = og_join(h);
-    *reinterpret_cast<og_h8 *>(p1) = og_join(l);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<og_b8 *>(p + k * 64) = og_join(l[0][k], l[1][k]);
   }
 }
 
@@ -828,30 +833,26 @@ __device__ __forceinline__ void og_deliver(const OrthoGroup &g, int j0, int chun
   }
 }
 
-// this wave's 32 x 32 tile of Y Y^T, Y = `chunks` chunks at `in`, each chunk's operands requested a chunk ahead; small cross products
-// apart from hi hi, as in ortho_product_kernel
+// this wave's 32 x 32 tile of Y Y^T, Y = `chunks` chunks at `in`, each chunk's operands requested a chunk ahead
 template <bool DIAG>
 __device__ __forceinline__ void og_square_tile(const char *in, int chunks, int ti, int tj, float (&v)[16]) {
   const int l31 = threadIdx.x & 31;
   og_f16v acc, acx;
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = acx[e] = 0.f;
-  og_h8 f[2][4], g[2][4];
+  og_b8 f[2][2][3], g[2][2][3];
   auto load = [&](int c, int b) {
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      f[b][h] = og_frag(in + c * 8192, ti + l31, h >> 1, h & 1);
-      if constexpr (!DIAG) g[b][h] = og_frag(in + c * 8192, tj + l31, h >> 1, h & 1);
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        f[b][h][k] = og_frag(in + c * OG_CHUNK, ti + l31, h, k);
+        if constexpr (!DIAG) g[b][h][k] = og_frag(in + c * OG_CHUNK, tj + l31, h, k);
+      }
   };
   auto multiply = [&](int b) {
 #pragma unroll
-    for (int h = 0; h < 4; h += 2) {
-      const og_h8 jh = DIAG ? f[b][h] : g[b][h], jl = DIAG ? f[b][h + 1] : g[b][h + 1];
-      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, f[b][h + 1], acx, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(jh, f[b][h], acc, 0, 0, 0);
-      acx = __builtin_amdgcn_mfma_f32_32x32x16_f16(jl, f[b][h], acx, 0, 0, 0);
-    }
+    for (int h = 0; h < 2; ++h) og_multiply(DIAG ? f[b][h] : g[b][h], f[b][h], acc, acx);
   };
   load(0, 0);
   for (int c = 0;;) {
@@ -870,49 +871,46 @@ __device__ __forceinline__ void og_square(const char *in, int chunks, int ti, in
   else og_square_tile<false>(in, chunks, ti, tj, v);
 }
 
-// A from the wave's tile of it (v, unscaled), then Q; a barrier in between, none behind
-__device__ __forceinline__ void og_make_q(char *A, char *Q, int tiles, int ti, int tj, float (&v)[16], const OrthoSmallStep &st) {
+// Q = a I + b A + c A A from the wave's tile v of A; A passes through Q's place.  Two barriers in between, none behind
+__device__ __forceinline__ void og_make_q(char *Q, int tiles, int ti, int tj, const float (&v)[16], const OrthoSmall &co) {
   const int l31 = threadIdx.x & 31, lh = (threadIdx.x >> 5) & 1;
   const bool mine = tiles > 1 || threadIdx.x < 64;
-  if (mine) {
+  auto put = [&](const float (&t)[16]) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float w[4] = {v[q * 4] *= st.gram, v[q * 4 + 1] *= st.gram, v[q * 4 + 2] *= st.gram, v[q * 4 + 3] *= st.gram};
-      og_put(A + (tj >> 5) * 8192, ti + l31, q, w);
+      const float w[4] = {t[q * 4], t[q * 4 + 1], t[q * 4 + 2], t[q * 4 + 3]};
+      og_put(Q + (tj >> 5) * OG_CHUNK, ti + l31, q, w);
     }
-  }
+  };
+  if (mine) put(v);
+  __syncthreads();
+  float p[16];
+  if (mine) og_square(Q, tiles, ti, tj, p);
   __syncthreads();
   if (mine) {
-    float p[16];
-    og_square(A, tiles, ti, tj, p);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = fmaf(st.s0, p[q * 4 + e], fmaf(st.s1, v[q * 4 + e], ti + l31 == tj + q * 8 + lh * 4 + e ? st.diag : 0.f));
-      og_put(Q + (tj >> 5) * 8192, ti + l31, q, w);
-    }
+    for (int e = 0; e < 16; ++e) p[e] = fmaf(co.c, p[e], fmaf(co.b, v[e], ti + l31 == tj + (e >> 2) * 8 + lh * 4 + (e & 3) ? co.a : 0.f));
+    put(p);
   }
 }
 
-// X <- Q X, a wave's chunks one after the other (so a result may go where the chunk was read).  Begins with a barrier, in front of
-// which the first chunk is requested (transposing reads).  `last`: f32 instead of limbs.
+// X <- factor Q X, a wave's chunks one after the other (so a result may go where the chunk was read).  Begins with a barrier, in front
+// of which the first chunk is requested (transposing reads).  `last`: f32 instead of limbs.
 template <int MT>
 __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, float factor, bool last) {
   const int lane = threadIdx.x & 63, l31 = lane & 31, lh = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  og_h8 x[2 * MT][2], qf[2 * MT][MT][2];
+  og_b8 x[2 * MT][3], qf[2 * MT][MT][3];
   auto load = [&](const char *chunk) {
 #pragma unroll
     for (int h = 0; h < 2 * MT; ++h) {
-      const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 4 + ((lane & 2) >> 1) * 2;
+      const int r = h * 16 + lh * 8 + ((lane & 15) >> 2), u = ((lane >> 4) & 1) * 2 + ((lane & 2) >> 1);
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        x[h][q] = __builtin_bit_cast(og_h8, c8_tr_frag((const unsigned char *)chunk + og_unit(r, u + q) + (lane & 1) * 8,
-                                                       (const unsigned char *)chunk + og_unit(r + 4, u + q) + (lane & 1) * 8));
+      for (int k = 0; k < 3; ++k)
+        x[h][k] = c8_tr_frag((const unsigned char *)chunk + og_unit(r, u, k) + (lane & 1) * 8,
+                             (const unsigned char *)chunk + og_unit(r + 4, u, k) + (lane & 1) * 8);
     }
   };
-  if (wave < chunks) load(X + wave * 8192);
+  if (wave < chunks) load(X + wave * OG_CHUNK);
   __syncthreads();
   if (wave >= chunks) return;
 #pragma unroll
@@ -920,9 +918,9 @@ __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, flo
 #pragma unroll
     for (int f = 0; f < MT; ++f)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) qf[h][f][q] = og_frag(Q + (h >> 1) * 8192, f * 32 + l31, h & 1, q);
+      for (int k = 0; k < 3; ++k) qf[h][f][k] = og_frag(Q + (h >> 1) * OG_CHUNK, f * 32 + l31, h & 1, k);
   for (int ch = wave; ch < chunks; ch += 4) {
-    char *chunk = X + ch * 8192;
+    char *chunk = X + ch * OG_CHUNK;
     og_f16v acc[MT], acx[MT];
 #pragma unroll
     for (int f = 0; f < MT; ++f)
@@ -931,12 +929,8 @@ __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, flo
 #pragma unroll
     for (int h = 0; h < 2 * MT; ++h)
 #pragma unroll
-      for (int f = 0; f < MT; ++f) {
-        acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][0], qf[h][f][1], acx[f], 0, 0, 0);
-        acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][0], qf[h][f][0], acc[f], 0, 0, 0);
-        acx[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][1], qf[h][f][0], acx[f], 0, 0, 0);
-      }
-    if (ch + 4 < chunks) load(chunk + 4 * 8192);
+      for (int f = 0; f < MT; ++f) og_multiply(x[h], qf[h][f], acc[f], acx[f]);
+    if (ch + 4 < chunks) load(chunk + 4 * OG_CHUNK);
 #pragma unroll
     for (int f = 0; f < MT; ++f)
 #pragma unroll
@@ -951,7 +945,7 @@ __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, flo
         }
     };
     if (last)
-      each([&](int i, int q, const float(&v)[4]) { *reinterpret_cast<og_f4 *>(chunk + og_unit(i, q * 2 + lh)) = og_f4{v[0], v[1], v[2], v[3]}; });
+      each([&](int i, int q, const float(&v)[4]) { *reinterpret_cast<og_f4 *>(chunk + og_unit(i, q, lh)) = og_f4{v[0], v[1], v[2], v[3]}; });
     else
       each([&](int i, int q, const float(&v)[4]) { og_put(chunk, i, q, v); });
   }
@@ -987,18 +981,17 @@ __device__ __forceinline__ OrthoPtr og_small_ptr(const OrthoSmall &c, const Orth
 template <typename T, bool MUON, int MT>
 __device__ __forceinline__ void ortho_alone(const OrthoSmall &c, const OrthoGroup &g, const OrthoPtr &ptr, char *smem, double *red) {
   const int chunks = (og_long(g) + 31) / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  char *A = smem, *Q = smem + 16384, *X = smem + 32768;
+  char *Q = smem, *X = smem + 2 * OG_CHUNK;
   const bool tall = g.rows > g.cols;
   const double sum = tall ? og_fetch<T, MUON, true>(g, 0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false>(g, 0, chunks, ptr, c.mo, X);
-  og_limbs<MT>(X, chunks, sqrt(og_block_sum(sum, red)) + (double)c.eps, c.x0);
+  og_limbs<MT>(X, chunks, sqrt(og_block_sum(sum, red)) + (double)c.eps);
   const int ti = MT > 1 ? (wave >> 1) * 32 : 0, tj = MT > 1 ? (wave & 1) * 32 : 0;          // this wave's tile of A and Q
   for (int k = 0; k < c.steps; ++k) {
-    const OrthoSmallStep st = c.step[k];
     float v[16];
     __syncthreads();
     if (MT > 1 || wave == 0) og_square(X, chunks, ti, tj, v);
-    og_make_q(A, Q, MT, ti, tj, v, st);
-    og_apply<MT>(Q, X, chunks, st.x, k + 1 == c.steps);
+    og_make_q(Q, MT, ti, tj, v, c);
+    og_apply<MT>(Q, X, chunks, 1.f, k + 1 == c.steps);
   }
   __syncthreads();
   if (tall) og_deliver<T, MUON, true>(g, 0, chunks, ptr, X, c.decay);
@@ -1026,14 +1019,14 @@ template <typename T, bool MUON, int MT>
 __device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGroup &g, char *ws, double *sums, int k, char *smem, double *red) {
   const int panels = og_panels(g), wide = g.jobs, mat = og_div(blockIdx.x - g.first, panels), pan = blockIdx.x - g.first - mat * panels;
   const int all = (og_long(g) + 31) / 32, chunks = all - pan * wide < wide ? all - pan * wide : wide;
-  char *A = smem, *Q = smem + 16384, *X = smem + 32768;
+  char *Q = smem, *X = smem + 2 * OG_CHUNK;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ti = MT > 1 ? (wave >> 1) * 32 : 0, tj = MT > 1 ? (wave & 1) * 32 : 0;
   const bool square = MT > 1 || wave == 0;
   const OrthoPtr ptr = og_small_ptr(c, g, mat, sizeof(T));
   const bool tall = g.rows > g.cols;
   const int j0 = pan * wide * 32;
-  char *mine = ws + (size_t)g.x_off * 256 + ((size_t)mat * all + pan * wide) * 8192;
+  char *mine = ws + (size_t)g.x_off * 256 + ((size_t)mat * all + pan * wide) * OG_CHUNK;
   og_f4 *share = reinterpret_cast<og_f4 *>(ws + (size_t)g.p_off * 256);                       // [set][mat][panel][q][thread]
   const size_t set = (size_t)g.count * panels * 1024;
   float v[16];
@@ -1043,11 +1036,10 @@ __device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGrou
     const double part = tall ? og_fetch<T, MUON, true>(g, j0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false>(g, j0, chunks, ptr, c.mo, X);
     const double sum = og_block_sum(part, red);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
-    og_limbs<MT>(X, chunks, sum == 0. ? 1. : sqrt(sum), c.x0);
+    og_limbs<MT>(X, chunks, sum == 0. ? 1. : sqrt(sum));
   } else {
-    for (int t = threadIdx.x; t < chunks * 512; t += 256)
-      reinterpret_cast<og_h8 *>(X)[t] = reinterpret_cast<const og_h8 *>(mine)[t];
-    const OrthoSmallStep st = c.step[k - 1];
+    for (int t = threadIdx.x; t < chunks * (OG_CHUNK / 16); t += 256)
+      reinterpret_cast<og_b8 *>(X)[t] = reinterpret_cast<const og_b8 *>(mine)[t];
     const og_f4 *p = share + ((k - 1) & 1) * set + (size_t)mat * panels * 1024 + threadIdx.x;
     float own = 1.f;
     float *weight = reinterpret_cast<float *>(red + 16);
@@ -1076,8 +1068,8 @@ __device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGrou
     };
     if (square && k == 1) gather([&](int z) { return weight[z]; });
     else if (square) gather([](int) { return 1.f; });
-    og_make_q(A, Q, MT, ti, tj, v, st);
-    og_apply<MT>(Q, X, chunks, st.x * own, k == c.steps);
+    og_make_q(Q, MT, ti, tj, v, c);
+    og_apply<MT>(Q, X, chunks, own, k == c.steps);
   }
   __syncthreads();
   if (k == c.steps) {
@@ -1091,7 +1083,7 @@ __device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGrou
 #pragma unroll
     for (int q = 0; q < 4; ++q) o[q * 256] = og_f4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
   }
-  for (int t = threadIdx.x; t < chunks * 512; t += 256) reinterpret_cast<og_h8 *>(mine)[t] = reinterpret_cast<const og_h8 *>(X)[t];
+  for (int t = threadIdx.x; t < chunks * (OG_CHUNK / 16); t += 256) reinterpret_cast<og_b8 *>(mine)[t] = reinterpret_cast<const og_b8 *>(X)[t];
 }
 
 template <typename T, bool MUON>
@@ -1128,56 +1120,32 @@ static int ortho_chain(const OrthoGroup &g, long tiles) {
   return M < 256 || N < 4 * M ? 2 : 3;
 }
 
-// Bounds of the matrices' spectral norms (hence of their entries) along the iteration: every one of them is a polynomial of
-// X0's singular values, which lie in [0, 1].  The scales that put them into the range of f16 limbs: X before and behind a chain,
-// A, S, T = A P and R at its steps, Q = a^n I + R at its end (s for a chain of one step).
-struct OrthoScale {
-  float x[2], a[ORTHO_CHAINS], s[ORTHO_CHAINS], t[ORTHO_CHAINS], r[ORTHO_CHAINS], q;
-};
+// Coefficients that let a singular value of [0, 1] grow out of hand are refused: what a chain computes of it would pass the range of
+// f32, and its rounding would drown the others.  One chain of n steps from the singular values sv, which are advanced to those
+// behind the chain; every matrix of the chain (X, A, S, T = A P, R, Q = a^n I + R) has polynomials of them as singular values.
 #define ORTHO_SAMPLES 257
 #define ORTHO_GROWTH 1e4
-static bool ortho_scale_of(double bound, float *scale) {
-  if (!(bound <= ORTHO_GROWTH)) return false;
-  if (bound < 1e-6) bound = 1e-6;
-  *scale = (float)exp2(floor(log2(16384. / bound)));     // a factor of 4 below the largest f16: rounding, and between the samples
-  return true;
-}
-// one chain of n steps from the singular values sv (advanced to those behind the chain).  False if the coefficients let the
-// iteration grow out of hand (or are not finite).
-static bool ortho_bounds(double *sv, int n, const OrthoCall &c, OrthoScale *o) {
-  double r[ORTHO_SAMPLES], lam[ORTHO_SAMPLES], most = 0.;
+static bool ortho_bounded(double *sv, int n, const OrthoCall &c) {
+  bool ok = true;
   for (int i = 0; i < ORTHO_SAMPLES; ++i) {
-    lam[i] = sv[i] * sv[i];
-    most = fmax(most, fabs(sv[i]));
-    if (!isfinite(sv[i])) return false;
-  }
-  if (!ortho_scale_of(most, &o->x[0])) return false;
-  double an = 1.;
-  for (int k = 0; k < n; ++k) {
-    double ma = 0., ms = 0., mt = 0., mr = 0.;
-    for (int i = 0; i < ORTHO_SAMPLES; ++i) {
-      const double A = lam[i], S = c.b * A + c.c * A * A, P = c.a + S;
-      r[i] = k ? c.a * r[i] + an * S + r[i] * S : S;
-      lam[i] = A * P * P;
-      if (!isfinite(lam[i]) || !isfinite(r[i])) return false;
-      ma = fmax(ma, fabs(A));
-      ms = fmax(ms, fabs(S));
-      mt = fmax(mt, fabs(A * P));
-      mr = fmax(mr, fabs(r[i]));
+    auto see = [&ok](double v) { ok = ok && fabs(v) <= ORTHO_GROWTH; };    // (false for a NaN)
+    double lam = sv[i] * sv[i], r = 0., an = 1.;
+    see(sv[i]);
+    for (int k = 0; k < n; ++k) {
+      const double A = lam, S = c.b * A + c.c * A * A, P = c.a + S;
+      r = k ? c.a * r + an * S + r * S : S;
+      lam = A * P * P;
+      see(A);
+      see(S);
+      see(A * P);
+      see(r);
+      an *= c.a;
     }
-    if (!ortho_scale_of(ma, &o->a[k]) || !ortho_scale_of(ms, &o->s[k]) || !ortho_scale_of(mt, &o->t[k]) || !ortho_scale_of(mr, &o->r[k]))
-      return false;
-    an *= c.a;
+    see(an + r);
+    sv[i] *= an + r;
+    see(sv[i]);
   }
-  double mq = 0.;
-  most = 0.;
-  for (int i = 0; i < ORTHO_SAMPLES; ++i) {
-    mq = fmax(mq, fabs(an + r[i]));
-    sv[i] *= an + r[i];
-    if (!isfinite(sv[i])) return false;
-    most = fmax(most, fabs(sv[i]));
-  }
-  return ortho_scale_of(mq, &o->q) && ortho_scale_of(most, &o->x[1]);
+  return ok;
 }
 
 // the products of one chain length, in order
@@ -1187,7 +1155,6 @@ struct OrthoPlan {
     int jobs, type;
   } level[3 * ORTHO_STEPS + ORTHO_STEPS];
   int levels;                       // 0: not asked for yet
-  float x0;                         // scale of X0
 };
 
 static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
@@ -1202,32 +1169,25 @@ static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
     p->level[p->levels].jobs = 1;
     p->level[p->levels++].job[0] = job;
   };
-  OrthoScale sc;
   for (int left = c.steps, set = 0; left > 0; set ^= 1) {
     const int chain = left < most ? left : most;
-    if (!ortho_bounds(sv, chain, c, &sc)) return false;
-    if (left == c.steps) p->x0 = sc.x[0];
+    if (!ortho_bounded(sv, chain, c)) return false;
     const int x = set ? OB_X1 : OB_X0;
-    add(OL_SYM, OrthoJob{x, x, OB_NONE, OB_NONE, OB_A, sc.a[0] / (sc.x[0] * sc.x[0]), 0.f, 0.f, 0.f});
+    add(OL_SYM, OrthoJob{x, x, OB_NONE, OB_NONE, OB_A, 1.f, 0.f, 0.f, 0.f});
     int r = OB_R0;                                                         // R of the first step is its S
-    float rs = sc.s[0], an = c.a;                                          // R's scale; a^k
+    float an = c.a;                                                        // a^k
     for (int k = 0; k < chain; ++k) {
       const bool more = k + 1 < chain;
-      const float sa = sc.a[k], ss = k || more ? sc.s[k] : sc.q;
       const int s = k ? OB_S : OB_R0;
       // S = b A + c A A (the whole chain's Q = a I + S if it is one step)
-      add(OL_SYM, OrthoJob{OB_A, OB_A, OB_A, OB_NONE, s, c.c * ss / (sa * sa), c.b * ss / sa, 0.f, k || more ? 0.f : an * ss});
-      if (!k && !more) rs = ss;
+      add(OL_SYM, OrthoJob{OB_A, OB_A, OB_A, OB_NONE, s, c.c, c.b, 0.f, k || more ? 0.f : an});
       OrthoJob todo[2];
       int jobs = 0;
-      if (more)                                                                                                    // T = a A + A S
-        todo[jobs++] = OrthoJob{OB_A, s, OB_A, OB_NONE, OB_T, sc.t[k] / (sa * ss), c.a * sc.t[k] / sa, 0.f, 0.f};
+      if (more) todo[jobs++] = OrthoJob{OB_A, s, OB_A, OB_NONE, OB_T, 1.f, c.a, 0.f, 0.f};                         // T = a A + A S
       if (k) {                                                                            // R = a R + a^k S + R S (+ a^(k+1) I: Q)
         const int to = r == OB_R0 ? OB_R1 : OB_R0;
-        const float sr = more ? sc.r[k] : sc.q;
-        todo[jobs++] = OrthoJob{r, s, r, s, to, sr / (rs * ss), c.a * sr / rs, an * sr / ss, more ? 0.f : an * c.a * sr};
+        todo[jobs++] = OrthoJob{r, s, r, s, to, 1.f, c.a, an, more ? 0.f : an * c.a};
         r = to;
-        rs = sr;
         an *= c.a;
       }
       if (jobs) {
@@ -1235,12 +1195,10 @@ static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
         p->level[p->levels - 1].job[1] = todo[1];
         p->level[p->levels - 1].jobs = jobs;
       }
-      if (more)                                                                                                    // A = a T + T S
-        add(OL_SYM, OrthoJob{OB_T, s, OB_T, OB_NONE, OB_A, sc.a[k + 1] / (sc.t[k] * ss), c.a * sc.a[k + 1] / sc.t[k], 0.f, 0.f});
+      if (more) add(OL_SYM, OrthoJob{OB_T, s, OB_T, OB_NONE, OB_A, 1.f, c.a, 0.f, 0.f});                           // A = a T + T S
     }
     left -= chain;
-    const float to = left > 0 ? sc.x[1] : 1.f;                                                                     // X = Q X
-    add(left > 0 ? OL_RECT : OL_LAST, OrthoJob{r, x, OB_NONE, OB_NONE, set ? OB_X0 : OB_X1, to / (rs * sc.x[0]), 0.f, 0.f, 0.f});
+    add(left > 0 ? OL_RECT : OL_LAST, OrthoJob{r, x, OB_NONE, OB_NONE, set ? OB_X0 : OB_X1, 1.f, 0.f, 0.f, 0.f});  // X = Q X
   }
   return true;
 }
@@ -1311,7 +1269,7 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
     at = lo.sums + align_up(blocks * sizeof(double), 256);
     for (int i = 0; i < n; ++i) {
       g[i].x_off = (unsigned)(at / 256);
-      at += (size_t)g[i].count * ((og_long(g[i]) + 31) / 32) * 8192;
+      at += (size_t)g[i].count * ((og_long(g[i]) + 31) / 32) * OG_CHUNK;
       g[i].p_off = (unsigned)(at / 256);
       at += (size_t)g[i].count * og_panels(g[i]) * 2 * 16384;
     }
@@ -1329,9 +1287,9 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
   for (int i = 0; i < n; ++i) {
     const size_t M = og_pad(og_short(g[i])), N = og_pad(og_long(g[i]));
     g[i].x_off = (unsigned)(at / 256);
-    at += M * N * 4 * g[i].count * (steps > lo.chain[i] ? 2 : 1);        // multiples of 64 x 64 x 4 bytes
+    at += M * N * OG_BYTES * g[i].count * (steps > lo.chain[i] ? 2 : 1);  // multiples of 64 x 64 x 6 bytes
     g[i].s_off = (unsigned)(at / 256);
-    at += M * M * 4 * g[i].count * OB_SMALL;
+    at += M * M * OG_BYTES * g[i].count * OB_SMALL;
     g[i].p_off = (unsigned)(at / 256);
     lo.kz[i] = ortho_kz((int)N, (long)g[i].count * og_tiles(g[i], OL_SYM, 64), tiles);
     if (lo.kz[i] > 1) at += (size_t)lo.kz[i] * g[i].count * og_tiles(g[i], OL_SYM, 64) * 64 * 64 * 4;
@@ -1342,7 +1300,7 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
 
 template <int T, int KC, int S, int WI, int WJ>
 static int ortho_launch(char *ws, const OrthoLevel &lv, int blocks, hipStream_t st) {
-  const int lds = S * 2 * T * KC * 4;
+  const int lds = S * 2 * T * KC * OG_BYTES;
   if (const int rc = lds_optin(reinterpret_cast<const void *>(&ortho_product_kernel<T, KC, S, WI, WJ>), lds, "ortho_product_kernel")) return rc;
   hipLaunchKernelGGL((ortho_product_kernel<T, KC, S, WI, WJ>), dim3(blocks), dim3(WI * WJ * 64), lds, st, ws, lv);
   return 0;
@@ -1354,7 +1312,6 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
   const OrthoLayout lo = ortho_layout(g, n, c.steps);
   double *sums = (double *)(ws + lo.sums);
   int levels = 0;
-  const float x0 = plan[lo.chain[0] - 1].x0;                             // (the same for every chain length)
   for (int i = 0; i < n; ++i)
     if (plan[lo.chain[i] - 1].levels > levels) levels = plan[lo.chain[i] - 1].levels;
   const bool few = (lo.small || lo.panels) && nptr <= ORTHO_FEW;
@@ -1382,10 +1339,11 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     if (few && nptr) memcpy(sm.few, ptrs, nptr * sizeof(OrthoPtr));
     sm.mo = c.mo;
     sm.steps = c.steps;
-    sm.mode = c.mode;
+    sm.a = c.a;
+    sm.b = c.b;
+    sm.c = c.c;
     sm.decay = c.decay;
     sm.eps = c.eps;
-    sm.x0 = x0;
     int blocks = 0, most = 0;                                            // most: chunks that a workgroup keeps in LDS
     for (int i = 0; i < n; ++i) {
       const int chunks = (og_long(g[i]) + 31) / 32, kept = lo.panels && g[i].jobs < chunks ? g[i].jobs : chunks;
@@ -1393,15 +1351,11 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
       blocks += lo.panels ? g[i].count * og_panels(g[i]) : g[i].count;
       if (kept > most) most = kept;
     }
-    for (int k = 0; k < c.steps; ++k) {
-      const OrthoJob *a = plan[0].level[3 * k].job, *q = plan[0].level[3 * k + 1].job, *x = plan[0].level[3 * k + 2].job;
-      sm.step[k] = OrthoSmallStep{a->k0, q->k0, q->k1, q->diag, x->k0};
-    }
-    const int lds = 32768 + (most + 1) / 2 * 16384;                      // (og_fetch's padding: an even number of chunks)
+    const int lds = 2 * OG_CHUNK + (most + 1) / 2 * 2 * OG_CHUNK;         // (og_fetch's padding: an even number of chunks)
 #define ORTHO_SMALL(T, MUON)                                                                                                            \
   do {                                                                                                                                  \
     const void *fn = lo.small ? reinterpret_cast<const void *>(&ortho_small_kernel<T, MUON>) : reinterpret_cast<const void *>(&ortho_panel_kernel<T, MUON>); \
-    if (const int rc = lds_optin(fn, 32768 + ORTHO_SMALL_N / 32 * 8192, "ortho_small_kernel")) return rc;                               \
+    if (const int rc = lds_optin(fn, (2 + ORTHO_SMALL_N / 32) * OG_CHUNK, "ortho_small_kernel")) return rc;                               \
     if (lo.small) {                                                                                                                     \
       hipLaunchKernelGGL((ortho_small_kernel<T, MUON>), dim3(blocks), dim3(256), lds, st, sm);                                          \
     } else {                                                                                                                            \
@@ -1421,7 +1375,7 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
 #define ORTHO_PRE(T, MUON)                                                                                                            \
   do {                                                                                                                                \
     hipLaunchKernelGGL((ortho_norm_kernel<T, MUON>), dim3(lo.norm_blocks), dim3(256), 0, st, lv.gs, sums, c.mo);                      \
-    hipLaunchKernelGGL((ortho_split_kernel<T, MUON>), dim3(lo.split_blocks), dim3(256), 0, st, split, ws, sums, c.mo, c.eps, x0);     \
+    hipLaunchKernelGGL((ortho_split_kernel<T, MUON>), dim3(lo.split_blocks), dim3(256), 0, st, split, ws, sums, c.mo, c.eps);         \
   } while (0)
   if (c.mode == OM_MUON) ORTHO_PRE(float, true);
   else if (!c.bf16) ORTHO_PRE(float, false);
@@ -1511,7 +1465,7 @@ static int ortho_check(const char *what, OrthoGroup *g, int n, const OrthoCall &
   const OrthoLayout lo = ortho_layout(g, n, c.steps);
   for (int i = 0; i < n; ++i) {
     OrthoPlan *p = plan + lo.chain[i] - 1;
-    LSPS_CHECK_ARG(p->levels || ortho_plan(p, lo.chain[i], c), "%s: the iteration with (%g, %g, %g) leaves the range of its 16-bit limbs on [0, 1]",
+    LSPS_CHECK_ARG(p->levels || ortho_plan(p, lo.chain[i], c), "%s: the iteration with (%g, %g, %g) grows out of bounds on [0, 1]",
                    what, (double)c.a, (double)c.b, (double)c.c);
   }
   LSPS_CHECK_ARG(!((uintptr_t)ws & 15), "%s: the workspace is not 16-byte aligned", what);

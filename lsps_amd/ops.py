@@ -1877,7 +1877,8 @@ def _ints(what, *values):
 def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """Newton-Schulz iterate of the matrices [..., rows, cols] of `g` (float32 or bfloat16; the same type comes back): singular vectors
     kept, singular values driven towards 1 (csrc/orthogonal.hip).  X = G / (|G|_F + eps), then `steps` times
-    X <- a X + (b A + c A^2) X, A = X X^T on the shorter side.  Float32-class arithmetic for either type.  No backward pass."""
+    X <- a X + (b A + c A^2) X, A = X X^T on the shorter side.  Arithmetic is float32 for either type, also for rows and columns far
+    below the others.  No backward pass."""
     if not isinstance(g, torch.Tensor) or g.dim() < 2:
         raise _lib.LspsHipError("newton_schulz: matrices [..., rows, cols] expected")
     if g.dtype not in _DTYPES:
