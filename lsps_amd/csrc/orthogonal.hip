@@ -15,8 +15,8 @@
 // their own, so that rows and columns far below the others (1e-9 and less) keep the relative accuracy they have in f32 arithmetic;
 // they grow by `a` a step and are as large as the others in the end.  (Two f16 limbs under one scale per matrix need half the
 // MFMAs, but are good for 22 bits down to 1e-5 of the norm only: rows of 1e-8 were off by 4 %.)  A product is six
-// v_mfma_f32_32x32x16_bf16 with f32 accumulation (limbs 0 0, 0 1, 1 0, 1 1, 0 2, 2 0; the dropped ones are below 2^-26 of it): 1.3 x
-// the rate of the f32 MFMAs.
+// v_mfma_f32_32x32x16_bf16 with f32 accumulation (limbs 0 0, 0 1, 1 0, 1 1, 0 2, 2 0; the dropped ones are at most
+// 2^-24 of it, half a step of f32): 1.3 x the rate of the f32 MFMAs.
 // Layout of a matrix with R rows: [column / 32][R][limb][(column % 32) / 8][8], rows and columns padded with zeros to multiples of 64:
 // a 32-deep chunk of a row is one line of 192 bytes and the rows of a chunk follow each other, so that a tile's chunk is one
 // contiguous run.  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.  X is kept one way round only:
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
           for (int f = 0; f < FI; ++f) lf[h][f][q] = *reinterpret_cast<const og_b8 *>(la[h] + at * 2 * STAGE + f * 32 * OG_LINE + q * 64);
         }
       };
-      // limbs (r, l) of the products, the smallest first; 1 2, 2 1 and 2 2 are below 2^-26 of 0 0
+      // limbs (r, l) of the products, the smallest first; 1 2, 2 1 and 2 2 are at most 2^-24 of the product
       auto multiply = [&](int h) {
         auto add = [&](int r, int l, og_f16v (&to)[FI][FJ]) {
 #pragma unroll

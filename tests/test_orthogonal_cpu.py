@@ -31,5 +31,6 @@ def test_six_products_make_one():
     x, y = [t[keep].double() for t in limbs(v)], [t[keep].double() for t in limbs(w)]
     got = x[0] * y[0] + x[0] * y[1] + x[1] * y[0] + x[1] * y[1] + x[0] * y[2] + x[2] * y[0]
     want = v[keep].double() * w[keep].double()
-    # dropped: 1 2, 2 1 and 2 2; a limb is half a step of the one before, 2^-9 and 2^-18 of the value's power of two, at most
-    assert bool(((got - want).abs() <= (2 * 2.0 ** -27 + 2.0 ** -36) * want.abs()).all())
+    # v = m 2^e, 1 <= m < 2: the first limb leaves half a step of 8 bits, |limb 1| <= 2^(e - 8); limb 1 is below that power of two or is
+    # exactly it, so it leaves |limb 2| <= 2^(e - 17).  Dropped are 1 2, 2 1 and 2 2: at most 2 * 2^-25 + 2^-34 of the product
+    assert bool(((got - want).abs() <= (2.0 ** -24 + 2.0 ** -34) * want.abs()).all())
