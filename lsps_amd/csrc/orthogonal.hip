@@ -22,7 +22,9 @@
 // contiguous run.  LDS-DMA copies it in 16-byte units whose source addresses carry the bank swizzle.  X is kept one way round only:
 // Q X reads it transposed from LDS (28 x 256 x 2304 with an earlier loop on two limbs: 407 us, 451 with X^T beside X).
 //
-// Times (MI355X): 28 x 256 x 2304 450 us, the generator's 38 matrices 570, 2048 x 9216 and the discriminator's other eight 3300.
+// Times (MI355X): 28 x 256 x 2304 440 us (prologue 45, two Gram matrices 51 each, twelve 256 x 256 products 14.5 to 22, Q X 65 to 70 each),
+// the generator's 38 matrices 560, 2048 x 9216 2420 and 2830 with the discriminator's other eight: 0.9 PFLOP/s of bf16 MFMAs, a large
+// library product at 1.21.  The 256 x 256 products are latency: launch, first and last bytes.
 // All matrices of a call go through one launch per product (a block finds its group of equal matrices in the kernel's arguments).
 #include <limits.h>
 #include <math.h>
@@ -669,19 +671,16 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
 }
 
 // ---- short sides of up to 64 ---------------------------------------------------------------------------------------------
-// A, Q and up to 448 columns of X fit into LDS as limbs (16 + 16 + 112 KB), so one workgroup can take a step's products one after the
-// other with a barrier between them; as launches they cost 5 us each at these sizes.  Matrices of up to 448 columns run their whole
-// iteration in one workgroup (ortho_small_kernel).  Longer ones are cut into panels of columns, one workgroup each: a launch per step
-// adds the panels' shares of the Gram matrix up (every workgroup for itself, in a fixed order), forms Q, multiplies its panel by it and
-// leaves the panel's share of the next Gram matrix (ortho_panel_kernel).  A step of 108 x 50 takes 2.8 us: 0.7 for the Gram matrix, 0.8
-// for A A and Q, 1.2 for Q X; of them 24 + 12 + 24 MFMAs of 33 cycles 0.8, the LDS reads at 250 bytes a cycle 0.4, the conversions 0.6,
-// one after the other with a single wave per SIMD, and three barriers.
-// Five steps, panels / the products as launches, us (one workgroup: 50 x 108 20, 64 x 256 31, 64 x 448 47):
-//   64 x 449  51 / 113     8 of 33 x 1000  59 / 127     100 of 64 x 576  93 / 150     64 x 4096   79 / 142    16 of 64 x 8192 221 / 246
-//   20 x 8192 86 / 152    40 of 64 x 576  69 / 126      256 of 64 x 576 183 / 229     64 x 14336 121 / 171    30 of 64 x 4096 204 / 224
-// Past two workgroups per CU their shares of the Gram matrices cost more than they save (1000 of 20 x 1500: 2140, 1700 as launches).
-// Panels of 1 or 2 chunks are as fast for one matrix and slower for several; 16 panels at most instead of 32 cost 20 x 8192 a third, 64
-// cost 64 x 4096 a quarter.
+// A and Q (one after the other, 24 KB) and up to 320 columns of X (120 KB) fit into LDS as limbs, so one workgroup can take a step's
+// products one after the other with barriers between them; as launches they cost 5 us each at these sizes.  Matrices of up to 320
+// columns run their whole iteration in one workgroup (ortho_small_kernel).  Longer ones are cut into panels of columns, one
+// workgroup each: a launch per step adds the panels' shares of the Gram matrix up (every workgroup for itself, in a fixed order),
+// forms Q, multiplies its panel by it and leaves the panel's share of the next Gram matrix (ortho_panel_kernel).
+// Five steps, panels / the products as launches, us (one workgroup: 50 x 108 29, 64 x 256 43, 64 x 320 53):
+//   64 x 449  56 / 115     8 of 33 x 1000  67 / 132     100 of 64 x 576  121 / 166     64 x 4096   83 / 141     16 of 64 x 8192 273 / 259
+//   20 x 8192 96 / 154    40 of 64 x 576  75 / 133      256 of 64 x 576 240 / 251     64 x 10240 122 / 164     30 of 64 x 4096 261 / 253
+// The right-hand column takes more than one workgroup per CU (two rounds of them, 98 KB of LDS and more each): those go as products.
+// Narrowest panels of 2 / 4 / 6 chunks: 8 of 33 x 1000 70 / 67 / 78, 20 of 64 x 576 69 / 65 / 73, 64 x 449 53 / 56 / 70.
 #define ORTHO_SMALL_M 64
 #define ORTHO_SMALL_N 320      // columns that fit into LDS (chunks are handled in pairs)
 #define ORTHO_WIDE 4           // narrowest panel, in chunks of 32 columns
@@ -1108,12 +1107,12 @@ struct OrthoCall {
 
 // Steps between two Gram matrices.  Longer chains save products with the long side and add M x M products, so they pay from N = 2 M
 // on, and only where the long side's products fill the chip (`tiles`: 128 x 128 tiles of Q X of the whole pass; below, the number of
-// launches counts, and chains of one have the fewest).  They carry rounding further, the more the smaller M.  Five steps with chains
-// of 1 / 2 / 3, time and relative error against 64 bits, and the error of the plain iteration in f32:
-//   28 x 256 x 2304  423 / 356 / 331 us    1.5 / 1.7 / 3.0e-6  (3.4e-6)      4 x 256 x 1152   156 / 150 / 162 us    1.2 / 1.8 / 3.0e-6  (2.7e-6)
-//   2048 x 9216     2060 / 1586 / 1348     1.8 / 1.8 / 2.6e-6  (5.4e-6)      3 x 333 x 1021   163 / 164 / 176       1.2 / 1.6 / 2.7e-6  (2.7e-6)
-//   20 x 200 x 1000  205 / 194 / 196       1.3 / 2.1 / 3.7e-6  (2.5e-6)      1500 x 2000      447 / 460 / 455       1.3 / 1.3 / 4.1e-6  (3.6e-6)
-//   1024 x 4608      435 / 363 / 329       1.3 / 1.3 / 3.1e-6  (3.8e-6)      4 x 128 x 576    122 / 121 / 135       0.7 / 2.8 / 3.5e-6  (1.8e-6)
+// launches counts, and chains of one have the fewest).  They carry rounding further, the more the smaller M: the lengths taken stay
+// below the error of the plain iteration in f32.  Five steps with chains of 1 / 2 / 3, time and relative error against 64 bits (plain f32):
+//   28 x 256 x 2304  663 / 526 / 460 us    1.3 / 1.5 / 2.6e-6  (3.4e-6)      4 x 256 x 1152   185 / 190 / 182 us    0.9 / 1.5 / 2.5e-6  (2.7e-6)
+//   2048 x 9216     3796 / 2903 / 2422     1.8 / 1.8 / 2.5e-6  (5.4e-6)      3 x 333 x 1021   199 / 207 / 206       0.9 / 1.4 / 2.4e-6  (2.7e-6)
+//   20 x 200 x 1000  251 / 234 / 226       1.0 / 1.8 / 3.1e-6  (2.5e-6)      1500 x 2000      657 / 670 / 668       1.2 / 1.3 / 4.0e-6  (3.5e-6)
+//   1024 x 4608      647 / 533 / 469       1.2 / 1.2 / 3.0e-6  (3.7e-6)      4 x 128 x 576    134 / 148 / 145       0.6 / 2.3 / 2.8e-6  (1.7e-6)
 static int ortho_chain(const OrthoGroup &g, long tiles) {
   const int M = og_short(g), N = og_long(g);
   if (tiles < 256 || M < 192 || N < 2 * M) return 1;
@@ -1204,8 +1203,8 @@ static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
 }
 
 // Ranges of a Gram matrix' reduction.  A product whose tiles leave CUs idle splits a long reduction into ranges of 512 columns, at the
-// price of the launch that adds them up.  Five steps: 512 x 2304 177 us, 187 with ranges of 1024; 200 x 4000 157, 168 with 256, 170 with
-// 1024; 4 x 128 x 576 110, 118 in two ranges; 3 x 333 x 1021 160 to 164 whatever the ranges.
+// price of the launch that adds them up.  Five steps, no ranges / 1024 / 512 / 256 columns: 512 x 2304 292 / 248 / 226 / 226 us, 200 x 4000
+// 322 / 213 / 184 / 186, 128 x 8192 508 / 194 / 186 / 185, 3 x 333 x 1021 209 / 211 / 204 / 198, 4 x 128 x 576 137 / 136 / 137 / 147.
 #define ORTHO_KZ 16
 static int ortho_kz(int K, long own, long tiles) {
   long z = 256 / (tiles > 0 ? tiles : 1);
@@ -1225,19 +1224,18 @@ struct OrthoLayout {
   int norm_blocks, split_blocks;
 };
 
-// Widths of the panels (g[i].jobs): the smallest from ORTHO_WIDE chunks on that leaves the pass no more workgroups than CUs, or else
-// than twice as many (two fit on a CU), and no matrix more than ORTHO_PANELS panels.  False if there is none.
+// Widths of the panels (g[i].jobs): the smallest from ORTHO_WIDE chunks on that leaves the pass no more workgroups than CUs and no
+// matrix more than ORTHO_PANELS panels.  False if there is none.
 static bool ortho_panel_chunks(OrthoGroup *g, int n) {
-  for (long limit : {256L, 512L})
-    for (int w = ORTHO_WIDE; w <= ORTHO_SMALL_N / 32; ++w) {
-      long blocks = 0, most = 0;
-      for (int i = 0; i < n; ++i) {
-        g[i].jobs = w;
-        blocks += (long)g[i].count * og_panels(g[i]);
-        if (og_panels(g[i]) > most) most = og_panels(g[i]);
-      }
-      if (blocks <= limit && most <= ORTHO_PANELS) return true;
+  for (int w = ORTHO_WIDE; w <= ORTHO_SMALL_N / 32; ++w) {
+    long blocks = 0, most = 0;
+    for (int i = 0; i < n; ++i) {
+      g[i].jobs = w;
+      blocks += (long)g[i].count * og_panels(g[i]);
+      if (og_panels(g[i]) > most) most = og_panels(g[i]);
     }
+    if (blocks <= 256 && most <= ORTHO_PANELS) return true;
+  }
   return false;
 }
 
@@ -1382,27 +1380,26 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
   else ORTHO_PRE(__bf16, false);
 #undef ORTHO_PRE
   for (int l = 0; l < levels; ++l) {
-    long b128 = 0, mid128 = 0, long128 = 0;                             // 128 x 128 tiles, those of short sides from 256, 1024 on
-    bool square = true;
+    long wide = 0;                                                       // 128 x 128 tiles of short sides from 1024 on
+    bool square = true, narrow = false;
     for (int i = 0; i < n; ++i) {
       const OrthoPlan &p = plan[lo.chain[i] - 1];
       lv.gs.g[i].type = l < p.levels ? p.level[l].type : OL_SYM;
       lv.gs.g[i].jobs = l < p.levels ? p.level[l].jobs : 0;
       if (l < p.levels) memcpy(lv.job + 2 * i, p.level[l].job, sizeof p.level[l].job);
       square = square && lv.gs.g[i].type == OL_SYM;
-      const long units = (long)g[i].count * lv.gs.g[i].jobs * og_tiles(g[i], lv.gs.g[i].type, 128);
-      b128 += units;
-      if (og_short(g[i]) >= 256) mid128 += units;
-      if (og_short(g[i]) >= 1024) long128 += units;
+      if (og_short(g[i]) >= 1024) wide += (long)g[i].count * lv.gs.g[i].jobs * og_tiles(g[i], lv.gs.g[i].type, 128);
+      else narrow |= lv.gs.g[i].jobs > 0;
     }
-    // 128 x 128 tiles read each operand half as often but need enough of them to fill the 256 CUs, symmetric products of short sides
-    // below 1024 (a few chunks to a tile, more of it padding or above the diagonal) two per CU.  Symmetric products, 64 / 128 wide:
-    // 2048 x 9216 (136 of 128) 1281 / 1465 us, 6 x 1024 x 1024 (216) 590 / 553, 2500 x 2500 (210) 1272 / 1119, 3700 x 3700 (435) 3330 /
-    // 3030; 100 x 200 x 300 (300) 325 / 369, 64 x 256 x 2304 (192) 599 / 674, 40 x 512 x 512 (400) 561 / 564.  A split reduction on 128
-    // does not help: 2048 x 2048, 3 ranges 34 us and 17 to join them, 46 on 64
-    // Q X: 2048 x 9216 (1152) 1545 / 1370, 64 x 256 x 2304 (2304) 660 / 642; 28 x 256 x 2304 (1008) 341 / 341, 1024 x 4608 (288) 346 / 343,
-    // 8 x 512 x 2304 (576) 340 / 347, 200 x 128 x 576 (1000) 327 / 342, the generator's 38 matrices (1080) 437 / 453
-    const int T = square ? (b128 >= 500 || long128 >= 200 ? 128 : 64) : mid128 >= 2000 || long128 >= 256 ? 128 : 64;
+    // 128 x 128 tiles read each operand half as often, but there are fewer of them and one at a time on a CU (98 KB of LDS): for short
+    // sides from 1024 on where they go round the 256 CUs once, most of them busy, or (Q X) more than twice; symmetric ones not in the
+    // company of shorter sides, which need their reductions split (the discriminator's step 3170 us so, 2830 on 64).  Five steps, us, 64 / 128 wide:
+    //   symmetric: 1800 x 3000 (120 tiles) 1205 / 1409, 2048 x 9216 (136) 2416 / 2364, 2300 x 2300 (171) 1608 / 1579, 2500 x 9000 (210) 4225 /
+    //   3914, 6 x 1024 x 1024 (216) 915 / 847; two rounds: 8 x 1024 x 1024 (288) 1073 / 1260, 3000 x 3000 (300) 3255 / 3687, 3700 x 3700
+    //   (435) 5659 / 5485, 4096 x 4096 (528) 7465 / 7850; sides below 1024: 64 x 512 x 512 (640) 1387 / 1432, 200 x 256 x 500 (600) 1291 / 1381
+    //   Q X: 1500 x 2000 (192) 678 / 654, 2048 x 2048 (256) 1268 / 1134, 1024 x 4608 (288) 488 / 518, 1200 x 9000 (710) 814 / 787, 2048 x 9216
+    //   (1152) 2576 / 2416; sides below 1024: 40 x 512 x 512 (640) 846 / 856, 4 x 700 x 700 (144) 314 / 350
+    const int T = square ? (!narrow && wide > 160 && wide <= 256 ? 128 : 64) : (wide > 160 && wide <= 256) || wide > 512 ? 128 : 64;
     bool split_any = false;
     for (int pass = 0; pass < 2; ++pass) {
       int blocks = 0;
@@ -1417,13 +1414,12 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
         blocks += (int)((units + 7) / 8 * 8);
       }
       if (!blocks) break;
-      // 64 x 64 tiles: more stages hide more latency as long as the blocks that a CU gets fit beside each other: 4 for one block per CU
-      // (1024 x 4608: 326 us, 347 with 3, 475 with 2), 3 for two (28 x 256 x 2304: 310; 316 with 4, 329 with 2), else 2 (2048 x 9216:
-      // 1282; 1398 with 3).  128 x 128 tiles: 2 stages, two blocks per CU (2048 x 9216: 1281; 1468 with 3)
-      const int rc = T == 128       ? ortho_launch<128, 32, 2, 2, 2>(ws, lv, blocks, st)
+      // Stages hide latency as long as the blocks that a CU gets fit beside each other: 64-wide tiles with 3 (73 KB) for two blocks per CU
+      // (28 x 256 x 2304 452 us, 463 with 2; 1024 x 1024 263 / 327; no more with 4 or 6 for one), else 2, three blocks (28 x 256 x 2304
+      // with 3: 471; 200 x 128 x 576 456 / 507).  128-wide ones: 8 waves of 64 x 32 (2048 x 9216 2464, 4 waves of 64 x 64 2687; 3 stages 2443)
+      const int rc = T == 128       ? ortho_launch<128, 32, 2, 2, 4>(ws, lv, blocks, st)
                      : blocks > 512 ? ortho_launch<64, 32, 2, 2, 2>(ws, lv, blocks, st)
-                     : blocks > 256 ? ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st)
-                                    : ortho_launch<64, 32, 4, 2, 2>(ws, lv, blocks, st);
+                                    : ortho_launch<64, 32, 3, 2, 2>(ws, lv, blocks, st);
       if (rc) return rc;
       if (!split_any) break;
     }

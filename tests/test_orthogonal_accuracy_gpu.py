@@ -87,6 +87,14 @@ def test_graded_rows_over_many_steps(count, rows, cols, decades):
     check(ops.newton_schulz(g, 20), g, 20, scale=scale)
 
 
+@pytest.mark.parametrize('count,rows,cols', [(4, 1030, 1950), (4, 1950, 1030), (1, 2250, 2250)])
+def test_wide_tiles_of_odd_halves(count, rows, cols):
+    """128 x 128 tiles, symmetric and not, on an odd number of 64-row and 64-column halves."""
+    from lsps_amd import ops
+    g = torch.randn(count, rows, cols, generator=torch.Generator().manual_seed(5)).cuda()
+    check(ops.newton_schulz(g), g)
+
+
 @pytest.mark.parametrize('count,rows,cols', [(2, 48, 100), (2, 40, 1000), (2, 128, 400)])
 def test_graded_bf16(count, rows, cols):
     from lsps_amd import ops
