@@ -8,6 +8,7 @@ import ctypes as _ctypes
 import struct as _struct
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from . import options  # noqa: F401  (`ops.options.get()`: the process options in force)
@@ -1723,6 +1724,15 @@ def _same_device(what, t, *others):
     return index
 
 
+def _no_tangent(what, *tensors):
+    """Refuses dual tensors (torch.autograd.forward_ad): they do not require a gradient, so that the kernels would run on the primal
+    values and the tangent would be gone without a word."""
+    if getattr(_forward_ad, '_current_level', 0) >= 0:             # inside dual_level() only
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+                raise _lib.LspsHipError("%s has no forward-mode derivative: a tensor carries a tangent" % what)
+
+
 # hipStream_t of a device's current stream: what torch.cuda.current_stream(index).cuda_stream is, without building a Stream object
 # (2.4 us; the small layer norms are bound by such calls)
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -1838,7 +1848,7 @@ _layer_norm_backward_once = torch.autograd.function.once_differentiable(_layer_n
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     """nn.functional.layer_norm on the HIP kernels (csrc/layernorm.hip): `x` float32 or bfloat16 [..., *normalized_shape], `weight` and
-    `bias` float32 of `normalized_shape` or None.  Statistics and parameter gradients are float32; differentiable once.  Rows that lie
+    `bias` float32 of `normalized_shape` or None.  Statistics and parameter gradients are float32; differentiable once, in reverse mode.  Rows that lie
     at a pitch (a slice of wider rows) are read where they are."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     cols = 1
@@ -1851,6 +1861,7 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     for t in (weight, bias):
         if t is not None and (t.shape != shape or t.dtype != torch.float32):
             raise _lib.LspsHipError("layer_norm: weight or bias of shape %s, %s (expected %s, float32)" % (tuple(t.shape), t.dtype, shape))
+    _no_tangent('layer_norm', x, weight, bias)
     index = _same_device('layer_norm', x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
@@ -1885,6 +1896,7 @@ def newton_schulz(g, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         raise _lib.LspsHipError("newton_schulz: float32 or bfloat16 expected, not %s" % g.dtype)
     if g.requires_grad and torch.is_grad_enabled():
         raise _lib.LspsHipError("newton_schulz has no backward pass: call it under torch.no_grad() or on a detached tensor")
+    _no_tangent('newton_schulz', g)
     index = _same_device('newton_schulz', g)
     out = _like(g)
     if g.numel() == 0:
@@ -1913,6 +1925,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
         raise _lib.LspsHipError("muon_step_: %d weights, %d gradients, %d momenta" % (len(params), len(grads), len(momenta)))
     if not params:
         return
+    _no_tangent('muon_step_', *params, *grads, *momenta)
     mats, index = [], None
     for matrix in zip(params, grads, momenta):          # (the host's part of a small step: no more calls here than it takes)
         p, g, m = matrix
