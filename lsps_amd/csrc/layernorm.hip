@@ -176,7 +176,7 @@ __global__ __launch_bounds__(WG) void ln_fwd_kernel(const typename U::type *__re
     ln_load_param<V>(w, at[u], cols, 1.f, wv[u]);
     ln_load_param<V>(b, at[u], cols, 0.f, bv[u]);
   }
-  const float inv = 1.f / (float)cols;
+  const float n = (float)cols;                           // divided by: times 1 / n rounds twice, and a constant row has a variance then
   const long step = (long)gridDim.x * RPW, first = (long)blockIdx.x * RPW;
   typename U::reg q[NU];
   auto fetch = [&](long r0) {
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(WG) void ln_fwd_kernel(const typename U::type *__re
         s += e >= skip[u] ? v[u][e] : 0.f;
       }
     if (r0 + step < rows) fetch(r0 + step);                                            // the next row, before this one's reductions
-    const float mu = ln_row_sum<TPR>(s, red, phase) * inv;
+    const float mu = ln_row_sum<TPR>(s, red, phase) / n;
     float s2 = 0.f;
 #pragma unroll
     for (int u = 0; u < NU; ++u)
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(WG) void ln_fwd_kernel(const typename U::type *__re
         v[u][e] -= mu;
         s2 += e >= skip[u] ? v[u][e] * v[u][e] : 0.f;
       }
-    const float rs = 1.f / sqrtf(ln_row_sum<TPR>(s2, red, phase) * inv + eps);
+    const float rs = 1.f / sqrtf(ln_row_sum<TPR>(s2, red, phase) / n + eps);
     if (r >= rows) continue;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(WG) void ln_bwd_kernel(const typename U::type *__re
 #pragma unroll
     for (int e = 0; e < V; ++e) aw[u][e] = ab[u][e] = 0.f;
   }
-  const float inv = 1.f / (float)cols;
+  const float n = (float)cols;
   const long step = (long)gridDim.x * RPW;
   typename U::reg xq[NU], gq[NU];
   float mu = 0.f, rs = 0.f;
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(WG) void ln_bwd_kernel(const typename U::type *__re
         s2 = fmaf(once * wv[u][e], h[u][e], s2);
       }
     if (r0 + step < rows) fetch(r0 + step);
-    const float m1 = ln_row_sum<TPR>(s1, red, phase) * inv, m2 = ln_row_sum<TPR>(s2, red, phase) * inv;
+    const float m1 = ln_row_sum<TPR>(s1, red, phase) / n, m2 = ln_row_sum<TPR>(s2, red, phase) / n;
     if (r >= rows || !dx) continue;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
