@@ -100,3 +100,91 @@ def test_graded_bf16(count, rows, cols):
     from lsps_amd import ops
     g, scale = graded(count, rows, cols, 'ramp row col', 6)
     check(ops.newton_schulz(g.bfloat16()), g.bfloat16(), scale=scale)
+
+
+@pytest.mark.parametrize('rows,cols', [(21000, 22000), (22000, 20500)])
+def test_matrix_whose_limbs_pass_2_gib(rows, cols):
+    """One step of a matrix of 2.7 GB of limbs, against the formula applied to a vector: a missing chunk of 32 columns would be off
+    by 1e-3 of it; a sum of up to 22000 terms takes 1400 roundings in runs of 16, whose errors of 2^-24 add up to about their root's
+    number: 40 * 2^-24 < 2^-18."""
+    from lsps_amd import ops
+    gen = torch.Generator(device='cuda').manual_seed(2)
+    g = torch.randn(rows, cols, generator=gen, device='cuda')
+    out = ops.newton_schulz(g, 1)
+
+    def times(m, v, transposed=False):                       # in 64 bits, a block of rows at a time
+        parts = [(p.double().T.contiguous() @ v[k * 2048:k * 2048 + len(p)]) if transposed else p.double() @ v
+                 for k, p in enumerate(m.split(2048))]
+        return sum(parts) if transposed else torch.cat(parts)
+    norm = math.sqrt(sum(float(p.double().square().sum()) for p in g.split(2048))) + 1e-7
+    tall = rows > cols
+    v = torch.randn(rows if tall else cols, generator=gen, device='cuda', dtype=torch.float64)
+    a, b, c = COEFFS
+    y = times(g, v, tall) / norm                              # X v, X with its short side in rows
+    up = lambda u: times(g, times(g, u, not tall), tall) / norm ** 2           # noqa: E731     A u
+    ay = up(y)
+    want = a * y + b * ay + c * up(ay)
+    assert float((times(out, v, tall) - want).norm()) <= 2.0 ** -18 * float(want.norm())
+
+
+def gradients(count, rows, cols, seed=0):
+    """Low rank under noise, as weights' gradients are."""
+    gen = torch.Generator().manual_seed(seed + 7 * rows + cols)
+    r = max(1, min(rows, cols) // 6)
+    g = torch.randn(count, rows, r, generator=gen) @ torch.randn(count, r, cols, generator=gen) / math.sqrt(r)
+    return ((g + torch.randn(count, rows, cols, generator=gen)) * 1e-3).cuda()
+
+
+@pytest.mark.parametrize('count,rows,cols', [
+    # one workgroup: short sides on both sides of 32, up to 320 columns; panels of several widths; products: few tiles and many, split
+    # reductions, chains of one, two and three steps, 64- and 128-wide tiles
+    (3, 20, 50), (1, 50, 108), (2, 31, 33), (2, 64, 64), (2, 33, 319), (2, 320, 64), (300, 40, 300), (2, 64, 321), (1, 20, 8192), (3, 50, 1000),
+    (2, 9000, 33), (40, 64, 576), (25, 64, 640), (70, 64, 448), (1, 65, 63), (1, 65, 700), (2, 130, 65), (4, 128, 576), (5, 100, 333), (1, 333, 1021),
+    (1, 200, 4000), (2, 256, 256), (1, 257, 700), (20, 448, 1000), (20, 200, 1000), (8, 256, 2304), (40, 520, 600), (1, 1024, 1100), (4, 1030, 1030)])
+def test_as_accurate_as_f32(count, rows, cols):
+    from lsps_amd import ops
+    g = gradients(count, rows, cols)
+    check(ops.newton_schulz(g), g)
+
+
+EPS_PATHS = [(2, 48, 100), (2, 100, 20), (2, 40, 1000), (1, 900, 30), (2, 128, 400), (1, 300, 170)]
+
+
+@pytest.mark.parametrize('count,rows,cols', EPS_PATHS)
+@pytest.mark.parametrize('size', [0.1, 1.0, 10.0])
+@pytest.mark.parametrize('eps', [1e-7, 0.5])
+def test_eps_beside_the_norm(count, rows, cols, size, eps):
+    """|G|_F of a tenth of eps to ten times it: eps counts once per matrix, whatever path computes it."""
+    from lsps_amd import ops
+    g = gradients(count, rows, cols)
+    g *= size * eps / g.flatten(1).norm(dim=1)[:, None, None]
+    check(ops.newton_schulz(g, eps=eps), g, eps=eps)
+    p, m = [torch.zeros_like(t) for t in g], [torch.zeros_like(t) for t in g]
+    ops.muon_step_(p, list(g), m, lr=1.0, momentum=0.0, nesterov=False, rms=1.0, eps=eps)
+    check(torch.stack(p) / -math.sqrt(max(rows, cols)), g, eps=eps)
+
+
+# more matrices than travel in a launch's arguments (16), than one launch enters into the table (96), than a pass takes (1024), more
+# shapes than a pass takes (16)
+MANY = {'40 small': [(40, 24, 50)], '40 panels': [(40, 30, 700)], '40 products': [(40, 70, 90)], '130 small of two shapes': [(65, 24, 50), (65, 40, 20)],
+        '120 panels and small': [(100, 20, 330), (20, 330, 20)], '1100 tiny': [(600, 20, 24), (500, 30, 20)],
+        '1060 products': [(1060, 66, 70)], '19 shapes': [(2, 66 + k, 300 - 9 * k) for k in range(19)],
+        '18 shapes of panels': [(1, 20 + k, 340 + 9 * k) for k in range(18)]}
+
+
+@pytest.mark.parametrize('name', list(MANY))
+def test_many_matrices(name):
+    from lsps_amd import ops
+    stacks = [gradients(*s, seed=k) for k, s in enumerate(MANY[name])]
+    where = [(k, i) for k, s in enumerate(stacks) for i in range(len(s))]
+    order = torch.randperm(len(where), generator=torch.Generator().manual_seed(1)).tolist()
+    where = [where[i] for i in order]                         # shapes in no order
+    ps = [torch.zeros_like(s) for s in stacks]
+    ms = [torch.full_like(s, 1e-3) for s in stacks]
+    ops.muon_step_([ps[k][i] for k, i in where], [stacks[k][i] for k, i in where], [ms[k][i] for k, i in where], lr=1.0, momentum=0.5, rms=1.0)
+    for p, g, m in zip(ps, stacks, ms):
+        new = 0.5 * torch.full_like(g, 1e-3).double() + g.double()
+        # a product and a sum: 2^-24 of the momentum and of what is added to it
+        assert bool(((m.double() - new).abs() <= 2.0 ** -23 * (new.abs() + 1e-3)).all())
+        u = (g + 0.5 * m)
+        check(p / -math.sqrt(max(g.shape[1:])), u)
