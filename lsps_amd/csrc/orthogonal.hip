@@ -1203,11 +1203,15 @@ static bool ortho_plan(OrthoPlan *p, int most, const OrthoCall &c) {
 }
 
 // Ranges of a Gram matrix' reduction.  A product whose tiles leave CUs idle splits a long reduction into ranges of 512 columns, at the
-// price of the launch that adds them up.  Five steps, no ranges / 1024 / 512 / 256 columns: 512 x 2304 292 / 248 / 226 / 226 us, 200 x 4000
-// 322 / 213 / 184 / 186, 128 x 8192 508 / 194 / 186 / 185, 3 x 333 x 1021 209 / 211 / 204 / 198, 4 x 128 x 576 137 / 136 / 137 / 147.
+// price of the launch that adds them up: no block longer than its share of the pass' whole reduction (`work`: columns times tiles)
+// on 256 CUs; of 4096 columns and more on 768 blocks, three to a CU, since one alone waits for its loads (0.75 us a chunk, 0.17 of
+// MFMAs).  Five steps, no ranges / 1024 / 512 / 256 columns: 512 x 2304 292 / 248 / 226 / 226 us, 200 x 4000 322 / 213 / 184 / 186,
+// 128 x 8192 508 / 194 / 186 / 185, 3 x 333 x 1021 209 / 211 / 204 / 198, 4 x 128 x 576 137 / 136 / 137 / 147.  Shares of 256 / 768: a step of
+// the generator and the pose mapping (1024 x 16384 and 1024 x 8192 among 42) 2377 / 2066, 1024 x 16384 949 / 905, 1024 x 4608 486 / 469, 1300 x
+// 9000 943 / 968; below 4096 columns: 1024 x 1024 263 / 284, 2 x 600 x 2000 300 / 314, 28 x 256 x 2304 441 / 457.
 #define ORTHO_KZ 16
-static int ortho_kz(int K, long own, long tiles) {
-  long z = 256 / (tiles > 0 ? tiles : 1);
+static int ortho_kz(int K, long own, long work) {
+  long z = (K >= 4096 ? 768L : 256L) * K / work;
   if (own <= 16 && z < K / 1024) z = K / 1024;             // few tiles in the company of many: not the launch's last ones
   const long most = K / 512;
   if (z > most) z = most;
@@ -1274,13 +1278,13 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
     lo.bytes = at;
     return lo;
   }
-  long tiles = 0, rect = 0;
+  long work = 0, rect = 0;
   for (int i = 0; i < n; ++i) rect += (long)g[i].count * og_tiles(g[i], OL_RECT, 128);
   for (int i = 0; i < n; ++i) {
     lo.chain[i] = ortho_chain(g[i], rect);
     lo.split_first[i] = lo.split_blocks;
     lo.split_blocks += g[i].count * og_split_blocks(g[i]);
-    tiles += (long)g[i].count * og_tiles(g[i], OL_SYM, 64);
+    work += (long)g[i].count * og_tiles(g[i], OL_SYM, 64) * og_pad(og_long(g[i]));
   }
   for (int i = 0; i < n; ++i) {
     const size_t M = og_pad(og_short(g[i])), N = og_pad(og_long(g[i]));
@@ -1289,7 +1293,7 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
     g[i].s_off = (unsigned)(at / 256);
     at += M * M * OG_BYTES * g[i].count * OB_SMALL;
     g[i].p_off = (unsigned)(at / 256);
-    lo.kz[i] = ortho_kz((int)N, (long)g[i].count * og_tiles(g[i], OL_SYM, 64), tiles);
+    lo.kz[i] = ortho_kz((int)N, (long)g[i].count * og_tiles(g[i], OL_SYM, 64), work);
     if (lo.kz[i] > 1) at += (size_t)lo.kz[i] * g[i].count * og_tiles(g[i], OL_SYM, 64) * 64 * 64 * 4;
   }
   lo.bytes = at;

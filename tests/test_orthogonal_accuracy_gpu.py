@@ -169,6 +169,7 @@ def test_eps_beside_the_norm(count, rows, cols, size, eps):
 MANY = {'40 small': [(40, 24, 50)], '40 panels': [(40, 30, 700)], '40 products': [(40, 70, 90)], '130 small of two shapes': [(65, 24, 50), (65, 40, 20)],
         '120 panels and small': [(100, 20, 330), (20, 330, 20)], '1100 tiny': [(600, 20, 24), (500, 30, 20)],
         '1060 products': [(1060, 66, 70)], '19 shapes': [(2, 66 + k, 300 - 9 * k) for k in range(19)],
+        'long reductions in company': [(2, 300, 4100), (1, 20, 8192), (6, 256, 700), (1, 4500, 130)],
         '18 shapes of panels': [(1, 20 + k, 340 + 9 * k) for k in range(18)]}
 
 
