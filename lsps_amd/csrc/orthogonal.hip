@@ -23,7 +23,7 @@
 // Q X reads it transposed from LDS (28 x 256 x 2304 with an earlier loop on two limbs: 407 us, 451 with X^T beside X).
 //
 // Times (MI355X): 28 x 256 x 2304 440 us (prologue 45, two Gram matrices 51 each, twelve 256 x 256 products 14.5 to 22, Q X 65 to 70 each),
-// the generator's 38 matrices 560, 2048 x 9216 2420 and 2830 with the discriminator's other eight: 0.9 PFLOP/s of bf16 MFMAs, a large
+// the generator's 38 matrices 553, 2048 x 9216 2375 and 2795 with the discriminator's other eight: 0.9 PFLOP/s of bf16 MFMAs, a large
 // library product at 1.21.  The 256 x 256 products are latency: launch, first and last bytes.
 // All matrices of a call go through one launch per product (a block finds its group of equal matrices in the kernel's arguments).
 #include <limits.h>

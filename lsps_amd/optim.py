@@ -233,8 +233,8 @@ class FlatAdam(torch.optim.Optimizer):
 
 
 class FlatMuon(FlatAdam):
-    """Muon over a FlatArena: weight matrices (conv weights as (out, in * taps)) take an orthogonalised momentum step, all of them in
-    one lsps_muon_step call; what has no two directions of more than one element (biases, gains, a one-row head) takes Adam as in
+    """Muon over a FlatArena: weight matrices (conv weights with shape[0] rows: (out, in * taps), of transposed convs (in, out * taps)) take
+    an orthogonalised momentum step, all of them in one lsps_muon_step call; what has no two directions of more than one element (biases, gains, a one-row head) takes Adam as in
     FlatAdam, from the same buffers (a matrix' momentum lives where exp_avg would; exp_avg_sq is not used for it).
 
     `lr`, `betas`, `eps`: as FlatAdam (`eps`: Adam's).  A matrix moves by lr * rms in the root mean square of its entries, so `rms` = 0.2 suits
