@@ -226,6 +226,11 @@ __device__ __forceinline__ void og_value(const og_b4 (&l)[3], float (&v)[4]) {
   for (int k = 0; k < 4; ++k) v[k] = (float)l[0][k] + ((float)l[1][k] + (float)l[2][k]);
 }
 
+// In front of the first use of accumulators behind a join of paths: an MFMA's last registers arrive 12 wait states behind it, and the
+// compiler counts them along one of the paths only (seen: 15 instructions on a path round a conditional load, 7 on the one without;
+// the last product of every 16th value was lost).
+__device__ __forceinline__ void og_settle(og_f16v &a, og_f16v &b) { asm volatile("s_nop 15" : "+v"(a), "+v"(b)); }
+
 __device__ __forceinline__ og_b8 og_join(const og_b4 &a, const og_b4 &b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // v / norm as f32: norm = mantissa * 2^ex, v 2^-ex rounded by one factor, so that nothing overflows on the way for any norm
@@ -539,6 +544,10 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
       load(1, at);
       multiply(0);
       multiply(1);
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) og_settle(acc[i][j], acx[i][j]);
     };
     if (c0 < c1) {
       if (turned) product(OgTrue());
@@ -862,6 +871,7 @@ __device__ __forceinline__ void og_square_tile(const char *in, int chunks, int t
     multiply(1);
     if (++c == chunks) break;
   }
+  og_settle(acc, acx);
 #pragma unroll
   for (int e = 0; e < 16; ++e) v[e] = acc[e] + acx[e];
 }
@@ -930,6 +940,8 @@ __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, flo
 #pragma unroll
       for (int f = 0; f < MT; ++f) og_multiply(x[h], qf[h][f], acc[f], acx[f]);
     if (ch + 4 < chunks) load(chunk + 4 * OG_CHUNK);
+#pragma unroll
+    for (int f = 0; f < MT; ++f) og_settle(acc[f], acx[f]);
 #pragma unroll
     for (int f = 0; f < MT; ++f)
 #pragma unroll
