@@ -680,19 +680,20 @@ __global__ __launch_bounds__(WI * WJ * 64, T == 64 && S == 2 ? 3 : 2) void ortho
 }
 
 // ---- short sides of up to 64 ---------------------------------------------------------------------------------------------
-// A and Q (one after the other, 24 KB) and up to 320 columns of X (120 KB) fit into LDS as limbs, so one workgroup can take a step's
-// products one after the other with barriers between them; as launches they cost 5 us each at these sizes.  Matrices of up to 320
-// columns run their whole iteration in one workgroup (ortho_small_kernel).  Longer ones are cut into panels of columns, one
-// workgroup each: a launch per step adds the panels' shares of the Gram matrix up (every workgroup for itself, in a fixed order),
-// forms Q, multiplies its panel by it and leaves the panel's share of the next Gram matrix (ortho_panel_kernel).
-// Five steps, panels / the products as launches, us (one workgroup: 50 x 108 29, 64 x 256 43, 64 x 320 53):
-//   64 x 449  56 / 115     8 of 33 x 1000  67 / 132     100 of 64 x 576  121 / 166     64 x 4096   83 / 141     16 of 64 x 8192 273 / 259
-//   20 x 8192 96 / 154    40 of 64 x 576  75 / 133      256 of 64 x 576 240 / 251     64 x 10240 122 / 164     30 of 64 x 4096 261 / 253
+// A and Q (one after the other) and up to 320 columns of X of 33 to 64 rows (24 + 120 KB), 704 of up to 32 (6 + 132 KB), fit into LDS as
+// limbs, so one workgroup can take a step's products one after the other with barriers between them; as launches they cost 5 us each
+// at these sizes.  Such matrices run their whole iteration in one workgroup (ortho_small_kernel).  Longer ones are cut into panels of
+// columns, one workgroup each: a launch per step adds the panels' shares of the Gram matrix up (every workgroup for itself, in a fixed
+// order), forms Q, multiplies its panel by it and leaves the panel's share of the next Gram matrix (ortho_panel_kernel).
+// Five steps, panels / the products as launches, us (one workgroup: 50 x 108 30, 64 x 256 43, 64 x 320 55, 20 x 700 59, 1000 of 20 x 330 82):
+//   64 x 449  57 / 115     8 of 33 x 1000  67 / 132     100 of 64 x 576  121 / 166     64 x 4096   83 / 141     16 of 64 x 8192 273 / 259
+//   20 x 8192 83 / 154    40 of 64 x 576  75 / 133      256 of 64 x 576 240 / 251     64 x 10240 122 / 164     30 of 64 x 4096 261 / 253
 // The right-hand column takes more than one workgroup per CU (two rounds of them, 98 KB of LDS and more each): those go as products.
 // Narrowest panels of 2 / 4 / 6 chunks: 8 of 33 x 1000 70 / 67 / 78, 20 of 64 x 576 69 / 65 / 73, 64 x 449 53 / 56 / 70.
 #define ORTHO_SMALL_M 64
-#define ORTHO_SMALL_N 320      // columns that fit into LDS (chunks are handled in pairs)
+#define ORTHO_SMALL_LDS 147456 // 320 columns of 64 rows, 704 of 32
 #define ORTHO_WIDE 4           // narrowest panel, in chunks of 32 columns
+#define ORTHO_WIDEST 10        // widest: 320 columns
 #define ORTHO_PANELS 32        // longest row of panels: every workgroup reads 16 KB of each
 #define ORTHO_FEW 16           // pointers that travel in the kernels' arguments, without a launch that fills the table
 struct OrthoSmall {
@@ -704,7 +705,10 @@ struct OrthoSmall {
   float decay, eps;
 };
 
-#define OG_CHUNK (64 * OG_LINE) // bytes of 64 rows x 32 columns in LDS
+// MT: the short side in tiles of 32 rows
+__host__ __device__ static inline int og_mt(const OrthoGroup &g) { return og_short(g) <= 32 ? 1 : 2; }
+// bytes of 32 MT rows x 32 columns in LDS
+__host__ __device__ static constexpr int og_chunk(int MT) { return 32 * MT * OG_LINE; }
 // byte of columns 8 q ... 8 q + 7 of row r, one limb, in a chunk in LDS
 __device__ __forceinline__ int og_unit(int r, int q, int limb) { return r * OG_LINE + limb * 64 + ((q ^ ((r >> 2) & 3)) << 4); }
 // 8 columns of a row, half chunk `half`, one limb: a lane's MFMA operand
@@ -728,36 +732,43 @@ __device__ __forceinline__ void og_multiply(const og_b8 (&y)[3], const og_b8 (&x
   acx = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[1], x[0], acx, 0, 0, 0);
 }
 
-// A panel's elements, 256 threads, 64 columns x 16 per thread at a time; lanes run along the rows of G (TALL: along the short side).
-// Loads and stores go through buffer descriptors, whose bounds check does the padding's zeros: no branch stands between 16 loads.
-template <bool TALL>
+// A panel's elements, 256 threads, 64 columns at a time (8 MT elements per thread); lanes run along the rows of G (TALL: along the
+// short side).  Loads and stores go through buffer descriptors, whose bounds check does the padding's zeros: no branch stands between them.
+template <bool TALL, int MT>
 struct OgWalk {
+  static constexpr int E = 8 * MT, COLS = TALL ? 8 / MT : 1, CH = og_chunk(MT);      // COLS: columns from one of a thread's elements to the next
   int so, valid, row;             // elements between two of a thread's; how many it has there; bytes of its row and column in LDS
   int o, step, left;              // first element; to the next 64 columns; columns left
-  int lane, wave, m;
+  int lane, wave, m, r, c;        // r, c: TALL: its row and first column
   __device__ __forceinline__ OgWalk(const OrthoGroup &g, int j0, int chunks) {
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     m = og_short(g);
     const int n = og_long(g);
     left = n - j0 < chunks * 32 ? n - j0 : chunks * 32;
-    so = TALL ? 4 * m : 4 * n;
+    r = lane & (32 * MT - 1);
+    c = MT == 1 ? wave * 2 + (lane >> 5) : wave;
+    so = TALL ? COLS * m : 4 * n;
     step = TALL ? 64 * m : 64;
-    o = TALL ? (j0 + wave) * m + lane : wave * n + j0 + lane;
-    row = TALL ? lane * OG_LINE + wave * 4 : (lane >> 5) * OG_CHUNK + wave * OG_LINE + ((lane >> 2) & 1) * 64 + (lane & 3) * 4;
+    o = TALL ? (j0 + c) * m + r : wave * n + j0 + lane;
+    row = TALL ? r * OG_LINE + ((c >> 2) & 1) * 64 + (c & 3) * 4 : (lane >> 5) * CH + wave * OG_LINE + ((lane >> 2) & 1) * 64 + (lane & 3) * 4;
     count();
   }
-  __device__ __forceinline__ void count() { valid = TALL ? (lane < m ? (left - wave + 3) >> 2 : 0) : lane < left ? (m - wave + 3) >> 2 : 0; }
+  __device__ __forceinline__ void count() { valid = TALL ? (r < m ? (left - c + COLS - 1) / COLS : 0) : lane < left ? (m - wave + 3) >> 2 : 0; }
   __device__ __forceinline__ void next() {
     left -= 64;
     o += step;
-    row += 2 * OG_CHUNK;
+    row += 2 * CH;
     count();
   }
   __device__ __forceinline__ int at(int e) const { return e < valid ? o + e * so : -1; }      // -1: behind every buffer
   __device__ __forceinline__ int lds(int e) const {
-    if constexpr (TALL) return row + (e >> 3) * OG_CHUNK + (e & 1) * 64 + ((((e & 7) >> 1) ^ ((lane >> 2) & 3)) << 4);
-    else return row + e * 4 * OG_LINE + ((((lane & 31) >> 3) ^ (e & 3)) << 4);
+    if constexpr (TALL) {
+      const int first = e * COLS;                                                              // c + first: the column of 64
+      return row + (first >> 5) * CH + ((first >> 2) & 1) * 64 + ((((first >> 3) & 3) ^ ((r >> 2) & 3)) << 4);
+    } else {
+      return row + e * 4 * OG_LINE + ((((lane & 31) >> 3) ^ (e & 3)) << 4);
+    }
   }
 };
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t og_buffer(void *p, int bytes) { return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00027000); }
@@ -772,22 +783,23 @@ __device__ __forceinline__ void og_set(__amdgpu_buffer_rsrc_t b, int o, float v)
 
 // G (Muon: the momentum, updated on the way) as f32 into the place of its first two limbs (columns 8 q ... 8 q + 3 | 8 q + 4 ... 8 q + 7);
 // returns the thread's sum of squares
-template <typename T, bool MUON, bool TALL>
+template <typename T, bool MUON, bool TALL, int MT>
 __device__ __forceinline__ double og_fetch(const OrthoGroup &g, int j0, int chunks, const OrthoPtr &ptr, const OrthoMomentum &mo, char *X) {
   const int size = g.rows * g.cols;
   const __amdgpu_buffer_rsrc_t src = og_buffer(const_cast<void *>((const void *)ptr.g), size * (int)sizeof(T));
   const __amdgpu_buffer_rsrc_t mom = og_buffer(ptr.m, MUON ? size * 4 : 0);
-  OgWalk<TALL> w(g, j0, chunks);
+  OgWalk<TALL, MT> w(g, j0, chunks);
+  constexpr int E = 8 * MT;
   double sum = 0.;
   for (int c = 0; c < chunks; c += 2, w.next()) {
-    float v[16], mm[16];
+    float v[E], mm[E];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = og_get<T>(src, w.at(e));
+    for (int e = 0; e < E; ++e) v[e] = og_get<T>(src, w.at(e));
     if constexpr (MUON)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mm[e] = og_get<float>(mom, w.at(e));
+      for (int e = 0; e < E; ++e) mm[e] = og_get<float>(mom, w.at(e));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < E; ++e) {
       if constexpr (MUON) {
         v[e] *= mo.gscale;
         mm[e] = fmaf(mo.mu, mm[e], v[e]);
@@ -807,7 +819,7 @@ __device__ __forceinline__ void og_limbs(char *X, int chunks, double norm) {
   const OgUnit unit(norm);
   for (int t = threadIdx.x; t < chunks * 128 * MT; t += 256) {
     const int row = t & (32 * MT - 1), q = t / (32 * MT);
-    char *p = X + (q >> 2) * OG_CHUNK + og_unit(row, q & 3, 0);
+    char *p = X + (q >> 2) * og_chunk(MT) + og_unit(row, q & 3, 0);
     const og_f4 x[2] = {*reinterpret_cast<og_f4 *>(p), *reinterpret_cast<og_f4 *>(p + 64)};
     og_b4 l[2][3];
 #pragma unroll
@@ -821,17 +833,18 @@ __device__ __forceinline__ void og_limbs(char *X, int chunks, double norm) {
 }
 
 // the results, f32 in X, to where they belong
-template <typename T, bool MUON, bool TALL>
+template <typename T, bool MUON, bool TALL, int MT>
 __device__ __forceinline__ void og_deliver(const OrthoGroup &g, int j0, int chunks, const OrthoPtr &ptr, const char *X, float decay) {
   const __amdgpu_buffer_rsrc_t out = og_buffer(ptr.out, g.rows * g.cols * (int)sizeof(T));
-  OgWalk<TALL> w(g, j0, chunks);
+  OgWalk<TALL, MT> w(g, j0, chunks);
+  constexpr int E = 8 * MT;
   for (int c = 0; c < chunks; c += 2, w.next()) {
-    float old[16];
+    float old[E];
     if constexpr (MUON)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) old[e] = og_get<float>(out, w.at(e));
+      for (int e = 0; e < E; ++e) old[e] = og_get<float>(out, w.at(e));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < E; ++e) {
       const float v = *reinterpret_cast<const float *>(X + w.lds(e));
       const int o = w.at(e);
       if constexpr (MUON) og_set(out, o, fmaf(-g.step, v, old[e] * decay));
@@ -842,7 +855,7 @@ __device__ __forceinline__ void og_deliver(const OrthoGroup &g, int j0, int chun
 }
 
 // this wave's 32 x 32 tile of Y Y^T, Y = `chunks` chunks at `in`, each chunk's operands requested a chunk ahead
-template <bool DIAG>
+template <bool DIAG, int MT>
 __device__ __forceinline__ void og_square_tile(const char *in, int chunks, int ti, int tj, float (&v)[16]) {
   const int l31 = threadIdx.x & 31;
   og_f16v acc, acx;
@@ -854,8 +867,8 @@ __device__ __forceinline__ void og_square_tile(const char *in, int chunks, int t
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        f[b][h][k] = og_frag(in + c * OG_CHUNK, ti + l31, h, k);
-        if constexpr (!DIAG) g[b][h][k] = og_frag(in + c * OG_CHUNK, tj + l31, h, k);
+        f[b][h][k] = og_frag(in + c * og_chunk(MT), ti + l31, h, k);
+        if constexpr (!DIAG) g[b][h][k] = og_frag(in + c * og_chunk(MT), tj + l31, h, k);
       }
   };
   auto multiply = [&](int b) {
@@ -875,26 +888,28 @@ __device__ __forceinline__ void og_square_tile(const char *in, int chunks, int t
 #pragma unroll
   for (int e = 0; e < 16; ++e) v[e] = acc[e] + acx[e];
 }
+template <int MT>
 __device__ __forceinline__ void og_square(const char *in, int chunks, int ti, int tj, float (&v)[16]) {
-  if (ti == tj) og_square_tile<true>(in, chunks, ti, tj, v);
-  else og_square_tile<false>(in, chunks, ti, tj, v);
+  if (MT == 1 || ti == tj) og_square_tile<true, MT>(in, chunks, ti, tj, v);
+  else og_square_tile<false, MT>(in, chunks, ti, tj, v);
 }
 
 // Q = a I + b A + c A A from the wave's tile v of A; A passes through Q's place.  Two barriers in between, none behind
-__device__ __forceinline__ void og_make_q(char *Q, int tiles, int ti, int tj, const float (&v)[16], const OrthoSmall &co) {
+template <int MT>
+__device__ __forceinline__ void og_make_q(char *Q, int ti, int tj, const float (&v)[16], const OrthoSmall &co) {
   const int l31 = threadIdx.x & 31, lh = (threadIdx.x >> 5) & 1;
-  const bool mine = tiles > 1 || threadIdx.x < 64;
+  const bool mine = MT > 1 || threadIdx.x < 64;
   auto put = [&](const float (&t)[16]) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float w[4] = {t[q * 4], t[q * 4 + 1], t[q * 4 + 2], t[q * 4 + 3]};
-      og_put(Q + (tj >> 5) * OG_CHUNK, ti + l31, q, w);
+      og_put(Q + (tj >> 5) * og_chunk(MT), ti + l31, q, w);
     }
   };
   if (mine) put(v);
   __syncthreads();
   float p[16];
-  if (mine) og_square(Q, tiles, ti, tj, p);
+  if (mine) og_square<MT>(Q, MT, ti, tj, p);
   __syncthreads();
   if (mine) {
 #pragma unroll
@@ -919,7 +934,7 @@ __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, flo
                              (const unsigned char *)chunk + og_unit(r + 4, u, k) + (lane & 1) * 8);
     }
   };
-  if (wave < chunks) load(X + wave * OG_CHUNK);
+  if (wave < chunks) load(X + wave * og_chunk(MT));
   __syncthreads();
   if (wave >= chunks) return;
 #pragma unroll
@@ -927,9 +942,9 @@ __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, flo
 #pragma unroll
     for (int f = 0; f < MT; ++f)
 #pragma unroll
-      for (int k = 0; k < 3; ++k) qf[h][f][k] = og_frag(Q + (h >> 1) * OG_CHUNK, f * 32 + l31, h & 1, k);
+      for (int k = 0; k < 3; ++k) qf[h][f][k] = og_frag(Q + (h >> 1) * og_chunk(MT), f * 32 + l31, h & 1, k);
   for (int ch = wave; ch < chunks; ch += 4) {
-    char *chunk = X + ch * OG_CHUNK;
+    char *chunk = X + ch * og_chunk(MT);
     og_f16v acc[MT], acx[MT];
 #pragma unroll
     for (int f = 0; f < MT; ++f)
@@ -939,7 +954,7 @@ __device__ __forceinline__ void og_apply(const char *Q, char *X, int chunks, flo
     for (int h = 0; h < 2 * MT; ++h)
 #pragma unroll
       for (int f = 0; f < MT; ++f) og_multiply(x[h], qf[h][f], acc[f], acx[f]);
-    if (ch + 4 < chunks) load(chunk + 4 * OG_CHUNK);
+    if (ch + 4 < chunks) load(chunk + 4 * og_chunk(MT));
 #pragma unroll
     for (int f = 0; f < MT; ++f) og_settle(acc[f], acx[f]);
 #pragma unroll
@@ -992,21 +1007,21 @@ __device__ __forceinline__ OrthoPtr og_small_ptr(const OrthoSmall &c, const Orth
 template <typename T, bool MUON, int MT>
 __device__ __forceinline__ void ortho_alone(const OrthoSmall &c, const OrthoGroup &g, const OrthoPtr &ptr, char *smem, double *red) {
   const int chunks = (og_long(g) + 31) / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  char *Q = smem, *X = smem + 2 * OG_CHUNK;
+  char *Q = smem, *X = smem + MT * og_chunk(MT);
   const bool tall = g.rows > g.cols;
-  const double sum = tall ? og_fetch<T, MUON, true>(g, 0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false>(g, 0, chunks, ptr, c.mo, X);
+  const double sum = tall ? og_fetch<T, MUON, true, MT>(g, 0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false, MT>(g, 0, chunks, ptr, c.mo, X);
   og_limbs<MT>(X, chunks, sqrt(og_block_sum(sum, red)) + (double)c.eps);
   const int ti = MT > 1 ? (wave >> 1) * 32 : 0, tj = MT > 1 ? (wave & 1) * 32 : 0;          // this wave's tile of A and Q
   for (int k = 0; k < c.steps; ++k) {
     float v[16];
     __syncthreads();
-    if (MT > 1 || wave == 0) og_square(X, chunks, ti, tj, v);
-    og_make_q(Q, MT, ti, tj, v, c);
+    if (MT > 1 || wave == 0) og_square<MT>(X, chunks, ti, tj, v);
+    og_make_q<MT>(Q, ti, tj, v, c);
     og_apply<MT>(Q, X, chunks, 1.f, k + 1 == c.steps);
   }
   __syncthreads();
-  if (tall) og_deliver<T, MUON, true>(g, 0, chunks, ptr, X, c.decay);
-  else og_deliver<T, MUON, false>(g, 0, chunks, ptr, X, c.decay);
+  if (tall) og_deliver<T, MUON, true, MT>(g, 0, chunks, ptr, X, c.decay);
+  else og_deliver<T, MUON, false, MT>(g, 0, chunks, ptr, X, c.decay);
 }
 
 template <typename T, bool MUON>
@@ -1016,10 +1031,12 @@ __global__ __launch_bounds__(256, 2) void ortho_small_kernel(OrthoSmall c) {
   int grp;
   const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
   const OrthoPtr ptr = og_small_ptr(c, g, blockIdx.x - g.first, sizeof(T));
-  if (og_short(g) <= 32) ortho_alone<T, MUON, 1>(c, g, ptr, smem, red);
+  if (og_mt(g) == 1) ortho_alone<T, MUON, 1>(c, g, ptr, smem, red);
   else ortho_alone<T, MUON, 2>(c, g, ptr, smem, red);
 }
 
+// LDS of a workgroup that keeps `chunks` chunks of X: A or Q, and an even number of chunks (OgWalk goes over 64 columns at a time)
+static inline int og_small_lds(const OrthoGroup &g, int chunks) { return (og_mt(g) + (chunks + 1) / 2 * 2) * og_chunk(og_mt(g)); }
 __host__ __device__ static inline int og_panels(const OrthoGroup &g) { return ((og_long(g) + 31) / 32 + g.jobs - 1) / g.jobs; }
 
 // Launch k of a chain of panels: k = 0 forms X0's panel and its share of the first Gram matrix, launch k > 0 takes step k - 1.  X's
@@ -1030,26 +1047,26 @@ template <typename T, bool MUON, int MT>
 __device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGroup &g, char *ws, double *sums, int k, char *smem, double *red) {
   const int panels = og_panels(g), wide = g.jobs, mat = og_div(blockIdx.x - g.first, panels), pan = blockIdx.x - g.first - mat * panels;
   const int all = (og_long(g) + 31) / 32, chunks = all - pan * wide < wide ? all - pan * wide : wide;
-  char *Q = smem, *X = smem + 2 * OG_CHUNK;
+  char *Q = smem, *X = smem + MT * og_chunk(MT);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ti = MT > 1 ? (wave >> 1) * 32 : 0, tj = MT > 1 ? (wave & 1) * 32 : 0;
   const bool square = MT > 1 || wave == 0;
   const OrthoPtr ptr = og_small_ptr(c, g, mat, sizeof(T));
   const bool tall = g.rows > g.cols;
   const int j0 = pan * wide * 32;
-  char *mine = ws + (size_t)g.x_off * 256 + ((size_t)mat * all + pan * wide) * OG_CHUNK;
+  char *mine = ws + (size_t)g.x_off * 256 + ((size_t)mat * all + pan * wide) * og_chunk(MT);
   og_f4 *share = reinterpret_cast<og_f4 *>(ws + (size_t)g.p_off * 256);                       // [set][mat][panel][q][thread]
   const size_t set = (size_t)g.count * panels * 1024;
   float v[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) v[e] = 0.f;
   if (k == 0) {
-    const double part = tall ? og_fetch<T, MUON, true>(g, j0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false>(g, j0, chunks, ptr, c.mo, X);
+    const double part = tall ? og_fetch<T, MUON, true, MT>(g, j0, chunks, ptr, c.mo, X) : og_fetch<T, MUON, false, MT>(g, j0, chunks, ptr, c.mo, X);
     const double sum = og_block_sum(part, red);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
     og_limbs<MT>(X, chunks, sum == 0. ? 1. : sqrt(sum));
   } else {
-    for (int t = threadIdx.x; t < chunks * (OG_CHUNK / 16); t += 256)
+    for (int t = threadIdx.x; t < chunks * (og_chunk(MT) / 16); t += 256)
       reinterpret_cast<og_b8 *>(X)[t] = reinterpret_cast<const og_b8 *>(mine)[t];
     const og_f4 *p = share + ((k - 1) & 1) * set + (size_t)mat * panels * 1024 + threadIdx.x;
     float own = 1.f;
@@ -1079,22 +1096,22 @@ __device__ __forceinline__ void ortho_panel(const OrthoSmall &c, const OrthoGrou
     };
     if (square && k == 1) gather([&](int z) { return weight[z]; });
     else if (square) gather([](int) { return 1.f; });
-    og_make_q(Q, MT, ti, tj, v, c);
+    og_make_q<MT>(Q, ti, tj, v, c);
     og_apply<MT>(Q, X, chunks, own, k == c.steps);
   }
   __syncthreads();
   if (k == c.steps) {
-    if (tall) og_deliver<T, MUON, true>(g, j0, chunks, ptr, X, c.decay);
-    else og_deliver<T, MUON, false>(g, j0, chunks, ptr, X, c.decay);
+    if (tall) og_deliver<T, MUON, true, MT>(g, j0, chunks, ptr, X, c.decay);
+    else og_deliver<T, MUON, false, MT>(g, j0, chunks, ptr, X, c.decay);
     return;
   }
   if (square) {
-    og_square(X, chunks, ti, tj, v);
+    og_square<MT>(X, chunks, ti, tj, v);
     og_f4 *o = share + (k & 1) * set + ((size_t)mat * panels + pan) * 1024 + threadIdx.x;
 #pragma unroll
     for (int q = 0; q < 4; ++q) o[q * 256] = og_f4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
   }
-  for (int t = threadIdx.x; t < chunks * (OG_CHUNK / 16); t += 256) reinterpret_cast<og_b8 *>(mine)[t] = reinterpret_cast<const og_b8 *>(X)[t];
+  for (int t = threadIdx.x; t < chunks * (og_chunk(MT) / 16); t += 256) reinterpret_cast<og_b8 *>(mine)[t] = reinterpret_cast<const og_b8 *>(X)[t];
 }
 
 template <typename T, bool MUON>
@@ -1103,7 +1120,7 @@ __global__ __launch_bounds__(256, 2) void ortho_panel_kernel(OrthoSmall c, char 
   __shared__ double red[16 + ORTHO_PANELS / 2];
   int grp;
   const OrthoGroup g = ortho_group_of(c.gs, blockIdx.x, grp);
-  if (og_short(g) <= 32) ortho_panel<T, MUON, 1>(c, g, ws, sums, k, smem, red);
+  if (og_mt(g) == 1) ortho_panel<T, MUON, 1>(c, g, ws, sums, k, smem, red);
   else ortho_panel<T, MUON, 2>(c, g, ws, sums, k, smem, red);
 }
 
@@ -1243,7 +1260,7 @@ struct OrthoLayout {
 // Widths of the panels (g[i].jobs): the smallest from ORTHO_WIDE chunks on that leaves the pass no more workgroups than CUs and no
 // matrix more than ORTHO_PANELS panels.  False if there is none.
 static bool ortho_panel_chunks(OrthoGroup *g, int n) {
-  for (int w = ORTHO_WIDE; w <= ORTHO_SMALL_N / 32; ++w) {
+  for (int w = ORTHO_WIDE; w <= ORTHO_WIDEST; ++w) {
     long blocks = 0, most = 0;
     for (int i = 0; i < n; ++i) {
       g[i].jobs = w;
@@ -1261,17 +1278,15 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
   OrthoLayout lo;
   memset(&lo, 0, sizeof lo);
   lo.sums = align_up(sizeof(OrthoPtr) * ORTHO_MATRICES, 256);
-  lo.panels = true;
-  int most = 0;
+  lo.small = lo.panels = true;
   for (int i = 0; i < n; ++i) {
     lo.chain[i] = 1;
     lo.norm_first[i] = lo.norm_blocks;
     lo.norm_blocks += g[i].count * og_norm_blocks(g[i]);
-    if (og_long(g[i]) > most) most = og_long(g[i]);
     lo.panels = lo.panels && og_short(g[i]) <= ORTHO_SMALL_M;
+    lo.small = lo.small && lo.panels && og_small_lds(g[i], (og_long(g[i]) + 31) / 32) <= ORTHO_SMALL_LDS;
   }
   size_t at = lo.sums + align_up(lo.norm_blocks * sizeof(double), 256);
-  lo.small = lo.panels && most <= ORTHO_SMALL_N;
   lo.panels = lo.panels && !lo.small && ortho_panel_chunks(g, n);
   if (lo.small) {
     lo.bytes = lo.sums;
@@ -1283,7 +1298,7 @@ static OrthoLayout ortho_layout(OrthoGroup *g, int n, int steps) {
     at = lo.sums + align_up(blocks * sizeof(double), 256);
     for (int i = 0; i < n; ++i) {
       g[i].x_off = (unsigned)(at / 256);
-      at += (size_t)g[i].count * ((og_long(g[i]) + 31) / 32) * OG_CHUNK;
+      at += (size_t)g[i].count * ((og_long(g[i]) + 31) / 32) * og_chunk(og_mt(g[i]));
       g[i].p_off = (unsigned)(at / 256);
       at += (size_t)g[i].count * og_panels(g[i]) * 2 * 16384;
     }
@@ -1358,18 +1373,17 @@ static int ortho_run(OrthoGroup *g, int n, const OrthoPtr &base, const OrthoPtr 
     sm.c = c.c;
     sm.decay = c.decay;
     sm.eps = c.eps;
-    int blocks = 0, most = 0;                                            // most: chunks that a workgroup keeps in LDS
+    int blocks = 0, lds = 0;
     for (int i = 0; i < n; ++i) {
       const int chunks = (og_long(g[i]) + 31) / 32, kept = lo.panels && g[i].jobs < chunks ? g[i].jobs : chunks;
       sm.gs.g[i].first = blocks;
       blocks += lo.panels ? g[i].count * og_panels(g[i]) : g[i].count;
-      if (kept > most) most = kept;
+      if (og_small_lds(g[i], kept) > lds) lds = og_small_lds(g[i], kept);
     }
-    const int lds = 2 * OG_CHUNK + (most + 1) / 2 * 2 * OG_CHUNK;         // (og_fetch's padding: an even number of chunks)
 #define ORTHO_SMALL(T, MUON)                                                                                                            \
   do {                                                                                                                                  \
     const void *fn = lo.small ? reinterpret_cast<const void *>(&ortho_small_kernel<T, MUON>) : reinterpret_cast<const void *>(&ortho_panel_kernel<T, MUON>); \
-    if (const int rc = lds_optin(fn, (2 + ORTHO_SMALL_N / 32) * OG_CHUNK, "ortho_small_kernel")) return rc;                               \
+    if (const int rc = lds_optin(fn, ORTHO_SMALL_LDS, "ortho_small_kernel")) return rc;                               \
     if (lo.small) {                                                                                                                     \
       hipLaunchKernelGGL((ortho_small_kernel<T, MUON>), dim3(blocks), dim3(256), lds, st, sm);                                          \
     } else {                                                                                                                            \

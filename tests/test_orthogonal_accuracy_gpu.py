@@ -139,7 +139,7 @@ def gradients(count, rows, cols, seed=0):
     # one workgroup: short sides on both sides of 32, up to 320 columns; panels of several widths; products: few tiles and many, split
     # reductions, chains of one, two and three steps, 64- and 128-wide tiles
     (3, 20, 50), (1, 50, 108), (2, 31, 33), (2, 64, 64), (2, 33, 319), (2, 320, 64), (300, 40, 300), (2, 64, 321), (1, 20, 8192), (3, 50, 1000),
-    (2, 9000, 33), (40, 64, 576), (25, 64, 640), (70, 64, 448), (1, 65, 63), (1, 65, 700), (2, 130, 65), (4, 128, 576), (5, 100, 333), (1, 333, 1021),
+    (2, 9000, 33), (1, 32, 700), (3, 31, 704), (2, 705, 32), (2, 700, 20), (300, 30, 400), (5, 7, 321), (40, 64, 576), (25, 64, 640), (70, 64, 448), (1, 65, 63), (1, 65, 700), (2, 130, 65), (4, 128, 576), (5, 100, 333), (1, 333, 1021),
     (1, 200, 4000), (2, 256, 256), (1, 257, 700), (20, 448, 1000), (20, 200, 1000), (8, 256, 2304), (40, 520, 600), (1, 1024, 1100), (4, 1030, 1030)])
 def test_as_accurate_as_f32(count, rows, cols):
     from lsps_amd import ops
